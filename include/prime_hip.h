@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define PRIME_HIP_ABI_VERSION 2
+#define PRIME_HIP_ABI_VERSION 3
 
 #define PRIME_EINVAL (-1)   /* null pointer, negative size, bad n_bins ... */
 #define PRIME_EWORKSPACE (-2) /* workspace missing, too small or not initialised */
@@ -339,6 +339,71 @@ int prime_outer_sgd_nesterov_f32_segmented(float* const* params, float* const* m
                                            const float* const* grads, float* const* inner_outs,
                                            const int64_t* ns, int64_t count, float lr, float momentum,
                                            int first_step, prime_stream_t stream);
+
+/* ---- low-bit operators of the model's own step (forward and backward, between two outer steps) ----
+ * Element types of their operands. */
+#define PRIME_F32 0
+#define PRIME_BF16 1
+#define PRIME_F16 2
+#define PRIME_I8 3
+#define PRIME_F8E4M3 4
+
+/* Root-mean-square norm of `rows` rows of `dim` elements, after the residual's addition if there is one, as 8-bit
+ * codes with one scale per row:
+ *   h = x + residual, rounded to `type` and stored to `hidden` (dense), or x without a residual (both pointers NULL)
+ *   z = h * weight rounded to fp32;  s = max |z| / 127 (PRIME_I8) or / 448 (PRIME_F8E4M3), rounded to fp32
+ *   codes (dense) = the int8 or e4m3 number nearest z / s, ties to even, exactly (not above 127 or 448 in magnitude)
+ *   inv_rms = 1 / sqrt(mean h^2 + eps);  scales = s * inv_rms
+ * so that codes * scales stands for h * inv_rms * weight.  The norm that this replaces in training is
+ * src/zeroband/models/norms.py:128 (in the input's precision, no residual, no codes).
+ * A row that holds a value that is not finite, or one whose product with the weight is not, gets scale NaN and codes 0.
+ * type: PRIME_F32, PRIME_BF16 or PRIME_F16 (x, residual, hidden); weight_type: the same or PRIME_F32.  Strides are in
+ * elements from row to row (0 repeats a row); within a row elements are consecutive.  1 <= dim <= 2^30.  scales and
+ * inv_rms have `rows` entries.  Outputs must not overlap inputs. */
+int prime_rms_norm_quantize(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                            const void* weight, int64_t rows, int64_t dim, int type, int weight_type,
+                            int code_type, double eps, void* codes, float* scales, void* hidden,
+                            float* inv_rms, prime_stream_t stream);
+
+/* Its gradients, straight through the rounding to codes: with grad the gradient of what the codes stand for and
+ * grad_hidden (optional) that of the stored sum,
+ *   n = hidden * inv_rms,  u = grad * weight
+ *   grad_x = inv_rms * (u - n * mean(u * n)) + grad_hidden      (dense; x and the residual both receive it)
+ *   grad_weight = sum over rows of grad * n                     (weight_type; zeros when rows is 0)
+ * (src/zeroband/models/norms.py:176).  hidden is the forward's `hidden`, or its x without a residual.  scratch: at
+ * least prime_rms_norm_backward_scratch_bytes(rows, dim) bytes of device memory, 4-byte aligned, whatever it holds;
+ * calls that share it must be ordered on one stream.  Sums are taken in an order that depends on rows, dim and
+ * the device alone. */
+int64_t prime_rms_norm_backward_scratch_bytes(int64_t rows, int64_t dim);
+int prime_rms_norm_quantize_backward(const void* grad, int64_t grad_stride, const void* hidden, int64_t hidden_stride,
+                                     const void* weight, const float* inv_rms, const void* grad_hidden,
+                                     int64_t grad_hidden_stride, int64_t rows, int64_t dim, int type, int weight_type,
+                                     void* grad_x, void* grad_weight, void* scratch, int64_t scratch_bytes,
+                                     prime_stream_t stream);
+
+/* A matrix of n rows of k weights as 4-bit codes with a scale per group of 32, 64 or 128 consecutive weights of a row:
+ *   s = max |w| / 7 rounded to fp32, then to scale_type (PRIME_F32 or PRIME_BF16)
+ *   code = the integer nearest w / s, ties to even, exactly, within -7 .. 7
+ * A row of `packed` is ceil(k / group) * group / 2 bytes, the even element in a byte's lower half, two's complement;
+ * codes behind the row's end are 0.  scales has ceil(k / group) entries a row.  Both dense.  A group
+ * that holds a value that is not finite gets scale NaN and codes 0.  No counterpart in the reference. */
+int prime_quantize_4bit(const void* weight, int64_t stride, int64_t n, int64_t k, int type, int group, int scale_type,
+                        uint8_t* packed, void* scales, prime_stream_t stream);
+
+/* out[i][j] = code * scale in 32 bits, rounded to out_type (dense rows of k).  packed_stride is in bytes, scale_stride in
+ * elements from row to row.  Codes are any of -8 .. 7. */
+int prime_dequantize_4bit(const uint8_t* packed, int64_t packed_stride, const void* scales, int64_t scale_stride,
+                          int64_t n, int64_t k, int group, int scale_type, void* out, int out_type,
+                          prime_stream_t stream);
+
+/* Products of rows with such a matrix: out[m][i] = x_scales[m] * sum over groups of scale[i][g] * sum over the
+ * group's j of code[i][j] * x[m][j], rounded once to out_type (dense rows of n).  x: PRIME_F32, PRIME_BF16 or PRIME_F16
+ * rows (x_scales NULL), or PRIME_I8 codes with a scale per row, as prime_rms_norm_quantize gives them: the
+ * sums within a group are then exact.  Meant for the few rows of a decoding step; many rows (hundreds) are better
+ * served by prime_dequantize_4bit and a library product. */
+int prime_matvec_4bit(const void* x, int64_t x_stride, int x_type, const float* x_scales, const uint8_t* packed,
+                      int64_t packed_stride, const void* scales, int64_t scale_stride, int64_t rows, int64_t n,
+                      int64_t k, int group, int scale_type, void* out, int out_type, prime_stream_t stream);
 
 /* A plain device copy of n bytes (16-byte vectors): the yardstick the profiler's byte
  * counters are scaled against.  No counterpart in the reference. */

@@ -10,7 +10,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "csrc" / "libprime_hip.so"
 
-ABI_VERSION = 2
+ABI_VERSION = 3
 
 
 class QParams(ctypes.Structure):
@@ -43,6 +43,8 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
+_int = ctypes.c_int
 
 # name -> (restype, argtypes); every symbol include/prime_hip.h declares
 SIGNATURES = {
@@ -81,6 +83,12 @@ SIGNATURES = {
     "prime_outer_sgd_nesterov_u8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _f32, _f32, ctypes.c_int, _vp]),
     "prime_pseudo_gradient_f32_segmented": (ctypes.c_int, [_vp, _vp, _vp, _i64, _f32, _vp, _vp]),
     "prime_outer_sgd_nesterov_f32_segmented": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _f32, _f32, ctypes.c_int, _vp]),
+    "prime_rms_norm_quantize": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _int, _int, _int, _f64, _vp, _vp, _vp, _vp, _vp]),
+    "prime_rms_norm_backward_scratch_bytes": (_i64, [_i64, _i64]),
+    "prime_rms_norm_quantize_backward": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _i64, _vp]),
+    "prime_quantize_4bit": (_int, [_vp, _i64, _i64, _i64, _int, _int, _int, _vp, _vp, _vp]),
+    "prime_dequantize_4bit": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _int, _int, _vp, _int, _vp]),
+    "prime_matvec_4bit": (_int, [_vp, _i64, _int, _vp, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _int, _int, _vp, _int, _vp]),
     "prime_copy_bytes": (ctypes.c_int, [_vp, _vp, _i64, _vp]),
 }
 

@@ -1,0 +1,230 @@
+// C entry points of the low-bit operators (kernels_norm.h, kernels_lowbit.h): argument checks, choice of the kernel,
+// launch.
+//
+// Included by prime_hip.hip behind its other host code; not a translation unit of its own.
+
+namespace {
+
+// Calls f with a value of the element type; false: not a type of this operand.
+template <typename F>
+bool with_float_type(int type, F&& f) {
+    if (type == PRIME_F32) f(float{});
+    else if (type == PRIME_BF16) f(__bf16{});
+    else if (type == PRIME_F16) f(_Float16{});
+    else return false;
+    return true;
+}
+bool is_float_type(int type) { return type == PRIME_F32 || type == PRIME_BF16 || type == PRIME_F16; }
+bool is_scale_type(int type) { return type == PRIME_F32 || type == PRIME_BF16; }
+int type_bytes(int type) { return type == PRIME_F32 ? 4 : type == PRIME_I8 || type == PRIME_F8E4M3 ? 1 : 2; }
+template <typename F>
+void with_scale_type(int type, F&& f) {
+    if (type == PRIME_F32) f(float{});
+    else f(__bf16{});
+}
+// A norm's weight has the rows' type or fp32.
+template <typename XT, typename F>
+void with_weight_type(int weight_type, int type, F&& f) {
+    if (weight_type == type) f(XT{});
+    else f(float{});
+}
+
+constexpr int64_t kMaxDim = int64_t(1) << 30;
+constexpr int64_t kRowsPerLaunch = int64_t(1) << 21;    // a dispatch counts its work-items in 32 bits: 1024 a row at most
+
+template <typename XT, typename WT>
+void launch_rms_norm(const NormArgs& a, double bytes, hipStream_t st) {
+    const int64_t r = a.rows;
+    const int quads = static_cast<int>((r + 3) / 4), all = static_cast<int>(r);
+    if (a.dim <= 512) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 64, 1>, quads, 256, st, a);
+    else if (a.dim <= 1024) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 64, 2>, quads, 256, st, a);
+    else if (a.dim <= 2048) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 256, 1>, all, 256, st, a);
+    else if (a.dim <= 4096) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 256, 2>, all, 256, st, a);
+    else if (a.dim <= 8192) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 512, 2>, all, 512, st, a);
+    else if (a.dim <= 16384) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 1024, 2>, all, 1024, st, a);
+    else launch(kIdRmsNorm, bytes, rms_norm_loop_kernel<XT, WT>, all, 1024, st, a);
+}
+
+// Workgroups (= partial rows of the weight's gradient) of the backward pass, and its scratch.
+constexpr int kGradRegisterDim = 16384;      // rows up to this long stay in registers
+int grad_lanes(int64_t dim) { return dim <= 1024 ? 64 : dim <= 2048 ? 128 : dim <= 4096 ? 256 : dim <= 8192 ? 512 : 1024; }
+int grad_stretches(int64_t dim) { return static_cast<int>((dim + 2047) / 2048); }
+int64_t grad_groups(int64_t rows, int64_t dim) {
+    int64_t most = dim <= kGradRegisterDim ? static_cast<int64_t>(cu_count()) * (1024 / grad_lanes(dim))
+                                           : static_cast<int64_t>(cu_count()) * 8 / grad_stretches(dim);
+    if (most < 1) most = 1;
+    return rows < most ? rows : most;
+}
+int64_t grad_scratch_bytes(int64_t rows, int64_t dim) {
+    return grad_groups(rows, dim) * dim * 4 + (dim > kGradRegisterDim ? rows * 4 : 0);
+}
+
+template <typename XT, typename WT>
+void launch_rms_norm_grad(const NormGradArgs& a, int groups, WT* grad_weight, double bytes, hipStream_t st) {
+    if (a.rows > 0) {
+        if (a.dim <= 512) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 64, 1>, groups, 64, st, a);
+        else if (a.dim <= 1024) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 64, 2>, groups, 64, st, a);
+        else if (a.dim <= 2048) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 128, 2>, groups, 128, st, a);
+        else if (a.dim <= 4096) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 256, 2>, groups, 256, st, a);
+        else if (a.dim <= 8192) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 512, 2>, groups, 512, st, a);
+        else if (a.dim <= kGradRegisterDim) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 1024, 2>, groups, 1024, st, a);
+        else {
+            float* dots = a.partials + static_cast<int64_t>(groups) * a.dim;
+            for (int64_t at = 0; at < a.rows; at += kRowsPerLaunch) {
+                NormGradArgs part = a;
+                part.rows = std::min(a.rows - at, kRowsPerLaunch);
+                part.grad = static_cast<const XT*>(a.grad) + at * a.g_stride;
+                part.hidden = static_cast<const XT*>(a.hidden) + at * a.h_stride;
+                part.inv_rms = a.inv_rms + at;
+                launch(kIdRmsNormGrad, bytes, rms_norm_grad_dot_kernel<XT, WT>, static_cast<int>(part.rows), 1024, st, part, dots + at);
+            }
+            const int stretches = grad_stretches(a.dim);
+            launch(kIdRmsNormGrad, bytes, rms_norm_grad_apply_kernel<XT, WT>, stretches * groups, 256, st, a, dots, stretches, groups);
+        }
+    }
+    launch(kIdColumnSum, 4.0 * groups * a.dim, column_sum_kernel<WT>, static_cast<int>((a.dim + 15) / 16), 256, st, a.partials, groups, a.dim, grad_weight);
+}
+
+bool bad_group(int group) { return group != 32 && group != 64 && group != 128; }
+bool bad_matrix(int64_t n, int64_t k) { return n < 0 || n >= (int64_t(1) << 40) || k < 1 || k > kMaxDim; }
+int group_shift(int group) { return group == 32 ? 5 : group == 64 ? 6 : 7; }
+
+}  // namespace
+
+extern "C" {
+
+int prime_rms_norm_quantize(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int64_t rows,
+                            int64_t dim, int type, int weight_type, int code_type, double eps, void* codes, float* scales, void* hidden,
+                            float* inv_rms, prime_stream_t stream) {
+    if (rows < 0 || rows > kMaxElems || dim < 1 || dim > kMaxDim || x_stride < 0 || residual_stride < 0)
+        return fail(PRIME_EINVAL, "prime_rms_norm_quantize: bad size");
+    if (!is_float_type(type) || (weight_type != type && weight_type != PRIME_F32) || (code_type != PRIME_I8 && code_type != PRIME_F8E4M3))
+        return fail(PRIME_EINVAL, "prime_rms_norm_quantize: bad type");
+    if (!(eps >= 0.0)) return fail(PRIME_EINVAL, "prime_rms_norm_quantize: eps must not be negative");
+    if (rows == 0) return 0;
+    if (!x || !weight || !codes || !scales || !inv_rms || (residual == nullptr) != (hidden == nullptr))
+        return fail(PRIME_EINVAL, "prime_rms_norm_quantize: null operand");
+    const double row_bytes = static_cast<double>(dim) * (type_bytes(type) * (residual ? 3 : 1) + 1) + 8.0;
+    for (int64_t at = 0; at < rows; at += kRowsPerLaunch) {
+        const int64_t part = std::min(rows - at, kRowsPerLaunch);
+        with_float_type(type, [&](auto t) {
+            using XT = decltype(t);
+            NormArgs a{static_cast<const XT*>(x) + at * x_stride, residual ? static_cast<const XT*>(residual) + at * residual_stride : nullptr, weight,
+                       hidden ? static_cast<XT*>(hidden) + at * dim : nullptr, static_cast<uint8_t*>(codes) + at * dim, scales + at, inv_rms + at,
+                       x_stride, residual_stride, part, static_cast<int>(dim), code_type == PRIME_F8E4M3, eps};
+            with_weight_type<XT>(weight_type, type, [&](auto w) { launch_rms_norm<XT, decltype(w)>(a, row_bytes * part, static_cast<hipStream_t>(stream)); });
+        });
+        if (int rc = launch_check("rms_norm_row_kernel")) return rc;
+    }
+    return 0;
+}
+
+int64_t prime_rms_norm_backward_scratch_bytes(int64_t rows, int64_t dim) {
+    if (rows < 0 || rows > kMaxElems || dim < 1 || dim > kMaxDim) return PRIME_EINVAL;
+    return grad_scratch_bytes(rows, dim);
+}
+
+int prime_rms_norm_quantize_backward(const void* grad, int64_t grad_stride, const void* hidden, int64_t hidden_stride, const void* weight,
+                                     const float* inv_rms, const void* grad_hidden, int64_t grad_hidden_stride, int64_t rows, int64_t dim,
+                                     int type, int weight_type, void* grad_x, void* grad_weight, void* scratch, int64_t scratch_bytes,
+                                     prime_stream_t stream) {
+    if (rows < 0 || rows > kMaxElems || dim < 1 || dim > kMaxDim || grad_stride < 0 || hidden_stride < 0 || grad_hidden_stride < 0)
+        return fail(PRIME_EINVAL, "prime_rms_norm_quantize_backward: bad size");
+    if (!is_float_type(type) || (weight_type != type && weight_type != PRIME_F32))
+        return fail(PRIME_EINVAL, "prime_rms_norm_quantize_backward: bad type");
+    if (!weight || !grad_weight || (rows > 0 && (!grad || !hidden || !inv_rms || !grad_x)))
+        return fail(PRIME_EINVAL, "prime_rms_norm_quantize_backward: null operand");
+    if (rows > 0 && (!scratch || scratch_bytes < grad_scratch_bytes(rows, dim) || !aligned_to(scratch, 4)))
+        return fail(PRIME_EWORKSPACE, "prime_rms_norm_quantize_backward: scratch missing, too small or not aligned");
+    const double bytes = static_cast<double>(rows) * dim * type_bytes(type) * (grad_hidden ? 4 : 3);
+    with_float_type(type, [&](auto t) {
+        using XT = decltype(t);
+        NormGradArgs a{grad, hidden, weight, inv_rms, grad_hidden, grad_x, static_cast<float*>(scratch), grad_stride, hidden_stride, grad_hidden_stride,
+                       rows, static_cast<int>(dim)};
+        with_weight_type<XT>(weight_type, type, [&](auto w) {
+            launch_rms_norm_grad<XT>(a, static_cast<int>(grad_groups(rows, dim)), static_cast<decltype(w)*>(grad_weight), bytes, static_cast<hipStream_t>(stream));
+        });
+    });
+    return launch_check("rms_norm_grad_kernel");
+}
+
+int prime_quantize_4bit(const void* weight, int64_t stride, int64_t n, int64_t k, int type, int group, int scale_type, uint8_t* packed,
+                        void* scales, prime_stream_t stream) {
+    if (bad_matrix(n, k) || stride < 0) return fail(PRIME_EINVAL, "prime_quantize_4bit: bad size");
+    if (!is_float_type(type) || !is_scale_type(scale_type)) return fail(PRIME_EINVAL, "prime_quantize_4bit: bad type");
+    if (bad_group(group)) return fail(PRIME_EINVAL, "prime_quantize_4bit: group must be 32, 64 or 128");
+    if (n == 0) return 0;
+    if (!weight || !packed || !scales) return fail(PRIME_EINVAL, "prime_quantize_4bit: null operand");
+    const int64_t groups = (k + group - 1) / group, eights = groups * group / 8;
+    const int64_t step = std::max<int64_t>(1, ((int64_t(1) << 30) - 1) / eights);      // rows a launch: indexes in 31 bits
+    for (int64_t at = 0; at < n; at += step) {
+        const int64_t rows = std::min(n - at, step), vectors = rows * eights;
+        with_float_type(type, [&](auto t) {
+            using T = decltype(t);
+            with_scale_type(scale_type, [&](auto s) {
+                using ST = decltype(s);
+                PackArgs a{static_cast<const T*>(weight) + at * stride, stride, packed + at * eights * 4, static_cast<ST*>(scales) + at * groups,
+                           static_cast<uint32_t>(vectors), static_cast<int>(k), group / 8, FastDiv(static_cast<uint32_t>(eights))};
+                launch(kIdGroupPack, static_cast<double>(rows) * (k * sizeof(T) + eights * 4 + groups * sizeof(ST)), group4_pack_kernel<T, ST>,
+                       static_cast<int>((vectors + 255) / 256), 256, static_cast<hipStream_t>(stream), a);
+            });
+        });
+        if (int rc = launch_check("group4_pack_kernel")) return rc;
+    }
+    return 0;
+}
+
+int prime_dequantize_4bit(const uint8_t* packed, int64_t packed_stride, const void* scales, int64_t scale_stride, int64_t n, int64_t k,
+                          int group, int scale_type, void* out, int out_type, prime_stream_t stream) {
+    if (bad_matrix(n, k) || packed_stride < 0 || scale_stride < 0) return fail(PRIME_EINVAL, "prime_dequantize_4bit: bad size");
+    if (!is_float_type(out_type) || !is_scale_type(scale_type)) return fail(PRIME_EINVAL, "prime_dequantize_4bit: bad type");
+    if (bad_group(group)) return fail(PRIME_EINVAL, "prime_dequantize_4bit: group must be 32, 64 or 128");
+    if (n == 0) return 0;
+    if (!packed || !scales || !out) return fail(PRIME_EINVAL, "prime_dequantize_4bit: null operand");
+    const int64_t eights = (k + 7) / 8, step = std::max<int64_t>(1, ((int64_t(1) << 30) - 1) / eights);
+    for (int64_t at = 0; at < n; at += step) {
+        const int64_t rows = std::min(n - at, step), vectors = rows * eights;
+        with_float_type(out_type, [&](auto t) {
+            using T = decltype(t);
+            with_scale_type(scale_type, [&](auto s) {
+                using ST = decltype(s);
+                UnpackArgs a{packed + at * packed_stride, static_cast<const ST*>(scales) + at * scale_stride, static_cast<T*>(out) + at * k, packed_stride,
+                             scale_stride, static_cast<uint32_t>(vectors), static_cast<int>(k), group_shift(group) - 3, FastDiv(static_cast<uint32_t>(eights))};
+                launch(kIdGroupUnpack, static_cast<double>(rows) * (k * (sizeof(T) + 0.5)), group4_unpack_kernel<T, ST>,
+                       static_cast<int>((vectors + 255) / 256), 256, static_cast<hipStream_t>(stream), a);
+            });
+        });
+        if (int rc = launch_check("group4_unpack_kernel")) return rc;
+    }
+    return 0;
+}
+
+int prime_matvec_4bit(const void* x, int64_t x_stride, int x_type, const float* x_scales, const uint8_t* packed, int64_t packed_stride,
+                      const void* scales, int64_t scale_stride, int64_t rows, int64_t n, int64_t k, int group, int scale_type, void* out,
+                      int out_type, prime_stream_t stream) {
+    if (bad_matrix(n, k) || n >= (int64_t(1) << 31) || rows < 0 || rows >= (int64_t(1) << 31) || x_stride < 0 || packed_stride < 0 || scale_stride < 0)
+        return fail(PRIME_EINVAL, "prime_matvec_4bit: bad size");
+    if ((!is_float_type(x_type) && x_type != PRIME_I8) || !is_float_type(out_type) || !is_scale_type(scale_type))
+        return fail(PRIME_EINVAL, "prime_matvec_4bit: bad type");
+    if (bad_group(group)) return fail(PRIME_EINVAL, "prime_matvec_4bit: group must be 32, 64 or 128");
+    if (n == 0 || rows == 0) return 0;
+    if (!x || !packed || !scales || !out || (x_type == PRIME_I8) != (x_scales != nullptr))
+        return fail(PRIME_EINVAL, "prime_matvec_4bit: null operand, or scales without int8 rows");
+    MatvecArgs a{x, x_scales, packed, scales, out, x_stride, packed_stride, scale_stride, static_cast<int>(rows), n, static_cast<int>(k), group_shift(group)};
+    const double bytes = static_cast<double>(n) * k / 2 + static_cast<double>(n) * ((k + group - 1) / group) * type_bytes(scale_type) +
+                         static_cast<double>(rows) * (k * type_bytes(x_type) + n * type_bytes(out_type));
+    with_scale_type(scale_type, [&](auto s) {
+        using ST = decltype(s);
+        with_float_type(out_type, [&](auto o) {
+            using OT = decltype(o);
+            auto go = [&](auto t) {
+                launch(kIdMatvec4, bytes, matvec4_kernel<decltype(t), ST, OT>, static_cast<int>((n + 3) / 4), 256, static_cast<hipStream_t>(stream), a);
+            };
+            if (x_type == PRIME_I8) go(int8_t{});
+            else with_float_type(x_type, go);
+        });
+    });
+    return launch_check("matvec4_kernel");
+}
+
+}  // extern "C"

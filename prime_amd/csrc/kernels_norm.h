@@ -1,0 +1,433 @@
+// Root-mean-square norm of rows with the residual's addition and an 8-bit output with one scale per row, and
+// the gradients of its input and weight.
+//
+//   h = x + r rounded to the rows' type (the stream as later blocks read it), or x itself
+//   z = fl32(h w),  a = max |z|,  s = fl32(a / top)          top = 127 (int8) or 448 (e4m3)
+//   code = the integer (e4m3 number) nearest z / s, ties to even
+//   inv = 1 / sqrt(sum h^2 / dim + eps),  scale = s inv      so that code * scale stands for h inv w
+//
+// The root mean square cancels out of the codes, so the sum of squares and the maximum are taken in one visit and
+// nothing waits for the other.  Codes are exact: see nearest_int().  Sums of squares are fp64 (a square of an fp32
+// value overflows fp32; at 8 bytes of traffic an element the fp64 additions cost nothing).
+// A row that holds a value that is not finite, or whose product with the weight is not, gets scale NaN and codes 0.
+//
+// Included by prime_hip.hip inside its anonymous namespace; not a translation unit of its own.
+
+// Eight consecutive elements of a row, at element alignment (a row of odd length starts anywhere).
+template <typename T> struct Eight;
+template <> struct Eight<float> { typedef float type __attribute__((ext_vector_type(8), aligned(4))); };
+template <> struct Eight<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2))); };
+template <> struct Eight<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(8), aligned(2))); };
+struct __attribute__((packed, aligned(1))) U64U { uint32_t lo, hi; };
+
+// Elements i .. i + 7 of a row of n as floats, zero behind its end.
+template <typename T>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int i, int n, float (&v)[8]) {
+    if (i + 8 <= n) {
+        const typename Eight<T>::type t = *reinterpret_cast<const typename Eight<T>::type*>(row + i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(t[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = i + e < n ? static_cast<float>(row[i + e]) : 0.0f;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* __restrict__ row, int i, int n, const float (&v)[8]) {
+    if (i + 8 <= n) {
+        typename Eight<T>::type t;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = static_cast<T>(v[e]);
+        *reinterpret_cast<typename Eight<T>::type*>(row + i) = t;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (i + e < n) row[i + e] = static_cast<T>(v[e]);
+    }
+}
+
+// Eight one-byte codes, lowest byte first.
+__device__ __forceinline__ void store8_codes(uint8_t* __restrict__ row, int i, int n, uint32_t lo, uint32_t hi) {
+    if (i + 8 <= n) {
+        *reinterpret_cast<U64U*>(row + i) = U64U{lo, hi};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (i + e < n) row[i + e] = static_cast<uint8_t>((e < 4 ? lo : hi) >> (8 * (e & 3)));
+    }
+}
+
+// The integer nearest z / unit, ties to even, for |z / unit| < 512, with r = 1 / unit rounded and unit normal.
+// t = z r is within 2^-23 |t| of the quotient, less than 2^-14, so away from a border rounding t is right.  Near one (one
+// element in ten thousand) the side is the sign of z - m unit with m the border, which a fused multiply-add
+// rounds once and therefore never gets wrong.
+__device__ __forceinline__ float nearest_int(float z, float unit, float r) {
+    const float t = z * r;
+    float k = __builtin_rintf(t);
+    const float d = t - k;
+    if (__builtin_fabsf(d) > 0.5f - 0x1p-14f) {
+        const float m = k + __builtin_copysignf(0.5f, d);
+        const float side = __builtin_fmaf(-m, unit, z);
+        k = side == 0.0f ? __builtin_rintf(m) : m + __builtin_copysignf(0.5f, side);
+    }
+    return k;
+}
+
+// int8 code of z under the scale s.
+__device__ __forceinline__ uint32_t code_int8(float z, float s, float r) {
+    const float k = __builtin_amdgcn_fmed3f(nearest_int(z, s, r), -127.0f, 127.0f);
+    return static_cast<uint32_t>(static_cast<int>(k)) & 0xffu;
+}
+
+// The e4m3 number nearest z / s, as a float: three mantissa bits, so the integer nearest z / (s step) in units of
+// step = 2^(e - 3), with e the quotient's exponent, not below -6 (subnormal numbers share the step 2^-9).
+__device__ __forceinline__ float value_e4m3(float z, float s, float r) {
+    const int e = max(static_cast<int>((__float_as_uint(z * r) >> 23) & 0xff), 127 - 6);
+    const float step = __uint_as_float(static_cast<uint32_t>(e - 3) << 23);
+    const float inv_step = __uint_as_float(static_cast<uint32_t>(254 - (e - 3)) << 23);
+    return __builtin_amdgcn_fmed3f(nearest_int(z, s * step, r * inv_step) * step, -448.0f, 448.0f);
+}
+
+// Codes of eight products, packed.
+template <bool FP8>
+__device__ __forceinline__ void codes8(const float (&z)[8], float s, float r, uint32_t& lo, uint32_t& hi) {
+    uint32_t w[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        if constexpr (FP8) {
+            // the values are e4m3 numbers: the conversion rounds nothing
+            int p = __builtin_amdgcn_cvt_pk_fp8_f32(value_e4m3(z[4 * q], s, r), value_e4m3(z[4 * q + 1], s, r), 0, false);
+            w[q] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(value_e4m3(z[4 * q + 2], s, r), value_e4m3(z[4 * q + 3], s, r), p, true));
+        } else {
+            w[q] = code_int8(z[4 * q], s, r) | code_int8(z[4 * q + 1], s, r) << 8 | code_int8(z[4 * q + 2], s, r) << 16 |
+                   code_int8(z[4 * q + 3], s, r) << 24;
+        }
+    }
+    lo = w[0];
+    hi = w[1];
+}
+
+// Sum over the lanes of a wavefront, the same value in every lane (a fixed butterfly).
+__device__ __forceinline__ double wave_sum_all(double v) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+    return v;
+}
+__device__ __forceinline__ float wave_sum_all(float v) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+    return v;
+}
+__device__ __forceinline__ uint32_t wave_max_all(uint32_t v) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, 64)));
+    return v;
+}
+
+struct NormArgs {
+    const void* x;
+    const void* residual;       // null: none, and hidden is null too
+    const void* weight;
+    void* hidden;
+    uint8_t* codes;
+    float* scales;
+    float* inv_rms;
+    int64_t x_stride, r_stride; // elements from row to row; outputs are dense
+    int64_t rows;
+    int dim;
+    int fp8;
+    double eps;
+};
+
+// What follows from a row's sum of squares and largest |z| (its bits: a NaN compares above all numbers).
+struct RowScale {
+    float s, r;                 // unit of the codes and its reciprocal, both of z * up
+    float up;                   // 1, or 2^64 where s is so small that its reciprocal or a residual could leave fp32's range
+    bool none;                  // nothing to divide by: all codes are zero
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t top_bits, bool fp8) {
+    const float a = __uint_as_float(top_bits);
+    RowScale o;
+    o.s = a / (fp8 ? 448.0f : 127.0f);
+    o.none = !(o.s > 0.0f) || top_bits >= 0x7f800000u;
+    o.up = o.s < 0x1p-90f ? 0x1p64f : 1.0f;
+    o.s *= o.up;
+    o.r = o.none ? 0.0f : 1.0f / o.s;
+    return o;
+}
+__device__ __forceinline__ void store_row_statistics(const NormArgs& a, int64_t row, double sumsq, uint32_t top_bits) {
+    const double inv = 1.0 / sqrt(sumsq / static_cast<double>(a.dim) + a.eps);
+    const float s = __uint_as_float(top_bits) / (a.fp8 ? 448.0f : 127.0f);
+    a.scales[row] = top_bits >= 0x7f800000u ? __builtin_nanf("") : static_cast<float>(static_cast<double>(s) * inv);
+    a.inv_rms[row] = static_cast<float>(inv);
+}
+
+// One row per TPR lanes (64: four rows a workgroup; else a workgroup), held in registers between the statistics and
+// the codes: every byte is read once and written once.  V vectors of eight per lane.
+template <typename XT, typename WT, int TPR, int V>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_row_kernel(NormArgs a) {
+    constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
+    const int lane = threadIdx.x % TPR;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
+    const bool live = row < a.rows;
+    float z[V][8];
+    double sq = 0.0;
+    uint32_t top = 0;
+    const XT* xr = static_cast<const XT*>(a.x) + row * a.x_stride;
+    const WT* wr = static_cast<const WT*>(a.weight);
+    if (live) {
+        float w[V][8];
+#pragma unroll
+        for (int j = 0; j < V; ++j) load8(xr, (lane + j * TPR) * 8, a.dim, z[j]);
+        if (a.residual) {
+            const XT* rr = static_cast<const XT*>(a.residual) + row * a.r_stride;
+            XT* hr = static_cast<XT*>(a.hidden) + row * a.dim;
+            float r[V][8];
+#pragma unroll
+            for (int j = 0; j < V; ++j) load8(rr, (lane + j * TPR) * 8, a.dim, r[j]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[j][e] = static_cast<float>(static_cast<XT>(z[j][e] + r[j][e]));
+                store8(hr, (lane + j * TPR) * 8, a.dim, z[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            load8(wr, (lane + j * TPR) * 8, a.dim, w[j]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const double h = z[j][e];
+                sq = fma(h, h, sq);
+                z[j][e] *= w[j][e];
+                top = max(top, __float_as_uint(z[j][e]) & 0x7fffffffu);
+            }
+        }
+    }
+    sq = wave_sum_all(sq);
+    top = wave_max_all(top);
+    if constexpr (TPR > 64) {
+        __shared__ double sh_sq[TPR / 64];
+        __shared__ uint32_t sh_top[TPR / 64];
+        if ((threadIdx.x & 63) == 0) { sh_sq[threadIdx.x >> 6] = sq; sh_top[threadIdx.x >> 6] = top; }
+        __syncthreads();
+        sq = sh_sq[0];
+        top = sh_top[0];
+#pragma unroll
+        for (int w = 1; w < TPR / 64; ++w) { sq += sh_sq[w]; top = max(top, sh_top[w]); }
+    }
+    if (!live) return;
+    const RowScale q = row_scale(top, a.fp8);
+    uint8_t* cr = a.codes + row * a.dim;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int i = (lane + j * TPR) * 8;
+        if (i >= a.dim) break;
+        uint32_t lo = 0, hi = 0;
+        if (!q.none) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[j][e] *= q.up;
+            if (a.fp8) codes8<true>(z[j], q.s, q.r, lo, hi);
+            else codes8<false>(z[j], q.s, q.r, lo, hi);
+        }
+        store8_codes(cr, i, a.dim, lo, hi);
+    }
+    if (lane == 0) store_row_statistics(a, row, sq, top);
+}
+
+// Rows too long for the registers of a workgroup: two visits, the second to what the first has just read or written
+// (a lane reads back its own elements only).
+template <typename XT, typename WT>
+__global__ __launch_bounds__(1024) void rms_norm_loop_kernel(NormArgs a) {
+    __shared__ double sh_sq[16];
+    __shared__ uint32_t sh_top[16];
+    const int64_t row = blockIdx.x;
+    const XT* xr = static_cast<const XT*>(a.x) + row * a.x_stride;
+    const XT* rr = a.residual ? static_cast<const XT*>(a.residual) + row * a.r_stride : nullptr;
+    XT* hr = a.residual ? static_cast<XT*>(a.hidden) + row * a.dim : nullptr;
+    const WT* wr = static_cast<const WT*>(a.weight);
+    double sq = 0.0;
+    uint32_t top = 0;
+    for (int64_t i = static_cast<int64_t>(threadIdx.x) * 8; i < a.dim; i += 8192) {
+        float h[8], r[8], w[8];
+        load8(xr, i, a.dim, h);
+        load8(wr, i, a.dim, w);
+        if (rr) {
+            load8(rr, i, a.dim, r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = static_cast<float>(static_cast<XT>(h[e] + r[e]));
+            store8(hr, i, a.dim, h);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const double d = h[e];
+            sq = fma(d, d, sq);
+            top = max(top, __float_as_uint(h[e] * w[e]) & 0x7fffffffu);
+        }
+    }
+    sq = wave_sum_all(sq);
+    top = wave_max_all(top);
+    if ((threadIdx.x & 63) == 0) { sh_sq[threadIdx.x >> 6] = sq; sh_top[threadIdx.x >> 6] = top; }
+    __syncthreads();
+    sq = sh_sq[0];
+    top = sh_top[0];
+#pragma unroll
+    for (int w = 1; w < 16; ++w) { sq += sh_sq[w]; top = max(top, sh_top[w]); }
+    const RowScale q = row_scale(top, a.fp8);
+    uint8_t* cr = a.codes + row * a.dim;
+    const XT* back = hr ? hr : xr;
+    for (int64_t i = static_cast<int64_t>(threadIdx.x) * 8; i < a.dim; i += 8192) {
+        float z[8], w[8];
+        uint32_t lo = 0, hi = 0;
+        if (!q.none) {
+            load8(back, i, a.dim, z);
+            load8(wr, i, a.dim, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] = z[e] * w[e] * q.up;
+            if (a.fp8) codes8<true>(z, q.s, q.r, lo, hi);
+            else codes8<false>(z, q.s, q.r, lo, hi);
+        }
+        store8_codes(cr, i, a.dim, lo, hi);
+    }
+    if (threadIdx.x == 0) store_row_statistics(a, row, sq, top);
+}
+
+// ---- gradients ----
+//   u = dy w,  c = inv^2 sum(u h) / dim,  dx = inv (u - h c) + dh,  dw = sum over rows of dy h inv
+// with dy the gradient of what the codes stand for (the rounding to codes is passed straight through) and dh that
+// of the stored sum.
+struct NormGradArgs {
+    const void* grad;
+    const void* hidden;
+    const void* weight;
+    const float* inv_rms;
+    const void* grad_hidden;    // null: none
+    void* grad_x;
+    float* partials;            // [groups][dim]: a workgroup's share of dw
+    int64_t g_stride, h_stride, gh_stride;
+    int64_t rows;
+    int dim;
+};
+
+// A workgroup of TPR lanes takes rows blockIdx.x, + gridDim.x, ...; a lane keeps its columns' share of dw in
+// registers over all of them, so dw costs one store of a row per workgroup.
+template <typename XT, typename WT, int TPR, int V>
+__global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
+    __shared__ float sh[2][TPR / 64];
+    const int lane = threadIdx.x;
+    float dw[V][8], w[V][8];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        load8(static_cast<const WT*>(a.weight), (lane + j * TPR) * 8, a.dim, w[j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[j][e] = 0.0f;
+    }
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const float inv = a.inv_rms[row];
+        float g[V][8], h[V][8];
+        float c = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            load8(static_cast<const XT*>(a.grad) + row * a.g_stride, (lane + j * TPR) * 8, a.dim, g[j]);
+            load8(static_cast<const XT*>(a.hidden) + row * a.h_stride, (lane + j * TPR) * 8, a.dim, h[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                h[j][e] *= inv;                                    // the normalised row
+                dw[j][e] = fmaf(g[j][e], h[j][e], dw[j][e]);
+                g[j][e] *= w[j][e];
+                c = fmaf(g[j][e], h[j][e], c);
+            }
+        c = wave_sum_all(c);
+        if constexpr (TPR > 64) {
+            // two slots in turn: a wavefront may write the next row's before another has read this row's
+            if ((lane & 63) == 0) sh[turn][lane >> 6] = c;
+            __syncthreads();
+            c = sh[turn][0];
+#pragma unroll
+            for (int q = 1; q < TPR / 64; ++q) c += sh[turn][q];
+        }
+        c /= static_cast<float>(a.dim);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int i = (lane + j * TPR) * 8;
+            float dh[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (a.grad_hidden) load8(static_cast<const XT*>(a.grad_hidden) + row * a.gh_stride, i, a.dim, dh);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[j][e] = fmaf(inv, fmaf(-h[j][e], c, g[j][e]), dh[e]);
+            store8(static_cast<XT*>(a.grad_x) + row * a.dim, i, a.dim, g[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) store8(a.partials + static_cast<int64_t>(blockIdx.x) * a.dim, (lane + j * TPR) * 8, a.dim, dw[j]);
+}
+
+// Rows too long for that: the row's c first, ...
+template <typename XT, typename WT>
+__global__ __launch_bounds__(1024) void rms_norm_grad_dot_kernel(NormGradArgs a, float* dots) {
+    __shared__ float sh[16];
+    const int64_t row = blockIdx.x;
+    const float inv = a.inv_rms[row];
+    float c = 0.0f;
+    for (int64_t i = static_cast<int64_t>(threadIdx.x) * 8; i < a.dim; i += 8192) {
+        float g[8], h[8], w[8];
+        load8(static_cast<const XT*>(a.grad) + row * a.g_stride, i, a.dim, g);
+        load8(static_cast<const XT*>(a.hidden) + row * a.h_stride, i, a.dim, h);
+        load8(static_cast<const WT*>(a.weight), i, a.dim, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c = fmaf(g[e] * w[e], h[e] * inv, c);
+    }
+    c = wave_sum_all(c);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = c;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int q = 1; q < 16; ++q) c += sh[q];
+        dots[row] = c / static_cast<float>(a.dim);
+    }
+}
+// ... then stretches of 2048 columns by bands of rows.
+template <typename XT, typename WT>
+__global__ __launch_bounds__(256) void rms_norm_grad_apply_kernel(NormGradArgs a, const float* dots, int stretches, int bands) {
+    const int band = blockIdx.x / stretches;
+    const int64_t i = static_cast<int64_t>(blockIdx.x % stretches) * 2048 + threadIdx.x * 8;
+    if (i >= a.dim) return;
+    float w[8], dw[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    load8(static_cast<const WT*>(a.weight), i, a.dim, w);
+    for (int64_t row = band; row < a.rows; row += bands) {
+        const float inv = a.inv_rms[row], c = dots[row];
+        float g[8], h[8], dh[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        load8(static_cast<const XT*>(a.grad) + row * a.g_stride, i, a.dim, g);
+        load8(static_cast<const XT*>(a.hidden) + row * a.h_stride, i, a.dim, h);
+        if (a.grad_hidden) load8(static_cast<const XT*>(a.grad_hidden) + row * a.gh_stride, i, a.dim, dh);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            h[e] *= inv;
+            dw[e] = fmaf(g[e], h[e], dw[e]);
+            g[e] = fmaf(inv, fmaf(-h[e], c, g[e] * w[e]), dh[e]);
+        }
+        store8(static_cast<XT*>(a.grad_x) + row * a.dim, i, a.dim, g);
+    }
+    store8(a.partials + static_cast<int64_t>(band) * a.dim, i, a.dim, dw);
+}
+
+// dw[i] = the sum of the workgroups' shares in their order: 16 columns a workgroup, 16 lanes a column.
+template <typename WT>
+__global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict__ partials, int groups, int dim, WT* __restrict__ out) {
+    __shared__ double sh[16][17];
+    const int c = threadIdx.x & 15, part = threadIdx.x >> 4;
+    const int64_t col = static_cast<int64_t>(blockIdx.x) * 16 + c;
+    double s = 0.0;
+    if (col < dim)
+        for (int g = part; g < groups; g += 16) s += static_cast<double>(partials[static_cast<int64_t>(g) * dim + col]);
+    sh[part][c] = s;
+    __syncthreads();
+    if (part == 0 && col < dim) {
+#pragma unroll
+        for (int q = 1; q < 16; ++q) s += sh[q][c];
+        out[col] = static_cast<WT>(static_cast<float>(s));
+    }
+}

@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_ext.h>
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <cstdint>
@@ -34,6 +35,8 @@ namespace {
 #include "kernels_codes.h"
 #include "kernels_outer.h"
 #include "kernels_segmented.h"
+#include "kernels_norm.h"
+#include "kernels_lowbit.h"
 
 // ---------------------------------------------------------------------------------------------
 // host side
@@ -167,7 +170,8 @@ int launch_check(const char* where) {
 enum KernelId {
     kIdStats, kIdStatsFinalize, kIdQuantize, kIdQuantizeHist, kIdHist, kIdLutFinalize, kIdDequantSet, kIdDequantAdd,
     kIdDequantAddStats, kIdDequantSetStats, kIdBatched, kIdCopy, kIdFill, kIdPseudoGrad, kIdOuterStep, kIdOuterStepCodes, kIdDiv, kIdFirstTouchCodes, kIdCodeCount, kIdCodeTotal, kIdRequantPlan, kIdCodeRemap, kIdNormLiteral, kIdUniformSmall,
-    kIdSegStats, kIdSegDequantAdd, kIdSegDequantSet, kIdSegQuantize, kIdSegLutFinalize, kIdSegPseudoGrad, kIdSegOuterStep, kIdCount
+    kIdSegStats, kIdSegDequantAdd, kIdSegDequantSet, kIdSegQuantize, kIdSegLutFinalize, kIdSegPseudoGrad, kIdSegOuterStep,
+    kIdRmsNorm, kIdRmsNormGrad, kIdColumnSum, kIdGroupPack, kIdGroupUnpack, kIdMatvec4, kIdCount
 };
 const char* const kKernelNames[kIdCount] = {
     "stats_kernel", "stats_finalize_kernel", "quantize_kernel", "quantize_kernel+hist", "hist_kernel", "lut_finalize_kernel",
@@ -175,7 +179,8 @@ const char* const kKernelNames[kIdCount] = {
     "batched_kernel", "copy_kernel", "fill_zero_kernel", "pseudo_gradient_kernel", "outer_step_kernel", "outer_step_kernel<codes>", "div_kernel",
     "first_touch_kernel<codes>", "code_count_kernel", "code_total_kernel", "requant_plan_kernel", "code_remap_kernel", "norm_literal_kernel", "uniform_small_kernel",
     "seg_stats_kernel", "seg_dequant_kernel<add,stats>", "seg_dequant_kernel<set,stats>", "seg_quantize_kernel+hist", "seg_lut_finalize_kernel",
-    "seg_pseudo_gradient_kernel", "seg_outer_step_kernel"};
+    "seg_pseudo_gradient_kernel", "seg_outer_step_kernel",
+    "rms_norm_kernel", "rms_norm_grad_kernel", "column_sum_kernel", "group4_pack_kernel", "group4_unpack_kernel", "matvec4_kernel"};
 
 struct TimedLaunch {
     int id;
@@ -1319,3 +1324,6 @@ int prime_copy_bytes(void* dst, const void* src, int64_t n_bytes, prime_stream_t
 }
 
 }  // extern "C"
+
+// low-bit operators of the model's own forward and backward step
+#include "entry_lowbit.h"

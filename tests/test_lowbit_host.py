@@ -1,0 +1,145 @@
+"""The low-bit operators on the CPU: schemas, shapes, refusals, argument checks of the C ABI (nothing here launches a kernel)."""
+import ctypes
+
+import pytest
+import torch
+
+from prime_amd import lowbit
+from tests import lowbit_reference as ref
+
+
+def test_every_lowbit_op_traces_on_fake_tensors():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x, r, w = torch.empty(2, 3, 70, dtype=torch.bfloat16), torch.empty(2, 3, 70, dtype=torch.bfloat16), torch.empty(70)
+        codes, scales, inv = lowbit.rms_norm_quantize(x, w)
+        assert codes.shape == (2, 3, 70) and codes.dtype == torch.int8 and scales.shape == inv.shape == (2, 3)
+        codes, scales, hidden, inv = lowbit.add_rms_norm_quantize(x, r, w, 1e-5, torch.float8_e4m3fn)
+        assert codes.dtype == torch.float8_e4m3fn and hidden.shape == x.shape and hidden.dtype == torch.bfloat16
+        assert scales.dtype == inv.dtype == torch.float32
+        gx, gw = lowbit.rms_norm_quantize_backward(x, hidden, w, inv, r)
+        assert gx.shape == x.shape and gx.dtype == torch.bfloat16 and gw.shape == (70,) and gw.dtype == torch.float32
+        packed, s = lowbit.quantize_4bit(torch.empty(5, 70), 32, torch.float32)
+        assert packed.shape == (5, 48) and packed.dtype == torch.uint8 and s.shape == (5, 3) and s.dtype == torch.float32
+        assert lowbit.dequantize_4bit(packed, s, 70, torch.float16).shape == (5, 70)
+        assert lowbit.dequantize_4bit(packed, s).shape == (5, 96)
+        y = lowbit.matvec_4bit(x, packed, s)
+        assert y.shape == (2, 3, 5) and y.dtype == torch.bfloat16
+        assert lowbit.matvec_4bit(codes.to(torch.int8), packed, s, scales).dtype == torch.float32
+    names = {s.name.split("::")[1] for s in torch._C._jit_get_all_schemas() if s.name.startswith("prime_lowbit::")}
+    assert names == {"rms_norm_quantize", "add_rms_norm_quantize", "rms_norm_quantize_backward", "quantize_4bit", "dequantize_4bit", "matvec_4bit"}
+
+
+def test_cpu_tensors_reach_no_kernel():
+    x, w = torch.randn(3, 64), torch.ones(64)
+    packed, s = torch.zeros(4, 32, dtype=torch.uint8), torch.ones(4, 1)
+    for call in (lambda: lowbit.rms_norm_quantize(x, w), lambda: lowbit.add_rms_norm_quantize(x, x, w),
+                 lambda: lowbit.rms_norm_quantize_backward(x, x, w, torch.ones(3)), lambda: lowbit.quantize_4bit(x, 64),
+                 lambda: lowbit.dequantize_4bit(packed, s), lambda: lowbit.matvec_4bit(x, packed, s)):
+        with pytest.raises(NotImplementedError):
+            call()
+
+
+def _refusals():
+    """(what is wrong, the implementation behind the dispatcher, arguments): the checks come before anything touches a device."""
+    x, w = torch.randn(3, 64), torch.ones(64)
+    packed, s = torch.zeros(4, 32, dtype=torch.uint8), torch.ones(4, 1)
+    n, a, b = lowbit._rms_norm_quantize, lowbit._add_rms_norm_quantize, lowbit._rms_norm_quantize_backward
+    q, d, m = lowbit._quantize_4bit, lowbit._dequantize_4bit, lowbit._matvec_4bit
+    i8 = torch.zeros(3, 64, dtype=torch.int8)
+    return [
+        ("Float, BFloat16 or Half", n, (x.double(), w)), ("1 to 2\\^30", n, (torch.tensor(1.0), w)), ("1 to 2\\^30", n, (x[:, :0], w[:0])),
+        ("weight needs shape", n, (x, w[:63])), ("weight needs shape", n, (x, w.view(1, 64))), ("weight must be", n, (x, w.half())),
+        ("codes are", n, (x, w, 1e-6, torch.uint8)), ("eps", n, (x, w, -1e-6)), ("eps", n, (x, w, float("nan"))),
+        ("residual must have", a, (x, x[:2], w)), ("residual must have", a, (x, x.half(), w)),
+        ("no gradient", n, (x, torch.nn.Parameter(w))), ("no gradient", a, (x, x.clone().requires_grad_(), w)),
+        ("grad must have", b, (x[:2], x, w, torch.ones(3))), ("inv_rms must be", b, (x, x, w, torch.ones(2))),
+        ("inv_rms must be", b, (x, x, w, torch.ones(3).double())), ("grad_hidden must have", b, (x, x, w, torch.ones(3), x.half())),
+        ("Float, BFloat16 or Half weight", q, (packed,)), ("a matrix", q, (w,)), ("a matrix", q, (x[:, :0],)), ("group size", q, (x, 48)),
+        ("scales are", q, (x, 64, torch.float16)),
+        ("Byte codes", d, (packed.int(), s)), ("Byte codes", d, (packed, s.half())), ("same rows", d, (packed, s[:3])), ("same rows", d, (packed, s[:, :0])),
+        ("do not make groups", d, (packed, torch.ones(4, 3))), ("do not make groups", d, (packed, torch.ones(4, 4))), ("hold 1 to 64", d, (packed, s, 65)),
+        ("hold 1 to 64", d, (packed, s, 0)), ("hold 33 to 64", d, (packed, torch.ones(4, 2), 32)), ("weights are", d, (packed, s, 64, torch.int8)),
+        ("Char rows", m, (x.double(), packed, s)), ("a scalar", m, (torch.tensor(1.0), packed, s)), ("hold 1 to 64", m, (torch.randn(3, 65), packed, s)),
+        ("come with x_scales", m, (i8, packed, s)), ("come with x_scales", m, (x, packed, s, torch.ones(3))),
+        ("x_scales must be", m, (i8, packed, s, torch.ones(2))), ("x_scales must be", m, (i8, packed, s, torch.ones(3).half())),
+        ("products are", m, (x, packed, s, None, torch.int8)), ("no gradient", m, (x.clone().requires_grad_(), packed, s)),
+    ]
+
+
+@pytest.mark.parametrize("case", range(len(_refusals())))
+def test_refusals(case):
+    what, call, args = _refusals()[case]
+    with pytest.raises(RuntimeError, match=what):
+        call(*args)
+
+
+def test_tensors_on_two_devices_are_refused():
+    x, w = torch.empty(3, 64, device="meta"), torch.ones(64)
+    with pytest.raises(RuntimeError, match="one device"):
+        lowbit._rms_norm_quantize(x, w)
+
+
+def test_c_abi_refuses_bad_arguments_before_any_launch():
+    from prime_amd import _lib
+
+    lib = _lib.load()
+    p = ctypes.c_void_p(4096)
+
+    def norm(x=p, xs=64, r=None, rs=0, w=p, rows=3, dim=64, t=0, wt=0, ct=3, eps=1e-6, codes=p, scales=p, hidden=None, inv=p):
+        return lib.prime_rms_norm_quantize(x, xs, r, rs, w, rows, dim, t, wt, ct, eps, codes, scales, hidden, inv, None)
+
+    assert norm(rows=0, x=None) == 0
+    for bad in (dict(x=None), dict(w=None), dict(codes=None), dict(scales=None), dict(inv=None), dict(r=p), dict(hidden=p), dict(rows=-1), dict(dim=0),
+                dict(dim=(1 << 30) + 1), dict(t=3), dict(wt=1), dict(ct=0), dict(eps=-1.0), dict(eps=float("nan")), dict(xs=-1)):
+        assert norm(**bad) == -1, bad
+        assert b"prime_rms_norm_quantize" in lib.prime_hip_last_error()
+    need = lib.prime_rms_norm_backward_scratch_bytes(3, 64)
+    assert need >= 64 * 4 and lib.prime_rms_norm_backward_scratch_bytes(-1, 64) < 0 and lib.prime_rms_norm_backward_scratch_bytes(1, 0) < 0
+
+    def back(g=p, h=p, w=p, inv=p, rows=3, dim=64, t=0, wt=0, gx=p, gw=p, scratch=p, nbytes=need):
+        return lib.prime_rms_norm_quantize_backward(g, 64, h, 64, w, inv, None, 0, rows, dim, t, wt, gx, gw, scratch, nbytes, None)
+
+    for bad in (dict(g=None), dict(h=None), dict(w=None), dict(inv=None), dict(gx=None), dict(gw=None), dict(rows=-1), dict(dim=0), dict(t=4), dict(wt=2)):
+        assert back(**bad) == -1, bad
+    assert back(scratch=None) == -2 and back(nbytes=need - 1) == -2 and back(scratch=ctypes.c_void_p(4098)) == -2
+
+    def quant(w=p, n=3, k=64, t=0, g=64, st=0, packed=p, scales=p):
+        return lib.prime_quantize_4bit(w, 64, n, k, t, g, st, packed, scales, None)
+
+    assert quant(n=0, w=None) == 0
+    for bad in (dict(w=None), dict(packed=None), dict(scales=None), dict(n=-1), dict(k=0), dict(t=3), dict(g=16), dict(g=96), dict(st=2)):
+        assert quant(**bad) == -1, bad
+
+    def deq(packed=p, scales=p, n=3, k=64, g=64, st=0, out=p, ot=0):
+        return lib.prime_dequantize_4bit(packed, 32, scales, 1, n, k, g, st, out, ot, None)
+
+    assert deq(n=0, out=None) == 0
+    for bad in (dict(packed=None), dict(scales=None), dict(out=None), dict(n=-1), dict(k=0), dict(ot=3), dict(g=0), dict(st=1 << 8)):
+        assert deq(**bad) == -1, bad
+
+    def mv(x=p, xt=0, xs=None, packed=p, scales=p, rows=2, n=3, k=64, g=64, st=0, out=p, ot=0):
+        return lib.prime_matvec_4bit(x, 64, xt, xs, packed, 32, scales, 1, rows, n, k, g, st, out, ot, None)
+
+    assert mv(rows=0, x=None) == 0 and mv(n=0, out=None) == 0
+    for bad in (dict(x=None), dict(packed=None), dict(scales=None), dict(out=None), dict(xt=4), dict(xt=3), dict(xs=p), dict(rows=-1), dict(n=-1), dict(k=0),
+                dict(g=33), dict(st=2), dict(ot=3)):
+        assert mv(**bad) == -1, bad
+
+
+def test_reference_rounds_to_e4m3_as_the_type_is_defined():
+    # every e4m3 number is its own nearest; midpoints go to the even neighbour
+    every = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).to(torch.float64)
+    fine = every[torch.isfinite(every)]
+    assert torch.equal(ref.e4m3(fine), fine)
+    v = torch.unique(fine[fine >= 0])
+    mid = (v[1:] + v[:-1]) / 2
+    even = torch.where(torch.arange(len(mid)) % 2 == 0, v[:-1], v[1:])
+    assert torch.equal(ref.e4m3(mid), even) and torch.equal(ref.e4m3(mid * (1 + 2.0 ** -40)), v[1:]) and torch.equal(ref.e4m3(mid * (1 - 2.0 ** -40)), v[:-1])
+
+
+def test_reference_packing_is_its_own_inverse():
+    codes = torch.randint(-8, 8, (3, 64), dtype=torch.int8)
+    assert torch.equal(ref.unpack(ref.pack(codes)), codes)
+    assert int(ref.pack(torch.tensor([[1, -1]], dtype=torch.int8))[0, 0]) == 0xF1
