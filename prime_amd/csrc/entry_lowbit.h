@@ -89,6 +89,49 @@ bool bad_group(int group) { return group != 32 && group != 64 && group != 128; }
 bool bad_matrix(int64_t n, int64_t k) { return n < 0 || n >= (int64_t(1) << 40) || k < 1 || k > kMaxDim; }
 int group_shift(int group) { return group == 32 ? 5 : group == 64 ? 6 : 7; }
 
+constexpr int kMatvecWaves = 8;
+
+template <typename XT, int GS, int IR, int NT, int XBYTES>
+void launch_matvec_as(MatvecArgs a, double bytes, hipStream_t st) {
+    const int row_tile = IR == 1 ? 4 : 16, held = std::min(a.rows, row_tile) * Held<XT>::kPlanes, blocks = (a.k + 127) / 128;
+    const int block_bytes = 16 * static_cast<int>(sizeof(typename Held<XT>::type));
+    // whole rows of x in LDS if they fit, else as many blocks as do, a multiple of what the wavefronts take in a turn
+    const int most = (XBYTES / held - 16) / block_bytes, turn = kMatvecWaves * (4 / NT);
+    a.chunk_blocks = blocks <= most ? blocks : most >= turn ? most / turn * turn : most;
+    a.tiles = (a.n + 16 * NT - 1) / (16 * NT);
+    // a dispatch counts its work-items in 32 bits: 2^22 workgroups at a time
+    const int64_t row_tiles = (a.rows + row_tile - 1) / row_tile, step = std::max<int64_t>(1, (int64_t(1) << 22) / a.tiles);
+    const int type = a.out_type, rows = a.rows;
+    for (int64_t at = 0; at < row_tiles; at += step) {
+        MatvecArgs part = a;
+        const int64_t row = at * row_tile;
+        part.rows = static_cast<int>(std::min(rows - row, step * row_tile));
+        part.x = static_cast<const XT*>(a.x) + row * a.x_stride;
+        if (a.x_scales) part.x_scales = a.x_scales + row;
+        part.out = static_cast<uint8_t*>(a.out) + row * a.n * type_bytes(type);
+        launch(kIdMatvec4, bytes, matvec4_kernel<XT, GS, IR, NT, kMatvecWaves, XBYTES>,
+               static_cast<int>(a.tiles * ((part.rows + row_tile - 1) / row_tile)), kMatvecWaves * 64, st, part);
+    }
+}
+
+template <typename XT, int GS>
+void launch_matvec_group(const MatvecArgs& a, double bytes, hipStream_t st) {
+    if (a.rows <= 4) {
+        if (a.n >= 32768) launch_matvec_as<XT, GS, 1, 4, 32768>(a, bytes, st);
+        else launch_matvec_as<XT, GS, 1, 1, 32768>(a, bytes, st);
+    } else {
+        if (a.n >= 32768) launch_matvec_as<XT, GS, 4, 4, 65536>(a, bytes, st);
+        else launch_matvec_as<XT, GS, 4, 1, 65536>(a, bytes, st);
+    }
+}
+
+template <typename XT>
+void launch_matvec(const MatvecArgs& a, int group, double bytes, hipStream_t st) {
+    if (group == 32) launch_matvec_group<XT, 5>(a, bytes, st);
+    else if (group == 64) launch_matvec_group<XT, 6>(a, bytes, st);
+    else launch_matvec_group<XT, 7>(a, bytes, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -202,7 +245,7 @@ int prime_dequantize_4bit(const uint8_t* packed, int64_t packed_stride, const vo
 int prime_matvec_4bit(const void* x, int64_t x_stride, int x_type, const float* x_scales, const uint8_t* packed, int64_t packed_stride,
                       const void* scales, int64_t scale_stride, int64_t rows, int64_t n, int64_t k, int group, int scale_type, void* out,
                       int out_type, prime_stream_t stream) {
-    if (bad_matrix(n, k) || n >= (int64_t(1) << 31) || rows < 0 || rows >= (int64_t(1) << 31) || x_stride < 0 || packed_stride < 0 || scale_stride < 0)
+    if (bad_matrix(n, k) || n > (int64_t(1) << 26) || rows < 0 || rows >= (int64_t(1) << 31) || x_stride < 0 || packed_stride < 0 || scale_stride < 0)
         return fail(PRIME_EINVAL, "prime_matvec_4bit: bad size");
     if ((!is_float_type(x_type) && x_type != PRIME_I8) || !is_float_type(out_type) || !is_scale_type(scale_type))
         return fail(PRIME_EINVAL, "prime_matvec_4bit: bad type");
@@ -210,20 +253,14 @@ int prime_matvec_4bit(const void* x, int64_t x_stride, int x_type, const float* 
     if (n == 0 || rows == 0) return 0;
     if (!x || !packed || !scales || !out || (x_type == PRIME_I8) != (x_scales != nullptr))
         return fail(PRIME_EINVAL, "prime_matvec_4bit: null operand, or scales without int8 rows");
-    MatvecArgs a{x, x_scales, packed, scales, out, x_stride, packed_stride, scale_stride, static_cast<int>(rows), n, static_cast<int>(k), group_shift(group)};
-    const double bytes = static_cast<double>(n) * k / 2 + static_cast<double>(n) * ((k + group - 1) / group) * type_bytes(scale_type) +
+    const int64_t groups = (k + group - 1) / group;
+    MatvecArgs a{x, x_scales, packed, scales, out, x_stride, packed_stride, scale_stride, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k),
+                 static_cast<int>(groups * group / 2), static_cast<int>(groups), scale_type == PRIME_BF16, out_type, 0, 0};
+    const double bytes = static_cast<double>(n) * k / 2 + static_cast<double>(n) * groups * type_bytes(scale_type) +
                          static_cast<double>(rows) * (k * type_bytes(x_type) + n * type_bytes(out_type));
-    with_scale_type(scale_type, [&](auto s) {
-        using ST = decltype(s);
-        with_float_type(out_type, [&](auto o) {
-            using OT = decltype(o);
-            auto go = [&](auto t) {
-                launch(kIdMatvec4, bytes, matvec4_kernel<decltype(t), ST, OT>, static_cast<int>((n + 3) / 4), 256, static_cast<hipStream_t>(stream), a);
-            };
-            if (x_type == PRIME_I8) go(int8_t{});
-            else with_float_type(x_type, go);
-        });
-    });
+    auto go = [&](auto t) { launch_matvec<decltype(t)>(a, group, bytes, static_cast<hipStream_t>(stream)); };
+    if (x_type == PRIME_I8) go(int8_t{});
+    else with_float_type(x_type, go);
     return launch_check("matvec4_kernel");
 }
 
