@@ -130,10 +130,11 @@ struct MatvecArgs {
     int k;
     int row_bytes;              // codes of a row that exist: whole groups
     int groups;
-    int scale_bf16;
     int out_type;               // PRIME_F32, PRIME_BF16 or PRIME_F16
-    int chunk_blocks;           // blocks of 128 columns of x that LDS holds at a time
-    int tiles;                  // workgroups along n
+    int chunk_quads;            // stretches of 512 columns of x that LDS holds at a time
+    int tiles;                  // 16 outputs each
+    int sets;                   // rounds of tiles a row tile takes: ceil(tiles / tiles a workgroup takes at a time)
+    int split_shift;            // log2 of the wavefronts that share a tile's columns
 };
 
 // Sums of one step: fp32, or exact integers.
@@ -223,176 +224,165 @@ __device__ __forceinline__ f32x4 product(u32x4 rows, u32x4 codes, f32x4 c) {
 // counts, the others are not used), else all 16.  Rows that do not exist repeat the last one; their sums are dropped.
 template <int IR> __device__ __forceinline__ int row_of(int v) { return IR == 1 ? v >> 2 : v; }
 
-template <typename XT, int GS, int IR, int NT, int WK, int XBYTES>
-__global__ __launch_bounds__(WK * 64) void matvec4_kernel(MatvecArgs a) {
-    constexpr int kThreadsHere = WK * 64;
-    constexpr int kPlanes = Held<XT>::kPlanes;
-    constexpr int NG = 1 << (7 - GS);             // groups of a block of 128 columns
-    constexpr int U = 4 / NT;                     // blocks a wavefront has in flight together
-    typedef typename Held<XT>::type held_t;
-    constexpr bool kInt = sizeof(XT) == 1;
-    __shared__ __align__(16) uint8_t lds[XBYTES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4;
-    const int tile = blockIdx.x % a.tiles, row0 = blockIdx.x / a.tiles * (IR == 1 ? 4 : 16);
-    const int rows = min(a.rows - row0, IR == 1 ? 4 : 16);
-    const int blocks = (a.k + 127) >> 7;
-    const int row_stride = a.chunk_blocks * 16 * static_cast<int>(sizeof(held_t)) + 16;      // 16 bytes more: rows start on other banks
-    const int plane_stride = rows * row_stride;
-    const int my_row = min(row_of<IR>(lane & 15), rows - 1) * row_stride + quarter * 4 * static_cast<int>(sizeof(held_t));
-    const uint8_t* codes[NT];
-    int64_t scale_at[NT];
+// Scales of the groups of 512 columns of one output, as they are stored.
+template <typename ST, int GS> struct QuadScales {
+    static constexpr int kCount = 4 << (7 - GS);
+    typedef ST vec __attribute__((ext_vector_type(kCount), aligned(sizeof(ST))));
+    vec v;
+    __device__ __forceinline__ void load(const ST* p) { v = *reinterpret_cast<const vec*>(p); }
+    __device__ __forceinline__ void load_some(const ST* p, int there) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int n = min((tile * NT + t) * 16 + (lane & 15), a.n - 1);
-        codes[t] = a.packed + n * a.p_stride + quarter * 16;
-        scale_at[t] = n * a.s_stride;
+        for (int i = 0; i < kCount; ++i) v[i] = i < there ? p[i] : static_cast<ST>(0.0f);
     }
-    auto fetch = [&](int b, u32x4 (&w)[NT], float (&s)[NT][NG]) {
-        const bool here = b < blocks && b * 64 + quarter * 16 < a.row_bytes;
+    __device__ __forceinline__ float at(int i) const { return static_cast<float>(v[i]); }
+};
+
+// 128 columns of 16 outputs against the rows at `mine` in LDS, added to y: `scale(g)` is the factor of group g of them.
+template <typename XT, int GS, int IR, typename Scale>
+__device__ __forceinline__ void add_block(u32x4 v, const uint8_t* mine, int plane_stride, Scale scale, float (&y)[IR]) {
+    constexpr int NG = 1 << (7 - GS);
+    constexpr int kPlanes = Held<XT>::kPlanes;
+    if constexpr (GS < 7) transpose_quarters(v);
+    typename Sum<XT>::type acc[NG];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            typedef u32x4 __attribute__((aligned(1))) u32x4u;
-            w[t] = here ? *reinterpret_cast<const u32x4u*>(codes[t] + static_cast<int64_t>(b) * 64) : u32x4{0, 0, 0, 0};
+    for (int g = 0; g < NG; ++g) acc[g] = typename Sum<XT>::type{0, 0, 0, 0};
+    if constexpr (sizeof(XT) == 1) {
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const int at = b * NG + g;
-                s[t][g] = 0.0f;
-                if (at < a.groups) {
-                    if (a.scale_bf16) s[t][g] = load_scale(static_cast<const __bf16*>(a.scales) + scale_at[t] + at);
-                    else s[t][g] = load_scale(static_cast<const float*>(a.scales) + scale_at[t] + at);
-                }
+        for (int j = 0; j < 2; ++j) {
+            const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + 16 * j);
+            const u32x4 b{(v[2 * j] << 4) & 0xf0f0f0f0u, v[2 * j] & 0xf0f0f0f0u, (v[2 * j + 1] << 4) & 0xf0f0f0f0u, v[2 * j + 1] & 0xf0f0f0f0u};
+            if constexpr (GS == 5) {
+                const u32x2 a0{xa[0], xa[1]}, a1{xa[2], xa[3]}, b0{b[0], b[1]}, b1{b[2], b[3]};
+                acc[2 * j] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a0), __builtin_bit_cast(long, b0), acc[2 * j], 0, 0, 0);
+                acc[2 * j + 1] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a1), __builtin_bit_cast(long, b1), acc[2 * j + 1], 0, 0, 0);
+            } else {
+                const int g = GS == 6 ? j : 0;
+                acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, xa), __builtin_bit_cast(i32x4, b), acc[g], 0, 0, 0);
             }
+        }
+    } else {
+        constexpr bool kBf16 = !std::is_same<XT, _Float16>::value;
+        constexpr uint32_t kOff = kBf16 ? kOffsetBf16 : kOffsetF16;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int g = j >> (GS - 5);
+            const u32x4 b = widen_word<kBf16>(v[j]);
+#pragma unroll
+            for (int p = 0; p < kPlanes; ++p) {
+                const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + p * plane_stride + 16 * j);
+                acc[g] = product<XT>(xa, u32x4{kOff, kOff, kOff, kOff}, acc[g]);
+                acc[g] = product<XT>(xa, b, acc[g]);
+            }
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int i = 0; i < IR; ++i) y[i] = fmaf(static_cast<float>(acc[g][i]), scale(g), y[i]);
+}
+
+__device__ __forceinline__ void store_product(const MatvecArgs& a, int64_t at, float v) {
+    if (a.out_type == PRIME_F32) static_cast<float*>(a.out)[at] = v;
+    else if (a.out_type == PRIME_BF16) static_cast<__bf16*>(a.out)[at] = static_cast<__bf16>(v);
+    else static_cast<_Float16*>(a.out)[at] = static_cast<_Float16>(v);
+}
+
+// Up to 4 (IR 1) or 16 (IR 4) rows.  A wavefront takes a tile of 16 outputs, or every second, fourth or eighth stretch of 512
+// columns of one (split_shift); a workgroup as many tiles side by side as that leaves wavefronts for, set after set.  The next
+// stretch's codes and scales are on their way while one is multiplied, across tiles too.
+template <typename XT, typename ST, int GS, int IR, int XBYTES>
+__global__ __launch_bounds__(512) void matvec4_kernel(MatvecArgs a) {
+    constexpr int kPlanes = Held<XT>::kPlanes;
+    constexpr int NG = 1 << (7 - GS);
+    typedef typename Held<XT>::type held_t;
+    constexpr int kBlock = 16 * static_cast<int>(sizeof(held_t));       // bytes of a row's 128 columns in LDS
+    __shared__ __align__(16) uint8_t lds[XBYTES];
+    __shared__ float part[2][8 * IR * 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
+    const int split = 1 << a.split_shift, kpart = wave & (split - 1);
+    const int side = static_cast<int>(blockDim.x >> 6) >> a.split_shift;                    // tiles at a time
+    constexpr int kRowTile = IR == 1 ? 4 : 16;
+    const int per_row_tile = gridDim.x / ((a.rows + kRowTile - 1) / kRowTile);               // workgroups of a row tile
+    const int row0 = blockIdx.x / per_row_tile * kRowTile, set0 = blockIdx.x % per_row_tile;
+    const int rows = min(a.rows - row0, kRowTile);
+    const int quads = (a.k + 511) >> 9;
+    const int row_stride = a.chunk_quads * 4 * kBlock + 16;              // 16 bytes more: rows start on other banks
+    const int plane_stride = rows * row_stride;
+    const uint8_t* mine = lds + min(row_of<IR>(lane & 15), rows - 1) * row_stride + quarter * 4 * static_cast<int>(sizeof(held_t));
+    const ST* scales = static_cast<const ST*>(a.scales);
+    u32x4 w[4], w2[4];
+    QuadScales<ST, GS> s, s2;
+    auto fetch = [&](int set, int q, u32x4 (&to)[4], QuadScales<ST, GS>& sc) {
+        const int64_t n = min((set * side + (wave >> a.split_shift)) * 16 + (lane & 15), a.n - 1);
+        typedef u32x4 __attribute__((aligned(1))) u32x4u;
+        const uint8_t* p = a.packed + n * a.p_stride + static_cast<int64_t>(q) * 256 + quarter * 16;
+        const ST* sp = scales + n * a.s_stride + static_cast<int64_t>(q) * (4 * NG);
+        if ((q + 1) * 256 <= a.row_bytes) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) to[u] = *reinterpret_cast<const u32x4u*>(p + 64 * u);
+            sc.load(sp);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                to[u] = q * 256 + u * 64 + quarter * 16 < a.row_bytes ? *reinterpret_cast<const u32x4u*>(p + 64 * u) : u32x4{0, 0, 0, 0};
+            sc.load_some(sp, a.groups - q * (4 * NG));
         }
     };
-    float y[NT][IR];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < IR; ++i) y[t][i] = 0.0f;
-    u32x4 w[U][NT], w2[U][NT];
-    float s[U][NT][NG], s2[U][NT][NG];
-#pragma unroll
-    for (int u = 0; u < U; ++u) fetch(wave + u * WK, w[u], s[u]);
     const XT* x = static_cast<const XT*>(a.x) + static_cast<int64_t>(row0) * a.x_stride;
-    for (int first = 0; first < blocks; first += a.chunk_blocks) {
-        const int held = min(a.chunk_blocks, blocks - first);
-        if (first) {
+    fetch(set0, kpart, w, s);
+    int turn = 0;
+    for (int set = set0; set < a.sets; set += per_row_tile, turn ^= 1) {
+        float y[IR];
+#pragma unroll
+        for (int i = 0; i < IR; ++i) y[i] = 0.0f;
+        for (int first = 0; first < quads; first += a.chunk_quads) {
+            const int held = min(a.chunk_quads, quads - first);
+            if (set == set0 || held < quads) {
+                if (set != set0 || first) __syncthreads();
+                // rows of x to LDS: eight columns a lane, put where the lane that multiplies them will look
+                for (int i = threadIdx.x; i < rows * held * 64; i += blockDim.x) {
+                    const int m = i / (held * 64), c = i - m * (held * 64);
+                    held_t v[kPlanes];
+                    hold8(x + m * a.x_stride, first * 512 + c * 8, a.k, v);
+                    const int in = c & 15, to = (c & ~15) | (GS == 7 ? in : (in & 3) * 4 + (in >> 2));
+#pragma unroll
+                    for (int p = 0; p < kPlanes; ++p) *reinterpret_cast<held_t*>(lds + p * plane_stride + m * row_stride + to * static_cast<int>(sizeof(held_t))) = v[p];
+                }
+                __syncthreads();
+            }
+            for (int q = kpart; q < held; q += split) {
+                const bool more = first + q + split < quads;
+                const int next_set = more ? set : min(set + per_row_tile, a.sets - 1);
+                fetch(next_set, more ? first + q + split : kpart, w2, s2);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    add_block<XT, GS, IR>(w[u], mine + (q * 4 + u) * kBlock, plane_stride, [&](int g) { return s.at(u * NG + g); }, y);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) w[u] = w2[u];
+                s = s2;
+            }
+        }
+        const int n = (set * side + (wave >> a.split_shift)) * 16 + (lane & 15);
+        if (split == 1) {
+#pragma unroll
+            for (int i = 0; i < IR; ++i) {
+                const int m = quarter * IR + i;
+                if (m < rows && n < a.n) store_product(a, static_cast<int64_t>(row0 + m) * a.n + n, sizeof(XT) == 1 ? y[i] * (a.x_scales[row0 + m] * 0.0625f) : y[i]);
+            }
+        } else {
+            // the wavefronts' sums, added in their order; two buffers in turn, so that one barrier a set is enough
+#pragma unroll
+            for (int i = 0; i < IR; ++i) part[turn][(wave * IR + i) * 64 + lane] = y[i];
             __syncthreads();
-            // a chunk that is no whole number of turns leaves its successor's first codes unasked for
-            if (a.chunk_blocks % (WK * U)) {
+            if (kpart == 0) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) fetch(first + wave + u * WK, w[u], s[u]);
-            }
-        }
-        // rows of x to LDS: eight columns a lane, put where the lane that multiplies them will look
-        for (int i = threadIdx.x; i < rows * held * 16; i += kThreadsHere) {
-            const int m = i / (held * 16), c = i - m * (held * 16);
-            held_t v[kPlanes];
-            hold8(x + m * a.x_stride, first * 128 + c * 8, a.k, v);
-            const int in = c & 15, to = (c & ~15) | (GS == 7 ? in : (in & 3) * 4 + (in >> 2));
-#pragma unroll
-            for (int p = 0; p < kPlanes; ++p) *reinterpret_cast<held_t*>(lds + p * plane_stride + m * row_stride + to * static_cast<int>(sizeof(held_t))) = v[p];
-        }
-        __syncthreads();
-        for (int at = wave; at < held; at += WK * U) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) fetch(first + at + (U + u) * WK, w2[u], s2[u]);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (at + u * WK >= held) break;      // the same for the whole wavefront
-                const uint8_t* mine = lds + my_row + (at + u * WK) * (16 * static_cast<int>(sizeof(held_t)));
-                if constexpr (kInt) {
-                    u32x4 xa[2];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) xa[j] = *reinterpret_cast<const u32x4*>(mine + 16 * j);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        u32x4 v = w[u][t];
-                        if constexpr (GS < 7) transpose_quarters(v);
-                        i32x4 acc[NG];
-#pragma unroll
-                        for (int g = 0; g < NG; ++g) acc[g] = i32x4{0, 0, 0, 0};
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const u32x4 b{(v[2 * j] << 4) & 0xf0f0f0f0u, v[2 * j] & 0xf0f0f0f0u, (v[2 * j + 1] << 4) & 0xf0f0f0f0u, v[2 * j + 1] & 0xf0f0f0f0u};
-                            if constexpr (GS == 5) {
-                                const u32x2 a0{xa[j][0], xa[j][1]}, a1{xa[j][2], xa[j][3]}, b0{b[0], b[1]}, b1{b[2], b[3]};
-                                acc[2 * j] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a0), __builtin_bit_cast(long, b0), acc[2 * j], 0, 0, 0);
-                                acc[2 * j + 1] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a1), __builtin_bit_cast(long, b1), acc[2 * j + 1], 0, 0, 0);
-                            } else {
-                                const int g = GS == 6 ? j : 0;
-                                acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, xa[j]), __builtin_bit_cast(i32x4, b), acc[g], 0, 0, 0);
-                            }
-                        }
-#pragma unroll
-                        for (int g = 0; g < NG; ++g)
-#pragma unroll
-                            for (int i = 0; i < IR; ++i) y[t][i] = fmaf(static_cast<float>(acc[g][i]), s[u][t][g], y[t][i]);
-                    }
-                } else {
-                    constexpr bool kBf16 = !std::is_same<XT, _Float16>::value;
-                    constexpr uint32_t kOff = kBf16 ? kOffsetBf16 : kOffsetF16;
-                    u32x4 xa[kPlanes][4];
-                    f32x4 start[NG];
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) start[g] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int p = 0; p < kPlanes; ++p)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            xa[p][j] = *reinterpret_cast<const u32x4*>(mine + p * plane_stride + 16 * j);
-                            start[j >> (GS - 5)] = product<XT>(xa[p][j], u32x4{kOff, kOff, kOff, kOff}, start[j >> (GS - 5)]);
-                        }
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        u32x4 v = w[u][t];
-                        if constexpr (GS < 7) transpose_quarters(v);
-                        f32x4 acc[NG];
-#pragma unroll
-                        for (int g = 0; g < NG; ++g) acc[g] = start[g];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const u32x4 b = widen_word<kBf16>(v[j]);
-#pragma unroll
-                            for (int p = 0; p < kPlanes; ++p) acc[j >> (GS - 5)] = product<XT>(xa[p][j], b, acc[j >> (GS - 5)]);
-                        }
-#pragma unroll
-                        for (int g = 0; g < NG; ++g)
-#pragma unroll
-                            for (int i = 0; i < IR; ++i) y[t][i] = fmaf(acc[g][i], s[u][t][g], y[t][i]);
-                    }
+                for (int i = 0; i < IR; ++i) {
+                    float v = y[i];
+                    for (int p = 1; p < split; ++p) v += part[turn][((wave + p) * IR + i) * 64 + lane];
+                    const int m = quarter * IR + i;
+                    if (m < rows && n < a.n) store_product(a, static_cast<int64_t>(row0 + m) * a.n + n, sizeof(XT) == 1 ? v * (a.x_scales[row0 + m] * 0.0625f) : v);
                 }
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    w[u][t] = w2[u][t];
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) s[u][t][g] = s2[u][t][g];
-                }
         }
-    }
-    // the wavefronts' sums, added in their order
-    float* part = reinterpret_cast<float*>(lds);
-    static_assert(WK * NT * IR * 64 * 4 <= XBYTES, "the sums fit where the rows were");
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < IR; ++i) part[((wave * NT + t) * IR + i) * 64 + lane] = y[t][i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < NT * IR * 64; i += kThreadsHere) {
-        float v = part[i];
-#pragma unroll
-        for (int q = 1; q < WK; ++q) v += part[q * NT * IR * 64 + i];
-        const int l = i & 63, r = (i >> 6) % IR, t = (i >> 6) / IR;
-        const int m = (l >> 4) * IR + r, n = (tile * NT + t) * 16 + (l & 15);
-        if (m >= rows || n >= a.n) continue;
-        if constexpr (kInt) v *= a.x_scales[row0 + m] * 0.0625f;
-        const int64_t at = static_cast<int64_t>(row0 + m) * a.n + n;
-        if (a.out_type == PRIME_F32) static_cast<float*>(a.out)[at] = v;
-        else if (a.out_type == PRIME_BF16) static_cast<__bf16*>(a.out)[at] = static_cast<__bf16>(v);
-        else static_cast<_Float16*>(a.out)[at] = static_cast<_Float16>(v);
     }
 }
