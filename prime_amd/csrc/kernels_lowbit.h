@@ -329,7 +329,13 @@ __global__ __launch_bounds__(512) void matvec4_kernel(MatvecArgs a) {
         }
     };
     const XT* x = static_cast<const XT*>(a.x) + static_cast<int64_t>(row0) * a.x_stride;
-    fetch(set0, kpart, w, s);
+    // Where a wavefront starts in its tile's columns: tiles side by side start at different ones, else all rows of
+    // a matrix whose row length is a power of two would be read at the same offset at a time, from the same memory channels.
+    const bool whole = a.chunk_quads >= quads;
+    const int own = (quads - kpart + split - 1) >> a.split_shift;
+    auto start = [&](int set) { return whole ? kpart + ((set * side + (wave >> a.split_shift)) % own << a.split_shift) : kpart; };
+    int at = start(set0);
+    fetch(set0, at, w, s);
     int turn = 0;
     for (int set = set0; set < a.sets; set += per_row_tile, turn ^= 1) {
         float y[IR];
@@ -350,10 +356,12 @@ __global__ __launch_bounds__(512) void matvec4_kernel(MatvecArgs a) {
                 }
                 __syncthreads();
             }
-            for (int q = kpart; q < held; q += split) {
-                const bool more = first + q + split < quads;
+            for (int i = kpart; i < held; i += split) {
+                const int q = at - first;
+                const bool more = first + i + split < quads;
                 const int next_set = more ? set : min(set + per_row_tile, a.sets - 1);
-                fetch(next_set, more ? first + q + split : kpart, w2, s2);
+                at = !more ? start(next_set) : at + split < quads ? at + split : kpart;
+                fetch(next_set, at, w2, s2);
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
                     add_block<XT, GS, IR>(w[u], mine + (q * 4 + u) * kBlock, plane_stride, [&](int g) { return s.at(u * NG + g); }, y);
