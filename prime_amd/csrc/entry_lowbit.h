@@ -123,10 +123,51 @@ void launch_matvec_as(MatvecArgs a, double bytes, hipStream_t st) {
     }
 }
 
+// Up to four floating rows at a time, or 16 of int8.
+template <typename XT, typename ST, int GS, int ROWS>
+void launch_matvec_few(MatvecArgs a, double bytes, hipStream_t st) {
+    constexpr int kMostLds = 56 << 10;
+    const int held = std::min(a.rows, ROWS), quads = (a.k + 511) / 512, quad_bytes = 4 * kFewBlock<XT> + 16;
+    a.tiles = (a.n + 15) / 16;
+    // wavefronts that share a tile's columns: enough for 16 wavefronts a compute unit, but not more than it has stretches
+    const int wanted = cu_count() * 16;
+    a.split_shift = 0;
+    while (a.split_shift < 3 && (static_cast<int64_t>(a.tiles) << a.split_shift) < wanted && (2 << a.split_shift) <= quads) ++a.split_shift;
+    const int waves = (static_cast<int64_t>(a.tiles) << a.split_shift) >= wanted / 2 ? 8 : std::max(4, 1 << a.split_shift);
+    // whole rows of x in LDS if they fit, else as many stretches as do, a multiple of what the wavefronts take in a turn
+    const int most = (kMostLds / held - kFewPad<XT>) / quad_bytes;
+    while (quads > most && (1 << a.split_shift) > most) --a.split_shift;
+    a.chunk_quads = quads <= most ? quads : most >> a.split_shift << a.split_shift;
+    const int side = waves >> a.split_shift;
+    a.sets = (a.tiles + side - 1) / side;
+    const int lds = held * (a.chunk_quads * quad_bytes + kFewPad<XT>);
+    int per_row_tile = a.sets;
+    if (quads <= most && a.sets > cu_count()) {
+        // workgroups that stay for all their tiles: as many as the device holds
+        int fit = 0;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&fit, matvec4_few_kernel<XT, ST, GS, ROWS>, waves * 64, lds) != hipSuccess || fit < 1) fit = 1;
+        per_row_tile = std::min(a.sets, cu_count() * fit);
+    }
+    // a dispatch counts its work-items in 32 bits: 2^22 workgroups at a time
+    const int64_t row_tiles = (a.rows + ROWS - 1) / ROWS, step = std::max<int64_t>(1, (int64_t(1) << 22) / per_row_tile);
+    const int type = a.out_type, rows = a.rows;
+    for (int64_t at = 0; at < row_tiles; at += step) {
+        MatvecArgs part = a;
+        const int64_t row = at * ROWS;
+        part.rows = static_cast<int>(std::min<int64_t>(rows - row, step * ROWS));
+        part.x = static_cast<const XT*>(a.x) + row * a.x_stride;
+        if (a.x_scales) part.x_scales = a.x_scales + row;
+        part.out = static_cast<uint8_t*>(a.out) + row * a.n * type_bytes(type);
+        launch_lds(kIdMatvec4, bytes, matvec4_few_kernel<XT, ST, GS, ROWS>, static_cast<int>(per_row_tile * ((part.rows + ROWS - 1) / ROWS)), waves * 64, lds,
+                   st, part);
+    }
+}
+
 template <typename XT, typename ST>
 void launch_matvec(const MatvecArgs& a, int group, double bytes, hipStream_t st) {
     auto go = [&](auto gs) {
-        if (a.rows <= 4) launch_matvec_as<XT, ST, decltype(gs)::value, 1, 65536>(a, bytes, st);
+        if (a.rows <= 4) launch_matvec_few<XT, ST, decltype(gs)::value, 4>(a, bytes, st);
+        else if constexpr (sizeof(XT) == 1) launch_matvec_few<XT, ST, decltype(gs)::value, 16>(a, bytes, st);
         else launch_matvec_as<XT, ST, decltype(gs)::value, 4, 65536>(a, bytes, st);
     };
     if (group == 32) go(std::integral_constant<int, 5>{});

@@ -97,19 +97,19 @@ __global__ __launch_bounds__(256) void group4_unpack_kernel(UnpackArgs a) {
 //
 //   y[m][n] = x_scale[m] * sum over groups g of scale[n][g] * sum over k in g of q[n][k] x[m][k]
 //
-// Rows of x are the A operand of 16 x 16 x 32 matrix instructions (16 x 16 x 64 for int8), 16 outputs n the B
-// operand: a lane holds eight consecutive k of one n, which is one 32-bit word of codes, so the codes go from memory to the
-// matrix cores through registers alone, eight instructions a word:
-//   bf16   a code's four bits, its sign bit flipped, in the middle of the mantissa of 16.0: that is 24 + q.  The 24 is taken off
-//          by a product of the same rows with -24, on the matrix cores too, which is where the sums start from
-//   fp16   the same
-//   fp32   a row is the sum of three bf16 rows exactly (8 bits of the mantissa each), so three products
-//   int8   a code in the upper half of a byte is 16 q; sums are exact integers, the 16 is taken off at the end
-// A wavefront takes 128 columns of 16 outputs at a time: lane (n, quarter) loads 16 bytes of row n.  With groups of 128 any
-// order of k within them does; with smaller ones the words are transposed between the quarters (four instructions for
-// four words), so that an instruction's 32 columns lie in one group and its sums can be scaled on their own.
-// The wavefronts of a workgroup split the columns; their sums meet in LDS.  The rows of x are brought to LDS once a workgroup,
-// in the order in which the codes come out of their words.
+// Everything is whole numbers up to the end of a group.  Codes become bytes by two masks and a shift a word of eight: a code in
+// the upper half of a byte is 16 q.  int8 rows are taken as they are.  Floating rows become fixed point under the largest
+// magnitude of each 128 columns, in base 256 digits of -128 .. 127: three digits for bf16 and fp16 (23 bits, so a value within
+// 2^-24 of a bound of the largest, what a 32-bit sum with it would keep), four for fp32 (31 bits).  A product's sums are
+// exact in each digit; the digits' sums are put together and scaled in fp32.
+// (The other way, codes widened to bf16 or fp16 for the rows as they are, takes 8 instructions a word instead of 3 and an offset's
+// second product: 1 x 8192 x 128000 bf16 114 us.)
+//
+// Rows of x are the A operand of 16 x 16 x 64 matrix instructions, 16 outputs n the B operand.  A wavefront takes 128 columns
+// of 16 outputs at a time: lane (n, quarter) loads 16 bytes of row n, so codes go from memory to the matrix cores through
+// registers alone.  With groups of 128 any order of k within them does; with smaller ones the words are transposed between the
+// quarters (four instructions for four words), so that an instruction's columns lie in one group and its sums can be
+// scaled on their own.  The rows of x are brought to LDS once a workgroup, in the order in which codes come out of their words.
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -391,6 +391,214 @@ __global__ __launch_bounds__(512) void matvec4_kernel(MatvecArgs a) {
                     if (m < rows && n < a.n) store_product(a, static_cast<int64_t>(row0 + m) * a.n + n, sizeof(XT) == 1 ? v * (a.x_scales[row0 + m] * 0.0625f) : v);
                 }
             }
+        }
+    }
+}
+
+// ---- up to four floating rows, or 16 of int8: whole numbers up to the end of a group ----
+
+// Digits in base 256 that a value is taken to.
+template <typename XT> constexpr int kDigits = sizeof(XT) == 1 ? 1 : 4;
+// Bytes of a row's 128 columns in LDS: [quarter][half][digit][16 columns], so that the lanes of a quarter, which read the digits of
+// one row side by side, read 64 consecutive bytes.  Rows lie 64 bytes off the banks' period (int8: 16).
+template <typename XT> constexpr int kFewBlock = 128 * kDigits<XT>;
+template <typename XT> constexpr int kFewPad = 16 * kDigits<XT>;
+
+// Largest of the 16 lanes of a row of 16.
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+#pragma unroll
+    for (int m = 8; m >= 1; m >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, 64)));
+    return v;
+}
+
+// Eight columns c * 8 .. of a row as digits, most significant first, bytes in the order 0 2 4 6 1 3 5 7; the 16 lanes of 128
+// columns call it together.  Returns the unit of the last digit (NaN, and zeros, if a column is not finite).
+template <typename XT>
+__device__ __forceinline__ float digits8(const XT* __restrict__ row, int64_t i, int n, u32x2 (&out)[kDigits<XT>]) {
+    if constexpr (sizeof(XT) == 1) {
+        uint32_t lo = 0, hi = 0;
+        if (i + 8 <= n) {
+            const U64U t = *reinterpret_cast<const U64U*>(row + i);
+            lo = t.lo;
+            hi = t.hi;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (i + e < n) (e < 4 ? lo : hi) |= static_cast<uint32_t>(static_cast<uint8_t>(row[i + e])) << (8 * (e & 3));
+        }
+        out[0] = u32x2{__builtin_amdgcn_perm(hi, lo, 0x06040200u), __builtin_amdgcn_perm(hi, lo, 0x07050301u)};
+        return 1.0f;
+    } else {
+        float x[8];
+        if (i < n) {
+            load8(row, static_cast<int>(i), n, x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+        top = row16_max(top);
+        // all magnitudes lie below 2^e; the last digit counts in units of 2^(e - 30).  (e stays above -95, so that the unit is a normal
+        // number: what such a row loses is below 2^-126.)
+        const int e2 = max(static_cast<int>(top >> 23) - 126, -95);
+        const bool fine = top < 0x7f800000u;
+        int v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fine ? static_cast<int>(__builtin_rintf(__builtin_ldexpf(x[e], 30 - e2))) : 0;
+#pragma unroll
+        for (int d = 3; d >= 0; --d) {
+            uint32_t b[2];
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+                const uint32_t p = __builtin_amdgcn_perm(v[2 + o], v[o], 0x0c0c0400u), q = __builtin_amdgcn_perm(v[6 + o], v[4 + o], 0x04000c0cu);
+                b[o] = p | q;
+            }
+            out[d] = u32x2{b[0], b[1]};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (v[e] + 128) >> 8;      // what the digit leaves: its byte counts as -128 .. 127
+        }
+        return fine ? __builtin_ldexpf(1.0f, e2 - 30) : __builtin_nanf("");
+    }
+}
+
+template <typename XT, typename ST, int GS, int ROWS>
+__global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
+    constexpr bool kInt = sizeof(XT) == 1;
+    constexpr int NG = 1 << (7 - GS);
+    constexpr int kBlock = kFewBlock<XT>, D = kDigits<XT>;
+    constexpr int IR = ROWS / 4;                                         // sums of a lane
+    static_assert(kInt || ROWS == 4, "a row of four digits takes four rows of the A operand");
+    extern __shared__ __align__(16) uint8_t few_lds[];
+    __shared__ float part[2][8 * IR * 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4, v16 = lane & 15;
+    const int split = 1 << a.split_shift, kpart = wave & (split - 1);
+    const int side = static_cast<int>(blockDim.x >> 6) >> a.split_shift;                    // tiles at a time
+    const int per_row_tile = gridDim.x / ((a.rows + ROWS - 1) / ROWS);                       // workgroups of a row tile
+    const int row0 = blockIdx.x / per_row_tile * ROWS, set0 = blockIdx.x % per_row_tile;
+    const int rows = min(a.rows - row0, ROWS);
+    const int quads = (a.k + 511) >> 9;
+    const int row_stride = a.chunk_quads * 4 * kBlock + kFewPad<XT>;
+    float* units = reinterpret_cast<float*>(few_lds + rows * row_stride);                    // [row][block of 128 columns]
+    // a lane's row of the A operand: digit v16 & 3 of row v16 >> 2; with 16 int8 rows the row v16.  Rows that do not exist repeat
+    // the last one; their sums are dropped
+    const int my_row = min(ROWS == 16 ? v16 : v16 >> 2, rows - 1);
+    const uint8_t* mine = few_lds + my_row * row_stride + (kInt ? quarter * 32 : quarter * 128 + (v16 & 3) * 16);
+    const float* unit = units + min(quarter, rows - 1) * (a.chunk_quads * 4);
+    const ST* scales = static_cast<const ST*>(a.scales);
+    u32x4 w[4], w2[4];
+    QuadScales<ST, GS> s, s2;
+    auto fetch = [&](int set, int q, u32x4 (&to)[4], QuadScales<ST, GS>& sc) {
+        const int64_t n = min((set * side + (wave >> a.split_shift)) * 16 + v16, a.n - 1);
+        typedef u32x4 __attribute__((aligned(1))) u32x4u;
+        const uint8_t* p = a.packed + n * a.p_stride + static_cast<int64_t>(q) * 256 + quarter * 16;
+        const ST* sp = scales + n * a.s_stride + static_cast<int64_t>(q) * (4 * NG);
+        if ((q + 1) * 256 <= a.row_bytes) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) to[u] = *reinterpret_cast<const u32x4u*>(p + 64 * u);
+            sc.load(sp);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                to[u] = q * 256 + u * 64 + quarter * 16 < a.row_bytes ? *reinterpret_cast<const u32x4u*>(p + 64 * u) : u32x4{0, 0, 0, 0};
+            sc.load_some(sp, a.groups - q * (4 * NG));
+        }
+    };
+    const XT* x = static_cast<const XT*>(a.x) + static_cast<int64_t>(row0) * a.x_stride;
+    // Where a wavefront starts in its tile's columns: tiles side by side start at different ones, else all rows of
+    // a matrix whose row length is a power of two would be read at the same offset at a time, from the same memory channels.
+    const bool whole = a.chunk_quads >= quads;
+    const int own = (quads - kpart + split - 1) >> a.split_shift;
+    auto start = [&](int set) { return whole ? kpart + ((set * side + (wave >> a.split_shift)) % own << a.split_shift) : kpart; };
+    int at = start(set0);
+    fetch(set0, at, w, s);
+    int turn = 0;
+    for (int set = set0; set < a.sets; set += per_row_tile, turn ^= 1) {
+        float y[IR];
+#pragma unroll
+        for (int i = 0; i < IR; ++i) y[i] = 0.0f;
+        for (int first = 0; first < quads; first += a.chunk_quads) {
+            const int held = min(a.chunk_quads, quads - first);
+            if (set == set0 || held < quads) {
+                if (set != set0 || first) __syncthreads();
+                // rows of x to LDS: eight columns a lane, put where the lane that multiplies them will look
+                for (int i = threadIdx.x; i < rows * held * 64; i += blockDim.x) {
+                    const int m = i / (held * 64), c = i - m * (held * 64);
+                    u32x2 v[D];
+                    const float last = digits8(x + m * a.x_stride, static_cast<int64_t>(first) * 512 + c * 8, a.k, v);
+                    // eighth `in` of a block: with groups of 128 a quarter's four lie side by side, else they are a quarter apart
+                    const int in = c & 15, q = GS == 7 ? in >> 2 : in & 3, j = GS == 7 ? in & 3 : in >> 2;
+                    uint8_t* to = few_lds + m * row_stride + (c >> 4) * kBlock + q * 32 * D + (j >> 1) * 16 * D + (j & 1) * 8;
+#pragma unroll
+                    for (int d = 0; d < D; ++d) *reinterpret_cast<u32x2*>(to + 16 * d) = v[d];
+                    if (!kInt && in == 0) units[m * (a.chunk_quads * 4) + (c >> 4)] = last;
+                }
+                __syncthreads();
+            }
+            for (int i = kpart; i < held; i += split) {
+                const int q = at - first;
+                const bool more = first + i + split < quads;
+                const int next_set = more ? set : min(set + per_row_tile, a.sets - 1);
+                at = !more ? start(next_set) : at + split < quads ? at + split : kpart;
+                fetch(next_set, at, w2, s2);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    u32x4 c = w[u];
+                    if constexpr (GS < 7) transpose_quarters(c);
+                    i32x4 acc[NG];
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) acc[g] = i32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + (q * 4 + u) * kBlock + j * 16 * D);
+                        const u32x4 b{(c[2 * j] << 4) & 0xf0f0f0f0u, c[2 * j] & 0xf0f0f0f0u, (c[2 * j + 1] << 4) & 0xf0f0f0f0u, c[2 * j + 1] & 0xf0f0f0f0u};
+                        if constexpr (GS == 5) {
+                            const u32x2 a0{xa[0], xa[1]}, a1{xa[2], xa[3]}, b0{b[0], b[1]}, b1{b[2], b[3]};
+                            acc[2 * j] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a0), __builtin_bit_cast(long, b0), acc[2 * j], 0, 0, 0);
+                            acc[2 * j + 1] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a1), __builtin_bit_cast(long, b1), acc[2 * j + 1], 0, 0, 0);
+                        } else {
+                            const int g = GS == 6 ? j : 0;
+                            acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, xa), __builtin_bit_cast(i32x4, b), acc[g], 0, 0, 0);
+                        }
+                    }
+                    if constexpr (kInt) {
+#pragma unroll
+                        for (int g = 0; g < NG; ++g)
+#pragma unroll
+                            for (int r = 0; r < IR; ++r) y[r] = fmaf(static_cast<float>(acc[g][r]), s.at(u * NG + g), y[r]);
+                    } else {
+                        // a digit's sum stays below 2^21: two digits go together in 32 bits, exactly
+                        float t = 0.0f;
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) {
+                            const float hi = static_cast<float>(acc[g][0] * 256 + acc[g][1]), lo = static_cast<float>(acc[g][2] * 256 + acc[g][3]);
+                            t = fmaf(fmaf(hi, 65536.0f, lo), s.at(u * NG + g), t);
+                        }
+                        y[0] = fmaf(t, unit[q * 4 + u], y[0]);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) w[u] = w2[u];
+                s = s2;
+            }
+        }
+        const int n = (set * side + (wave >> a.split_shift)) * 16 + v16;
+        if (split > 1) {
+            // the wavefronts' sums, added in their order; two buffers in turn, so that one barrier a set is enough
+#pragma unroll
+            for (int i = 0; i < IR; ++i) part[turn][(wave * IR + i) * 64 + lane] = y[i];
+            __syncthreads();
+            if (kpart) continue;
+#pragma unroll
+            for (int i = 0; i < IR; ++i)
+                for (int p = 1; p < split; ++p) y[i] += part[turn][((wave + p) * IR + i) * 64 + lane];
+        }
+#pragma unroll
+        for (int i = 0; i < IR; ++i) {
+            const int m = quarter * IR + i;
+            // codes were multiplied as 16 q
+            if (m < rows && n < a.n) store_product(a, static_cast<int64_t>(row0 + m) * a.n + n, kInt ? y[i] * (a.x_scales[row0 + m] * 0.0625f) : y[i] * 0.0625f);
         }
     }
 }

@@ -197,22 +197,27 @@ Profiler g_prof;
 // Every kernel launch of the library goes through here.  With timing on, the launch carries a
 // start and a stop event that take the dispatch's own begin and end timestamps (the same
 // interval a kernel trace reports); otherwise it is a plain launch.
+// (launch_lds: with that many bytes of LDS beyond what the kernel declares.)
 template <typename... KArgs, typename... Args>
-void launch(int id, double algo_bytes, void (*kernel)(KArgs...), int grid, int threads, hipStream_t st, Args... args) {
+void launch_lds(int id, double algo_bytes, void (*kernel)(KArgs...), int grid, int threads, int lds, hipStream_t st, Args... args) {
     if (!g_prof.on) {
-        hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, static_cast<KArgs>(args)...);
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, st, static_cast<KArgs>(args)...);
         return;
     }
     TimedLaunch t{};
     t.id = id;
     t.bytes = algo_bytes;
     if (hipEventCreate(&t.a) != hipSuccess || hipEventCreate(&t.b) != hipSuccess) {
-        hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, static_cast<KArgs>(args)...);
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, st, static_cast<KArgs>(args)...);
         return;
     }
-    hipExtLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, t.a, t.b, 0, static_cast<KArgs>(args)...);
+    hipExtLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, st, t.a, t.b, 0, static_cast<KArgs>(args)...);
     std::lock_guard<std::mutex> lock(g_prof.m);
     g_prof.launches.push_back(t);
+}
+template <typename... KArgs, typename... Args>
+void launch(int id, double algo_bytes, void (*kernel)(KArgs...), int grid, int threads, hipStream_t st, Args... args) {
+    launch_lds(id, algo_bytes, kernel, grid, threads, 0, st, args...);
 }
 
 // Calls f with the store policy as a compile-time constant.
