@@ -404,11 +404,26 @@ template <typename XT> constexpr int kDigits = sizeof(XT) == 1 ? 1 : 4;
 template <typename XT> constexpr int kFewBlock = 128 * kDigits<XT>;
 template <typename XT> constexpr int kFewPad = 16 * kDigits<XT>;
 
-// Largest of the 16 lanes of a row of 16.
+// Largest of the 16 lanes of a row of 16, in all of them: data-parallel moves, no LDS traffic.
+template <int N>
+__device__ __forceinline__ uint32_t row16_turned(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(v), static_cast<int>(v), 0x120 + N, 0xf, 0xf, false));     // row_ror:N
+}
 __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
-#pragma unroll
-    for (int m = 8; m >= 1; m >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, 64)));
-    return v;
+    v = max(v, row16_turned<8>(v));
+    v = max(v, row16_turned<4>(v));
+    v = max(v, row16_turned<2>(v));
+    return max(v, row16_turned<1>(v));
+}
+
+// Bytes of four words by their place: out[d] holds byte 3 - d of a, b, c and e, lowest first.
+__device__ __forceinline__ void transpose_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t e, uint32_t (&out)[4]) {
+    const uint32_t ab_lo = __builtin_amdgcn_perm(b, a, 0x05010400u), ab_hi = __builtin_amdgcn_perm(b, a, 0x07030602u);     // a0 b0 a1 b1, a2 b2 a3 b3
+    const uint32_t ce_lo = __builtin_amdgcn_perm(e, c, 0x05010400u), ce_hi = __builtin_amdgcn_perm(e, c, 0x07030602u);
+    out[3] = __builtin_amdgcn_perm(ce_lo, ab_lo, 0x05040100u);
+    out[2] = __builtin_amdgcn_perm(ce_lo, ab_lo, 0x07060302u);
+    out[1] = __builtin_amdgcn_perm(ce_hi, ab_hi, 0x05040100u);
+    out[0] = __builtin_amdgcn_perm(ce_hi, ab_hi, 0x07060302u);
 }
 
 // Eight columns c * 8 .. of a row as digits, most significant first, bytes in the order 0 2 4 6 1 3 5 7; the 16 lanes of 128
@@ -444,21 +459,18 @@ __device__ __forceinline__ float digits8(const XT* __restrict__ row, int64_t i, 
         // number: what such a row loses is below 2^-126.)
         const int e2 = max(static_cast<int>(top >> 23) - 126, -95);
         const bool fine = top < 0x7f800000u;
-        int v[8];
+        const float up = fine ? __builtin_ldexpf(1.0f, 30 - e2) : 0.0f;      // NaN and infinity times zero convert to zero
+        uint32_t v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fine ? static_cast<int>(__builtin_rintf(__builtin_ldexpf(x[e], 30 - e2))) : 0;
-#pragma unroll
-        for (int d = 3; d >= 0; --d) {
-            uint32_t b[2];
-#pragma unroll
-            for (int o = 0; o < 2; ++o) {
-                const uint32_t p = __builtin_amdgcn_perm(v[2 + o], v[o], 0x0c0c0400u), q = __builtin_amdgcn_perm(v[6 + o], v[4 + o], 0x04000c0cu);
-                b[o] = p | q;
-            }
-            out[d] = u32x2{b[0], b[1]};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (v[e] + 128) >> 8;      // what the digit leaves: its byte counts as -128 .. 127
+        for (int e = 0; e < 8; ++e) {
+            // half of 256 added at each digit but the first carries into the next where the byte is to count as negative
+            v[e] = (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(x[e] * up))) + 0x00808080u) ^ 0x00808080u;
         }
+        uint32_t even[4], odd[4];
+        transpose_bytes(v[0], v[2], v[4], v[6], even);
+        transpose_bytes(v[1], v[3], v[5], v[7], odd);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) out[d] = u32x2{even[d], odd[d]};
         return fine ? __builtin_ldexpf(1.0f, e2 - 30) : __builtin_nanf("");
     }
 }
