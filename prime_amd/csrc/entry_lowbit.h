@@ -89,40 +89,6 @@ bool bad_group(int group) { return group != 32 && group != 64 && group != 128; }
 bool bad_matrix(int64_t n, int64_t k) { return n < 0 || n >= (int64_t(1) << 40) || k < 1 || k > kMaxDim; }
 int group_shift(int group) { return group == 32 ? 5 : group == 64 ? 6 : 7; }
 
-template <typename XT, typename ST, int GS, int IR, int XBYTES>
-void launch_matvec_as(MatvecArgs a, double bytes, hipStream_t st) {
-    const int row_tile = IR == 1 ? 4 : 16, held = std::min(a.rows, row_tile) * Held<XT>::kPlanes, quads = (a.k + 511) / 512;
-    const int quad_bytes = 64 * static_cast<int>(sizeof(typename Held<XT>::type));
-    a.tiles = (a.n + 15) / 16;
-    // wavefronts that share a tile's columns: enough for 16 wavefronts a compute unit, but not more than it has stretches
-    const int wanted = cu_count() * 16;
-    a.split_shift = 0;
-    while (a.split_shift < 3 && (a.tiles << a.split_shift) < wanted && (2 << a.split_shift) <= quads) ++a.split_shift;
-    const int waves = (static_cast<int64_t>(a.tiles) << a.split_shift) >= wanted / 2 ? 8 : std::max(4, 1 << a.split_shift);
-    // whole rows of x in LDS if they fit, else as many stretches as do, a multiple of what the wavefronts take in a turn
-    const int most = (XBYTES / held - 16) / quad_bytes;
-    while (quads > most && (1 << a.split_shift) > most) --a.split_shift;
-    a.chunk_quads = quads <= most ? quads : most >> a.split_shift << a.split_shift;
-    const int side = waves >> a.split_shift;
-    a.sets = (a.tiles + side - 1) / side;
-    const int resident = std::max(1, cu_count() * 16 / waves);
-    // a dispatch counts its work-items in 32 bits: 2^22 workgroups at a time
-    const int64_t row_tiles = (a.rows + row_tile - 1) / row_tile;
-    const int per_row_tile = quads <= most ? std::min(a.sets, resident) : a.sets;
-    const int64_t step = std::max<int64_t>(1, (int64_t(1) << 22) / per_row_tile);
-    const int type = a.out_type, rows = a.rows;
-    for (int64_t at = 0; at < row_tiles; at += step) {
-        MatvecArgs part = a;
-        const int64_t row = at * row_tile;
-        part.rows = static_cast<int>(std::min(rows - row, step * row_tile));
-        part.x = static_cast<const XT*>(a.x) + row * a.x_stride;
-        if (a.x_scales) part.x_scales = a.x_scales + row;
-        part.out = static_cast<uint8_t*>(a.out) + row * a.n * type_bytes(type);
-        launch(kIdMatvec4, bytes, matvec4_kernel<XT, ST, GS, IR, XBYTES>, static_cast<int>(per_row_tile * ((part.rows + row_tile - 1) / row_tile)), waves * 64,
-               st, part);
-    }
-}
-
 // Up to four floating rows at a time, or 16 of int8.
 template <typename XT, typename ST, int GS, int ROWS>
 void launch_matvec_few(MatvecArgs a, double bytes, hipStream_t st) {
@@ -163,12 +129,49 @@ void launch_matvec_few(MatvecArgs a, double bytes, hipStream_t st) {
     }
 }
 
-template <typename XT, typename ST>
-void launch_matvec(const MatvecArgs& a, int group, double bytes, hipStream_t st) {
+template <typename XT, int GS, int MT, int SPLIT>
+void launch_matvec_many_as(MatvecArgs a, bool scale_bf16, double bytes, hipStream_t st) {
+    a.sets = (a.n + 32 * (8 / SPLIT) - 1) / (32 * (8 / SPLIT));
+    constexpr int kRows = 16 * MT;
+    const int64_t row_tiles = (a.rows + kRows - 1) / kRows, step = std::max<int64_t>(1, (int64_t(1) << 22) / a.sets);
+    const int type = a.out_type, rows = a.rows;
+    for (int64_t at = 0; at < row_tiles; at += step) {
+        MatvecArgs part = a;
+        const int64_t row = at * kRows;
+        part.rows = static_cast<int>(std::min<int64_t>(rows - row, step * kRows));
+        part.x = static_cast<const XT*>(a.x) + row * a.x_stride;
+        if (a.x_scales) part.x_scales = a.x_scales + row;
+        part.out = static_cast<uint8_t*>(a.out) + row * a.n * type_bytes(type);
+        launch(kIdMatvec4, bytes, matvec4_many_kernel<XT, GS, MT, SPLIT>, static_cast<int>(a.sets * ((part.rows + kRows - 1) / kRows)), 512, st, part,
+               static_cast<int>(scale_bf16));
+    }
+}
+
+template <typename XT, int GS>
+void launch_matvec_many(const MatvecArgs& a, bool scale_bf16, double bytes, hipStream_t st) {
+    const int64_t pairs = (a.n + 31) / 32;
+    if (a.rows <= 16) {
+        if (pairs * 2 >= cu_count() * 8) launch_matvec_many_as<XT, GS, 1, 2>(a, scale_bf16, bytes, st);
+        else launch_matvec_many_as<XT, GS, 1, sizeof(XT) == 4 ? 4 : 8>(a, scale_bf16, bytes, st);
+    } else if (a.rows <= 32 || sizeof(XT) == 4) {
+        if (pairs * 2 >= cu_count() * 8) launch_matvec_many_as<XT, GS, 2, 1>(a, scale_bf16, bytes, st);
+        else launch_matvec_many_as<XT, GS, 2, sizeof(XT) == 4 ? 2 : 4>(a, scale_bf16, bytes, st);
+    } else if constexpr (sizeof(XT) < 4) {
+        launch_matvec_many_as<XT, GS, 4, 2>(a, scale_bf16, bytes, st);
+    }
+}
+
+template <typename XT>
+void launch_matvec(const MatvecArgs& a, int group, int scale_type, double bytes, hipStream_t st) {
     auto go = [&](auto gs) {
-        if (a.rows <= 4) launch_matvec_few<XT, ST, decltype(gs)::value, 4>(a, bytes, st);
-        else if constexpr (sizeof(XT) == 1) launch_matvec_few<XT, ST, decltype(gs)::value, 16>(a, bytes, st);
-        else launch_matvec_as<XT, ST, decltype(gs)::value, 4, 65536>(a, bytes, st);
+        constexpr int GS = decltype(gs)::value;
+        with_scale_type(scale_type, [&](auto s) {
+            if (a.rows <= 4) launch_matvec_few<XT, decltype(s), GS, 4>(a, bytes, st);
+            else if constexpr (sizeof(XT) == 1) {
+                if (a.rows <= 16) launch_matvec_few<XT, decltype(s), GS, 16>(a, bytes, st);
+            }
+        });
+        if (a.rows > (sizeof(XT) == 1 ? 16 : 4)) launch_matvec_many<XT, GS>(a, scale_type == PRIME_BF16, bytes, st);
     };
     if (group == 32) go(std::integral_constant<int, 5>{});
     else if (group == 64) go(std::integral_constant<int, 6>{});
@@ -301,9 +304,7 @@ int prime_matvec_4bit(const void* x, int64_t x_stride, int x_type, const float* 
                  static_cast<int>(groups * group / 2), static_cast<int>(groups), out_type, 0, 0, 0, 0};
     const double bytes = static_cast<double>(n) * k / 2 + static_cast<double>(n) * groups * type_bytes(scale_type) +
                          static_cast<double>(rows) * (k * type_bytes(x_type) + n * type_bytes(out_type));
-    auto go = [&](auto t) {
-        with_scale_type(scale_type, [&](auto s) { launch_matvec<decltype(t), decltype(s)>(a, group, bytes, static_cast<hipStream_t>(stream)); });
-    };
+    auto go = [&](auto t) { launch_matvec<decltype(t)>(a, group, scale_type, bytes, static_cast<hipStream_t>(stream)); };
     if (x_type == PRIME_I8) go(int8_t{});
     else with_float_type(x_type, go);
     return launch_check("matvec4_kernel");

@@ -137,59 +137,6 @@ struct MatvecArgs {
     int split_shift;            // log2 of the wavefronts that share a tile's columns
 };
 
-// Sums of one step: fp32, or exact integers.
-template <typename XT> struct Sum { typedef f32x4 type; };
-template <> struct Sum<int8_t> { typedef i32x4 type; };
-
-// How eight columns of a row of x are held in LDS: 16-bit values in the order 0 4 1 5 2 6 3 7, bytes in the order
-// 0 2 4 6 1 3 5 7; fp32 as three bf16 planes, each the leading bits of what the ones before leave.
-template <typename XT> struct Held { typedef u32x4 type; static constexpr int kPlanes = 1; };
-template <> struct Held<float> { typedef u32x4 type; static constexpr int kPlanes = 3; };
-template <> struct Held<int8_t> { typedef u32x2 type; static constexpr int kPlanes = 1; };
-
-__device__ __forceinline__ uint32_t pair16(uint32_t lo, uint32_t hi) { return (lo & 0xffffu) | hi << 16; }
-
-template <typename XT>
-__device__ __forceinline__ void hold8(const XT* __restrict__ row, int i, int n, typename Held<XT>::type (&out)[Held<XT>::kPlanes]) {
-    if constexpr (sizeof(XT) == 1) {
-        uint32_t lo = 0, hi = 0;
-        if (i + 8 <= n) {
-            const U64U t = *reinterpret_cast<const U64U*>(row + i);
-            lo = t.lo;
-            hi = t.hi;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (i + e < n) (e < 4 ? lo : hi) |= static_cast<uint32_t>(static_cast<uint8_t>(row[i + e])) << (8 * (e & 3));
-        }
-        out[0] = u32x2{__builtin_amdgcn_perm(hi, lo, 0x06040200u), __builtin_amdgcn_perm(hi, lo, 0x07050301u)};
-    } else if constexpr (sizeof(XT) == 2) {
-        uint16_t v[8];
-        if (i + 8 <= n) {
-            const typename Eight<XT>::type t = *reinterpret_cast<const typename Eight<XT>::type*>(row + i);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = __builtin_bit_cast(uint16_t, static_cast<XT>(t[e]));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = i + e < n ? __builtin_bit_cast(uint16_t, row[i + e]) : uint16_t(0);
-        }
-        out[0] = u32x4{pair16(v[0], v[4]), pair16(v[1], v[5]), pair16(v[2], v[6]), pair16(v[3], v[7])};
-    } else {
-        float v[8];
-        load8(row, i, n, v);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-            uint32_t b[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                b[e] = __float_as_uint(v[e]) >> 16;
-                v[e] -= __uint_as_float(b[e] << 16);      // exact: the bits that are left
-            }
-            out[p] = u32x4{pair16(b[0], b[4]), pair16(b[1], b[5]), pair16(b[2], b[6]), pair16(b[3], b[7])};
-        }
-    }
-}
-
 // new[j] of quarter q = old[q] of quarter j
 __device__ __forceinline__ void transpose_quarters(u32x4& w) {
     const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
@@ -210,8 +157,6 @@ __device__ __forceinline__ u32x4 widen_word(uint32_t w) {
         return u32x4{((w << 6) & kMask) ^ kBase, ((w << 2) & kMask) ^ kBase, ((w >> 2) & kMask) ^ kBase, ((w >> 6) & kMask) ^ kBase};
     }
 }
-constexpr uint32_t kOffsetBf16 = 0xc1c0c1c0u, kOffsetF16 = 0xce00ce00u;      // -24 twice
-
 template <typename XT>
 __device__ __forceinline__ f32x4 product(u32x4 rows, u32x4 codes, f32x4 c) {
     if constexpr (std::is_same<XT, _Float16>::value)
@@ -219,10 +164,6 @@ __device__ __forceinline__ f32x4 product(u32x4 rows, u32x4 codes, f32x4 c) {
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, rows), __builtin_bit_cast(bf16x8, codes), c, 0, 0, 0);
 }
-
-// Which row of x a row of the A operand is: with up to 4 rows every fourth (a lane's first of four sums is then the one that
-// counts, the others are not used), else all 16.  Rows that do not exist repeat the last one; their sums are dropped.
-template <int IR> __device__ __forceinline__ int row_of(int v) { return IR == 1 ? v >> 2 : v; }
 
 // Scales of the groups of 512 columns of one output, as they are stored.
 template <typename ST, int GS> struct QuadScales {
@@ -237,162 +178,10 @@ template <typename ST, int GS> struct QuadScales {
     __device__ __forceinline__ float at(int i) const { return static_cast<float>(v[i]); }
 };
 
-// 128 columns of 16 outputs against the rows at `mine` in LDS, added to y: `scale(g)` is the factor of group g of them.
-template <typename XT, int GS, int IR, typename Scale>
-__device__ __forceinline__ void add_block(u32x4 v, const uint8_t* mine, int plane_stride, Scale scale, float (&y)[IR]) {
-    constexpr int NG = 1 << (7 - GS);
-    constexpr int kPlanes = Held<XT>::kPlanes;
-    if constexpr (GS < 7) transpose_quarters(v);
-    typename Sum<XT>::type acc[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) acc[g] = typename Sum<XT>::type{0, 0, 0, 0};
-    if constexpr (sizeof(XT) == 1) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + 16 * j);
-            const u32x4 b{(v[2 * j] << 4) & 0xf0f0f0f0u, v[2 * j] & 0xf0f0f0f0u, (v[2 * j + 1] << 4) & 0xf0f0f0f0u, v[2 * j + 1] & 0xf0f0f0f0u};
-            if constexpr (GS == 5) {
-                const u32x2 a0{xa[0], xa[1]}, a1{xa[2], xa[3]}, b0{b[0], b[1]}, b1{b[2], b[3]};
-                acc[2 * j] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a0), __builtin_bit_cast(long, b0), acc[2 * j], 0, 0, 0);
-                acc[2 * j + 1] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a1), __builtin_bit_cast(long, b1), acc[2 * j + 1], 0, 0, 0);
-            } else {
-                const int g = GS == 6 ? j : 0;
-                acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, xa), __builtin_bit_cast(i32x4, b), acc[g], 0, 0, 0);
-            }
-        }
-    } else {
-        constexpr bool kBf16 = !std::is_same<XT, _Float16>::value;
-        constexpr uint32_t kOff = kBf16 ? kOffsetBf16 : kOffsetF16;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int g = j >> (GS - 5);
-            const u32x4 b = widen_word<kBf16>(v[j]);
-#pragma unroll
-            for (int p = 0; p < kPlanes; ++p) {
-                const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + p * plane_stride + 16 * j);
-                acc[g] = product<XT>(xa, u32x4{kOff, kOff, kOff, kOff}, acc[g]);
-                acc[g] = product<XT>(xa, b, acc[g]);
-            }
-        }
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int i = 0; i < IR; ++i) y[i] = fmaf(static_cast<float>(acc[g][i]), scale(g), y[i]);
-}
-
 __device__ __forceinline__ void store_product(const MatvecArgs& a, int64_t at, float v) {
     if (a.out_type == PRIME_F32) static_cast<float*>(a.out)[at] = v;
     else if (a.out_type == PRIME_BF16) static_cast<__bf16*>(a.out)[at] = static_cast<__bf16>(v);
     else static_cast<_Float16*>(a.out)[at] = static_cast<_Float16>(v);
-}
-
-// Up to 4 (IR 1) or 16 (IR 4) rows.  A wavefront takes a tile of 16 outputs, or every second, fourth or eighth stretch of 512
-// columns of one (split_shift); a workgroup as many tiles side by side as that leaves wavefronts for, set after set.  The next
-// stretch's codes and scales are on their way while one is multiplied, across tiles too.
-template <typename XT, typename ST, int GS, int IR, int XBYTES>
-__global__ __launch_bounds__(512) void matvec4_kernel(MatvecArgs a) {
-    constexpr int kPlanes = Held<XT>::kPlanes;
-    constexpr int NG = 1 << (7 - GS);
-    typedef typename Held<XT>::type held_t;
-    constexpr int kBlock = 16 * static_cast<int>(sizeof(held_t));       // bytes of a row's 128 columns in LDS
-    __shared__ __align__(16) uint8_t lds[XBYTES];
-    __shared__ float part[2][8 * IR * 64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
-    const int split = 1 << a.split_shift, kpart = wave & (split - 1);
-    const int side = static_cast<int>(blockDim.x >> 6) >> a.split_shift;                    // tiles at a time
-    constexpr int kRowTile = IR == 1 ? 4 : 16;
-    const int per_row_tile = gridDim.x / ((a.rows + kRowTile - 1) / kRowTile);               // workgroups of a row tile
-    const int row0 = blockIdx.x / per_row_tile * kRowTile, set0 = blockIdx.x % per_row_tile;
-    const int rows = min(a.rows - row0, kRowTile);
-    const int quads = (a.k + 511) >> 9;
-    const int row_stride = a.chunk_quads * 4 * kBlock + 16;              // 16 bytes more: rows start on other banks
-    const int plane_stride = rows * row_stride;
-    const uint8_t* mine = lds + min(row_of<IR>(lane & 15), rows - 1) * row_stride + quarter * 4 * static_cast<int>(sizeof(held_t));
-    const ST* scales = static_cast<const ST*>(a.scales);
-    u32x4 w[4], w2[4];
-    QuadScales<ST, GS> s, s2;
-    auto fetch = [&](int set, int q, u32x4 (&to)[4], QuadScales<ST, GS>& sc) {
-        const int64_t n = min((set * side + (wave >> a.split_shift)) * 16 + (lane & 15), a.n - 1);
-        typedef u32x4 __attribute__((aligned(1))) u32x4u;
-        const uint8_t* p = a.packed + n * a.p_stride + static_cast<int64_t>(q) * 256 + quarter * 16;
-        const ST* sp = scales + n * a.s_stride + static_cast<int64_t>(q) * (4 * NG);
-        if ((q + 1) * 256 <= a.row_bytes) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u) to[u] = *reinterpret_cast<const u32x4u*>(p + 64 * u);
-            sc.load(sp);
-        } else {
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                to[u] = q * 256 + u * 64 + quarter * 16 < a.row_bytes ? *reinterpret_cast<const u32x4u*>(p + 64 * u) : u32x4{0, 0, 0, 0};
-            sc.load_some(sp, a.groups - q * (4 * NG));
-        }
-    };
-    const XT* x = static_cast<const XT*>(a.x) + static_cast<int64_t>(row0) * a.x_stride;
-    // Where a wavefront starts in its tile's columns: tiles side by side start at different ones, else all rows of
-    // a matrix whose row length is a power of two would be read at the same offset at a time, from the same memory channels.
-    const bool whole = a.chunk_quads >= quads;
-    const int own = (quads - kpart + split - 1) >> a.split_shift;
-    auto start = [&](int set) { return whole ? kpart + ((set * side + (wave >> a.split_shift)) % own << a.split_shift) : kpart; };
-    int at = start(set0);
-    fetch(set0, at, w, s);
-    int turn = 0;
-    for (int set = set0; set < a.sets; set += per_row_tile, turn ^= 1) {
-        float y[IR];
-#pragma unroll
-        for (int i = 0; i < IR; ++i) y[i] = 0.0f;
-        for (int first = 0; first < quads; first += a.chunk_quads) {
-            const int held = min(a.chunk_quads, quads - first);
-            if (set == set0 || held < quads) {
-                if (set != set0 || first) __syncthreads();
-                // rows of x to LDS: eight columns a lane, put where the lane that multiplies them will look
-                for (int i = threadIdx.x; i < rows * held * 64; i += blockDim.x) {
-                    const int m = i / (held * 64), c = i - m * (held * 64);
-                    held_t v[kPlanes];
-                    hold8(x + m * a.x_stride, first * 512 + c * 8, a.k, v);
-                    const int in = c & 15, to = (c & ~15) | (GS == 7 ? in : (in & 3) * 4 + (in >> 2));
-#pragma unroll
-                    for (int p = 0; p < kPlanes; ++p) *reinterpret_cast<held_t*>(lds + p * plane_stride + m * row_stride + to * static_cast<int>(sizeof(held_t))) = v[p];
-                }
-                __syncthreads();
-            }
-            for (int i = kpart; i < held; i += split) {
-                const int q = at - first;
-                const bool more = first + i + split < quads;
-                const int next_set = more ? set : min(set + per_row_tile, a.sets - 1);
-                at = !more ? start(next_set) : at + split < quads ? at + split : kpart;
-                fetch(next_set, at, w2, s2);
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    add_block<XT, GS, IR>(w[u], mine + (q * 4 + u) * kBlock, plane_stride, [&](int g) { return s.at(u * NG + g); }, y);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) w[u] = w2[u];
-                s = s2;
-            }
-        }
-        const int n = (set * side + (wave >> a.split_shift)) * 16 + (lane & 15);
-        if (split == 1) {
-#pragma unroll
-            for (int i = 0; i < IR; ++i) {
-                const int m = quarter * IR + i;
-                if (m < rows && n < a.n) store_product(a, static_cast<int64_t>(row0 + m) * a.n + n, sizeof(XT) == 1 ? y[i] * (a.x_scales[row0 + m] * 0.0625f) : y[i]);
-            }
-        } else {
-            // the wavefronts' sums, added in their order; two buffers in turn, so that one barrier a set is enough
-#pragma unroll
-            for (int i = 0; i < IR; ++i) part[turn][(wave * IR + i) * 64 + lane] = y[i];
-            __syncthreads();
-            if (kpart == 0) {
-#pragma unroll
-                for (int i = 0; i < IR; ++i) {
-                    float v = y[i];
-                    for (int p = 1; p < split; ++p) v += part[turn][((wave + p) * IR + i) * 64 + lane];
-                    const int m = quarter * IR + i;
-                    if (m < rows && n < a.n) store_product(a, static_cast<int64_t>(row0 + m) * a.n + n, sizeof(XT) == 1 ? v * (a.x_scales[row0 + m] * 0.0625f) : v);
-                }
-            }
-        }
-    }
 }
 
 // ---- up to four floating rows, or 16 of int8: whole numbers up to the end of a group ----
@@ -611,6 +400,333 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
             const int m = quarter * IR + i;
             // codes were multiplied as 16 q
             if (m < rows && n < a.n) store_product(a, static_cast<int64_t>(row0 + m) * a.n + n, kInt ? y[i] * (a.x_scales[row0 + m] * 0.0625f) : y[i] * 0.0625f);
+        }
+    }
+}
+
+// ---- more rows: 16, 32 or 64 at a time ----
+// Here the matrix cores' work grows with the rows and the rows are taken as they are: bf16 and fp16 codes are widened beside an
+// offset (widen_word()), the sums of a group start from what the offset adds, taken off; fp32 rows are three bf16 rows,
+// which together are exact; int8 as above.  A wavefront takes 32 outputs, and every SPLIT-th stretch of 256 columns; the rows of
+// the workgroup's next stretches are on their way to registers while LDS holds the ones that are multiplied.
+
+template <typename XT> constexpr int kPlanes = sizeof(XT) == 4 ? 3 : 1;
+template <typename XT> constexpr int kPlaneBytes = sizeof(XT) == 1 ? 1 : 2;      // of an element in LDS
+
+__device__ __forceinline__ uint32_t pair16(uint32_t lo, uint32_t hi) { return (lo & 0xffffu) | hi << 16; }
+
+// Eight columns of a row as read.
+template <typename XT> struct Raw8 { uint32_t w[8 * sizeof(XT) / 4]; };
+
+template <typename XT>
+__device__ __forceinline__ Raw8<XT> load_raw8(const XT* row, int64_t i, int n) {
+    struct __attribute__((packed, aligned(sizeof(XT)))) Loose { uint32_t w[8 * sizeof(XT) / 4]; };
+    Raw8<XT> r;
+    if (i + 8 <= n) {
+        const Loose t = *reinterpret_cast<const Loose*>(row + i);
+#pragma unroll
+        for (unsigned e = 0; e < 8 * sizeof(XT) / 4; ++e) r.w[e] = t.w[e];
+    } else {
+#pragma unroll
+        for (unsigned e = 0; e < 8 * sizeof(XT) / 4; ++e) r.w[e] = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (i + e < n) {
+                if constexpr (sizeof(XT) == 4) r.w[e] = __builtin_bit_cast(uint32_t, row[i + e]);
+                else if constexpr (sizeof(XT) == 2) r.w[e >> 1] |= static_cast<uint32_t>(__builtin_bit_cast(uint16_t, row[i + e])) << (16 * (e & 1));
+                else r.w[e >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[i + e])) << (8 * (e & 3));
+            }
+    }
+    return r;
+}
+
+// The sum of neighbouring lanes' values over a group's eights (4, 8 or 16 lanes of a row of 16), in all of them.
+template <int GS>
+__device__ __forceinline__ float group_sum(float v) {
+    auto turned = [](float f, auto n) {
+        return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(__float_as_uint(f)), static_cast<int>(__float_as_uint(f)),
+                                                                                 decltype(n)::value, 0xf, 0xf, false)));
+    };
+    v += turned(v, std::integral_constant<int, 0xb1>{});            // quad_perm 1 0 3 2
+    v += turned(v, std::integral_constant<int, 0x4e>{});            // quad_perm 2 3 0 1
+    if constexpr (GS >= 6) v += turned(v, std::integral_constant<int, 0x141>{});     // row_half_mirror: the other four of eight
+    if constexpr (GS == 7) v += turned(v, std::integral_constant<int, 0x140>{});     // row_mirror: the other eight
+    return v;
+}
+
+// f(0), f(1), ... with the index a constant: registers are indexed by it.
+template <int N, typename F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) { each_of<N>(static_cast<F&&>(f), std::make_integer_sequence<int, N>{}); }
+
+template <typename XT, int GS, int MT, int SPLIT>
+__global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a, int scale_bf16) {
+    constexpr bool kInt = sizeof(XT) == 1;
+    constexpr int P = kPlanes<XT>, E8 = 8 * kPlaneBytes<XT>;               // bytes of eight columns in LDS
+    constexpr int NG = 1 << (7 - GS), NT = 2, BW = 2;
+    constexpr int kBlocks = BW * SPLIT;                                    // blocks of 128 columns in LDS
+    constexpr int kRows = 16 * MT;
+    constexpr int kRowBytes = kBlocks * 16 * E8 + 16;                      // 16 bytes more: rows start on other banks
+    constexpr int kEach = kRows * kBlocks * 16 / 512;                      // eights of x a lane brings
+    constexpr int kSide = 8 / SPLIT;
+    static_assert(kEach >= 1 && kRows * kBlocks * 16 % 512 == 0, "whole rounds of the workgroup");
+    constexpr int kRowArea = P * kRows * kRowBytes, kSumArea = 8 * NT * 256 * 4 * (SPLIT > 1);
+    __shared__ __align__(16) uint8_t lds[kRowArea > kSumArea ? kRowArea : kSumArea];
+    __shared__ __align__(16) float starts[kInt ? 1 : kBlocks * NG * kRows];       // [group][row]: -24 times the sum of its columns
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4, v16 = lane & 15;
+    const int kpart = wave % SPLIT, col = wave / SPLIT;
+    const int set = blockIdx.x % a.sets, row0 = blockIdx.x / a.sets * kRows;
+    const int rows = min(a.rows - row0, kRows);
+    const int blocks = (a.k + 127) >> 7, chunks = (blocks + kBlocks - 1) / kBlocks;
+    const XT* x = static_cast<const XT*>(a.x) + static_cast<int64_t>(row0) * a.x_stride;
+    typedef u32x4 __attribute__((aligned(1))) u32x4u;
+    int n0[NT];
+    const uint8_t* codes[NT];
+    int64_t scale_row[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        n0[t] = ((set * kSide + col) * NT + t) * 16 + v16;
+        const int64_t n = min(n0[t], a.n - 1);
+        codes[t] = a.packed + n * a.p_stride + quarter * 16;
+        scale_row[t] = n * a.s_stride;
+    }
+    auto fetch_codes = [&](int chunk, u32x4 (&w)[NT][BW], uint32_t (&s)[NT][BW * NG]) {
+        const int b = chunk * kBlocks + kpart * BW;
+        const int there = a.groups - b * NG;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if ((b + BW) * 64 <= a.row_bytes) {
+#pragma unroll
+                for (int u = 0; u < BW; ++u) w[t][u] = *reinterpret_cast<const u32x4u*>(codes[t] + static_cast<int64_t>(b + u) * 64);
+            } else {
+#pragma unroll
+                for (int u = 0; u < BW; ++u)
+                    w[t][u] = (b + u) * 64 + quarter * 16 < a.row_bytes ? *reinterpret_cast<const u32x4u*>(codes[t] + static_cast<int64_t>(b + u) * 64) : u32x4{0, 0, 0, 0};
+            }
+            // scales as stored; behind the last group zeros
+            if (scale_bf16) {
+                const uint16_t* p = static_cast<const uint16_t*>(a.scales) + scale_row[t] + static_cast<int64_t>(b) * NG;
+                if (there >= BW * NG) {
+                    typedef uint16_t __attribute__((ext_vector_type(BW * NG), aligned(2))) some;
+                    const some v = *reinterpret_cast<const some*>(p);
+#pragma unroll
+                    for (int g = 0; g < BW * NG; ++g) s[t][g] = v[g];
+                } else {
+#pragma unroll
+                    for (int g = 0; g < BW * NG; ++g) s[t][g] = g < there ? p[g] : 0u;
+                }
+            } else {
+                const uint32_t* p = static_cast<const uint32_t*>(a.scales) + scale_row[t] + static_cast<int64_t>(b) * NG;
+                if (there >= BW * NG) {
+                    typedef uint32_t __attribute__((ext_vector_type(BW * NG), aligned(4))) some;
+                    const some v = *reinterpret_cast<const some*>(p);
+#pragma unroll
+                    for (int g = 0; g < BW * NG; ++g) s[t][g] = v[g];
+                } else {
+#pragma unroll
+                    for (int g = 0; g < BW * NG; ++g) s[t][g] = g < there ? p[g] : 0u;
+                }
+            }
+        }
+    };
+    const int scale_shift = scale_bf16 ? 16 : 0;
+    auto widen_scales = [&](const uint32_t (&from)[NT][BW * NG], float (&to)[NT][BW * NG]) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int g = 0; g < BW * NG; ++g) to[t][g] = __uint_as_float(from[t][g] << scale_shift);
+    };
+    // A lane's eights of x: 16 lanes side by side take 128 columns of a row.
+    auto fetch_rows = [&](int chunk, Raw8<XT> (&r)[kEach]) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int i = threadIdx.x + e * 512, m = i / (kBlocks * 16), c = i % (kBlocks * 16);
+            r[e] = load_raw8(x + static_cast<int64_t>(min(m, rows - 1)) * a.x_stride, static_cast<int64_t>(chunk) * (kBlocks * 128) + c * 8, a.k);
+        }
+    };
+    auto put_rows = [&](const Raw8<XT> (&r)[kEach]) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int i = threadIdx.x + e * 512, m = i / (kBlocks * 16), c = i % (kBlocks * 16), in = c & 15;
+            uint8_t* to = lds + m * kRowBytes + ((c & ~15) | (GS == 7 ? in : (in & 3) * 4 + (in >> 2))) * E8;
+            const auto& w = r[e].w;
+            if constexpr (kInt) {
+                *reinterpret_cast<u32x2*>(to) = u32x2{__builtin_amdgcn_perm(w[1], w[0], 0x06040200u), __builtin_amdgcn_perm(w[1], w[0], 0x07050301u)};
+            } else {
+                float v[8];
+                if constexpr (sizeof(XT) == 2) {
+                    // 0 4, 1 5, 2 6, 3 7
+                    *reinterpret_cast<u32x4*>(to) = u32x4{__builtin_amdgcn_perm(w[2], w[0], 0x05040100u), __builtin_amdgcn_perm(w[2], w[0], 0x07060302u),
+                                                          __builtin_amdgcn_perm(w[3], w[1], 0x05040100u), __builtin_amdgcn_perm(w[3], w[1], 0x07060302u)};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        v[k] = static_cast<float>(__builtin_bit_cast(XT, static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1)))));
+                } else {
+                    float left[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) left[k] = v[k] = __uint_as_float(w[k]);
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        uint32_t b[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            b[k] = __float_as_uint(left[k]) >> 16;
+                            left[k] -= __uint_as_float(b[k] << 16);      // exact: the bits that are left
+                        }
+                        *reinterpret_cast<u32x4*>(to + p * kRows * kRowBytes) = u32x4{pair16(b[0], b[4]), pair16(b[1], b[5]), pair16(b[2], b[6]), pair16(b[3], b[7])};
+                    }
+                }
+                const float sum = group_sum<GS>(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])));
+                if (in % (1 << (GS - 3)) == 0) starts[(c >> (GS - 3)) * kRows + m] = -24.0f * sum;
+            }
+        }
+    };
+    float y[NT][MT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[t][m][i] = 0.0f;
+    u32x4 w[NT][BW];
+    uint32_t s2[NT][BW * NG];
+    float s[NT][BW * NG];
+    Raw8<XT> r[kEach];
+    fetch_codes(0, w, s2);
+    fetch_rows(0, r);
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        if (chunk) __syncthreads();
+        put_rows(r);
+        __syncthreads();
+        u32x4 w2[NT][BW];
+        widen_scales(s2, s);
+        const int next = min(chunk + 1, chunks - 1);
+        fetch_codes(next, w2, s2);
+        fetch_rows(next, r);
+        each<BW>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            const int b = kpart * BW + u;
+            u32x4 v[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                v[t] = w[t][u];
+                if constexpr (GS < 7) transpose_quarters(v[t]);
+            }
+            const uint8_t* mine = lds + v16 * kRowBytes + (b * 16 + quarter * 4) * E8;
+            each<NG>([&](auto gc) {
+                constexpr int g = decltype(gc)::value;
+                constexpr int kSteps = 4 / NG;                       // words of a lane in a group
+                if constexpr (kInt) {
+                    i32x4 acc[NT][MT];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) acc[t][m] = i32x4{0, 0, 0, 0};
+                    constexpr int kPairs = kSteps >= 2 ? kSteps / 2 : 1;
+                    each<kPairs>([&](auto jc) {
+                        u32x4 cb[NT];
+                        constexpr int at = GS == 5 ? g : g * kSteps + 2 * decltype(jc)::value;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            const uint32_t w0 = v[t][at], w1 = GS == 5 ? 0u : v[t][GS == 5 ? at : at + 1];
+                            cb[t] = u32x4{(w0 << 4) & 0xf0f0f0f0u, w0 & 0xf0f0f0f0u, (w1 << 4) & 0xf0f0f0f0u, w1 & 0xf0f0f0f0u};
+                        }
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            if constexpr (GS == 5) {
+                                const u32x2 xa = *reinterpret_cast<const u32x2*>(mine + m * 16 * kRowBytes + at * E8);
+#pragma unroll
+                                for (int t = 0; t < NT; ++t)
+                                    acc[t][m] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, xa), __builtin_bit_cast(long, u32x2{cb[t][0], cb[t][1]}),
+                                                                                      acc[t][m], 0, 0, 0);
+                            } else {
+                                const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + m * 16 * kRowBytes + at * E8);
+#pragma unroll
+                                for (int t = 0; t < NT; ++t)
+                                    acc[t][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, xa), __builtin_bit_cast(i32x4, cb[t]), acc[t][m], 0, 0, 0);
+                            }
+                        }
+                    });
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const float f = s[t][u * NG + g];
+#pragma unroll
+                        for (int m = 0; m < MT; ++m)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) y[t][m][i] = fmaf(static_cast<float>(acc[t][m][i]), f, y[t][m][i]);
+                    }
+                } else {
+                    f32x4 acc[NT][MT];
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const f32x4 start = *reinterpret_cast<const f32x4*>(starts + (b * NG + g) * kRows + m * 16 + quarter * 4);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) acc[t][m] = start;
+                    }
+                    each<kSteps>([&](auto jc) {
+                        constexpr int j = g * kSteps + decltype(jc)::value;
+                        u32x4 cb[NT];
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) cb[t] = widen_word<!std::is_same<XT, _Float16>::value>(v[t][j]);
+#pragma unroll
+                        for (int p = 0; p < P; ++p)
+#pragma unroll
+                            for (int m = 0; m < MT; ++m) {
+                                const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + (p * kRows + m * 16) * kRowBytes + j * E8);
+#pragma unroll
+                                for (int t = 0; t < NT; ++t) acc[t][m] = product<XT>(xa, cb[t], acc[t][m]);
+                            }
+                    });
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const float f = s[t][u * NG + g];
+#pragma unroll
+                        for (int m = 0; m < MT; ++m)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) y[t][m][i] = fmaf(acc[t][m][i], f, y[t][m][i]);
+                    }
+                }
+            });
+        });
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int u = 0; u < BW; ++u) w[t][u] = w2[t][u];
+    }
+    auto put = [&](int t, int m, int i, float v) {
+        const int row = m * 16 + quarter * 4 + i;
+        if (row < rows && n0[t] < a.n) store_product(a, static_cast<int64_t>(row0 + row) * a.n + n0[t], kInt ? v * (a.x_scales[row0 + row] * 0.0625f) : v);
+    };
+    if constexpr (SPLIT == 1) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) put(t, m, i, y[t][m][i]);
+    } else {
+        // the wavefronts' sums, added in their order, 16 rows at a time
+        float* part = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[((wave * NT + t) * 4 + i) * 64 + lane] = y[t][m][i];
+            __syncthreads();
+            // the wavefronts of a tile pair share its eight values a lane
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if ((t * 4 + i) % SPLIT != kpart) continue;
+                    float v = 0.0f;
+#pragma unroll
+                    for (int p = 0; p < SPLIT; ++p) v += part[(((col * SPLIT + p) * NT + t) * 4 + i) * 64 + lane];
+                    put(t, m, i, v);
+                }
         }
     }
 }

@@ -21,6 +21,7 @@
 #include <cstring>
 #include <mutex>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "../../include/prime_hip.h"
