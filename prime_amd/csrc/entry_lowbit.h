@@ -50,7 +50,7 @@ constexpr int kGradRegisterDim = 16384;      // rows up to this long stay in reg
 int grad_lanes(int64_t dim) { return dim <= 1024 ? 64 : dim <= 2048 ? 128 : dim <= 4096 ? 256 : dim <= 8192 ? 512 : 1024; }
 int grad_stretches(int64_t dim) { return static_cast<int>((dim + 2047) / 2048); }
 int64_t grad_groups(int64_t rows, int64_t dim) {
-    int64_t most = dim <= kGradRegisterDim ? static_cast<int64_t>(cu_count()) * (1024 / grad_lanes(dim))
+    int64_t most = dim <= kGradRegisterDim ? static_cast<int64_t>(cu_count()) * std::max(1, 512 / grad_lanes(dim))
                                            : static_cast<int64_t>(cu_count()) * 8 / grad_stretches(dim);
     if (most < 1) most = 1;
     return rows < most ? rows : most;
@@ -82,7 +82,7 @@ void launch_rms_norm_grad(const NormGradArgs& a, int groups, WT* grad_weight, do
             launch(kIdRmsNormGrad, bytes, rms_norm_grad_apply_kernel<XT, WT>, stretches * groups, 256, st, a, dots, stretches, groups);
         }
     }
-    launch(kIdColumnSum, 4.0 * groups * a.dim, column_sum_kernel<WT>, static_cast<int>((a.dim + 15) / 16), 256, st, a.partials, groups, a.dim, grad_weight);
+    launch(kIdColumnSum, 4.0 * groups * a.dim, column_sum_kernel<WT>, static_cast<int>((a.dim + 31) / 32), 1024, st, a.partials, groups, a.dim, grad_weight);
 }
 
 bool bad_group(int group) { return group != 32 && group != 64 && group != 128; }
@@ -253,7 +253,7 @@ int prime_quantize_4bit(const void* weight, int64_t stride, int64_t n, int64_t k
             with_scale_type(scale_type, [&](auto s) {
                 using ST = decltype(s);
                 PackArgs a{static_cast<const T*>(weight) + at * stride, stride, packed + at * eights * 4, static_cast<ST*>(scales) + at * groups,
-                           static_cast<uint32_t>(vectors), static_cast<int>(k), group / 8, FastDiv(static_cast<uint32_t>(eights))};
+                           static_cast<uint32_t>(vectors), static_cast<int>(k), group / 8, group_shift(group) - 3, FastDiv(static_cast<uint32_t>(eights))};
                 launch(kIdGroupPack, static_cast<double>(rows) * (k * sizeof(T) + eights * 4 + groups * sizeof(ST)), group4_pack_kernel<T, ST>,
                        static_cast<int>((vectors + 255) / 256), 256, static_cast<hipStream_t>(stream), a);
             });

@@ -30,6 +30,7 @@ struct PackArgs {
     uint32_t vectors;           // eights of this launch: rows * groups * group / 8
     int k;
     int lanes;                  // eights of a group: 4, 8 or 16
+    int lane_shift;
     FastDiv per_row;            // eights of a row
 };
 
@@ -45,24 +46,36 @@ __global__ __launch_bounds__(256) void group4_pack_kernel(PackArgs a) {
     uint32_t top = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(w[e]) & 0x7fffffffu);
-    for (int m = a.lanes >> 1; m >= 1; m >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), m, 64)));
+    // the largest of the group's 4, 8 or 16 lanes, in all of them
+    auto turned = [](uint32_t v, auto n) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(v), static_cast<int>(v), decltype(n)::value, 0xf, 0xf, false));
+    };
+    top = max(top, turned(top, std::integral_constant<int, 0xb1>{}));                       // quad_perm 1 0 3 2
+    top = max(top, turned(top, std::integral_constant<int, 0x4e>{}));                       // quad_perm 2 3 0 1
+    if (a.lanes > 4) top = max(top, turned(top, std::integral_constant<int, 0x141>{}));     // row_half_mirror: the other four of eight
+    if (a.lanes > 8) top = max(top, turned(top, std::integral_constant<int, 0x140>{}));     // row_mirror: the other eight
     if (!live) return;
     const bool bad = top >= 0x7f800000u;
     const ST stored = bad ? static_cast<ST>(__builtin_nanf("")) : static_cast<ST>(__uint_as_float(top) / 7.0f);
     float s = static_cast<float>(stored);
     uint32_t codes = 0;
     if (s > 0.0f && s < __builtin_inff()) {
-        const float up = s < 0x1p-90f ? 0x1p64f : 1.0f;      // keeps the reciprocal and a residual inside fp32's range
-        s *= up;
-        const float r = 1.0f / s;
+        if (s < 0x1p-90f) {      // keeps the reciprocal and a residual inside fp32's range
+            s *= 0x1p64f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float q = __builtin_amdgcn_fmed3f(nearest_int(w[e] * up, s, r), -7.0f, 7.0f);
-            codes |= (static_cast<uint32_t>(static_cast<int>(q)) & 15u) << (4 * e);
+            for (int e = 0; e < 8; ++e) w[e] *= 0x1p64f;
         }
+        float f[8];
+        round8(w, s, 1.0f / s, f);
+        uint32_t c[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)      // the scale's own rounding can put a quotient above 7, far from 8 unless it is a subnormal number
+            c[e] = __float_as_uint(__builtin_amdgcn_fmed3f(f[e], kRoundToInt - 7.0f, kRoundToInt + 7.0f));
+        const uint32_t even = low_bytes(c[0], c[2], c[4], c[6]) & 0x0f0f0f0fu, odd = low_bytes(c[1], c[3], c[5], c[7]) & 0x0f0f0f0fu;
+        codes = even | odd << 4;
     }
     reinterpret_cast<U32U*>(a.packed)[t].v = codes;
-    if (v % static_cast<uint32_t>(a.lanes) == 0) static_cast<ST*>(a.scales)[t / static_cast<uint32_t>(a.lanes)] = stored;
+    if ((v & (a.lanes - 1)) == 0) static_cast<ST*>(a.scales)[t >> a.lane_shift] = stored;
 }
 
 struct UnpackArgs {
@@ -193,16 +206,12 @@ template <typename XT> constexpr int kDigits = sizeof(XT) == 1 ? 1 : 4;
 template <typename XT> constexpr int kFewBlock = 128 * kDigits<XT>;
 template <typename XT> constexpr int kFewPad = 16 * kDigits<XT>;
 
-// Largest of the 16 lanes of a row of 16, in all of them: data-parallel moves, no LDS traffic.
-template <int N>
-__device__ __forceinline__ uint32_t row16_turned(uint32_t v) {
-    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(v), static_cast<int>(v), 0x120 + N, 0xf, 0xf, false));     // row_ror:N
-}
+// Largest of the 16 lanes of a row of 16, in all of them.
 __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
-    v = max(v, row16_turned<8>(v));
-    v = max(v, row16_turned<4>(v));
-    v = max(v, row16_turned<2>(v));
-    return max(v, row16_turned<1>(v));
+    v = max(v, row_turned<8>(v));
+    v = max(v, row_turned<4>(v));
+    v = max(v, row_turned<2>(v));
+    return max(v, row_turned<1>(v));
 }
 
 // Bytes of four words by their place: out[d] holds byte 3 - d of a, b, c and e, lowest first.

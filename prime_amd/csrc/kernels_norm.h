@@ -20,17 +20,25 @@ template <> struct Eight<__bf16> { typedef __bf16 type __attribute__((ext_vector
 template <> struct Eight<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(8), aligned(2))); };
 struct __attribute__((packed, aligned(1))) U64U { uint32_t lo, hi; };
 
-// Elements i .. i + 7 of a row of n as floats, zero behind its end.
+// Elements i .. i + 7 of a row of n as they are, zero behind its end.
 template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int i, int n, float (&v)[8]) {
+__device__ __forceinline__ typename Eight<T>::type take8(const T* __restrict__ row, int i, int n) {
+    typename Eight<T>::type t;
     if (i + 8 <= n) {
-        const typename Eight<T>::type t = *reinterpret_cast<const typename Eight<T>::type*>(row + i);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(t[e]);
+        t = *reinterpret_cast<const typename Eight<T>::type*>(row + i);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = i + e < n ? static_cast<float>(row[i + e]) : 0.0f;
+        for (int e = 0; e < 8; ++e) t[e] = i + e < n ? row[i + e] : static_cast<T>(0.0f);
     }
+    return t;
+}
+
+// The same as floats.
+template <typename T>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int i, int n, float (&v)[8]) {
+    const typename Eight<T>::type t = take8(row, i, n);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(t[e]);
 }
 
 template <typename T>
@@ -59,9 +67,8 @@ __device__ __forceinline__ void store8_codes(uint8_t* __restrict__ row, int i, i
 }
 
 // The integer nearest z / unit, ties to even, for |z / unit| < 512, with r = 1 / unit rounded and unit normal.
-// t = z r is within 2^-23 |t| of the quotient, less than 2^-14, so away from a border rounding t is right.  Near one (one
-// element in ten thousand) the side is the sign of z - m unit with m the border, which a fused multiply-add
-// rounds once and therefore never gets wrong.
+// t = z r is within 2^-23 |t| of the quotient, less than 2^-14, so away from a border rounding t is right.  Near one the side is
+// the sign of z - m unit with m the border, which a fused multiply-add rounds once and therefore never gets wrong.
 __device__ __forceinline__ float nearest_int(float z, float unit, float r) {
     const float t = z * r;
     float k = __builtin_rintf(t);
@@ -74,10 +81,31 @@ __device__ __forceinline__ float nearest_int(float z, float unit, float r) {
     return k;
 }
 
-// int8 code of z under the scale s.
-__device__ __forceinline__ uint32_t code_int8(float z, float s, float r) {
-    const float k = __builtin_amdgcn_fmed3f(nearest_int(z, s, r), -127.0f, 127.0f);
-    return static_cast<uint32_t>(static_cast<int>(k)) & 0xffu;
+// 1.5 * 2^23: adding it rounds to a whole number, ties to even, which the sum's low byte then holds in two's complement.
+constexpr float kRoundToInt = 12582912.0f;
+constexpr float kNearBorder = 0.5f - 0x1p-14f;
+
+// Eight whole numbers z / unit to the nearest, as what they are plus kRoundToInt.  Elements near a border are rare (one in ten
+// thousand), so all eight share one test, and only then each is looked at on its own.
+__device__ __forceinline__ void round8(const float (&z)[8], float unit, float r, float (&f)[8]) {
+    float d[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        f[e] = __builtin_fmaf(z[e], r, kRoundToInt);
+        d[e] = __builtin_fabsf(__builtin_fmaf(z[e], r, kRoundToInt - f[e]));
+    }
+    if (__builtin_fmaxf(__builtin_fmaxf(__builtin_fmaxf(d[0], d[1]), __builtin_fmaxf(d[2], d[3])), __builtin_fmaxf(__builtin_fmaxf(d[4], d[5]), __builtin_fmaxf(d[6], d[7]))) >
+        kNearBorder) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (d[e] > kNearBorder) f[e] = kRoundToInt + nearest_int(z[e], unit, r);
+    }
+}
+
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x0c0c0400u);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 
 // The e4m3 number nearest z / s, as a float: three mantissa bits, so the integer nearest z / (s step) in units of
@@ -89,40 +117,89 @@ __device__ __forceinline__ float value_e4m3(float z, float s, float r) {
     return __builtin_amdgcn_fmed3f(nearest_int(z, s * step, r * inv_step) * step, -448.0f, 448.0f);
 }
 
-// Codes of eight products, packed.
+// Codes of eight products, packed.  `plain`: no quotient is beyond the largest code (the unit is no subnormal number, whose
+// rounding could put one there).
 template <bool FP8>
-__device__ __forceinline__ void codes8(const float (&z)[8], float s, float r, uint32_t& lo, uint32_t& hi) {
-    uint32_t w[2];
+__device__ __forceinline__ void codes8(const float (&z)[8], float s, float r, bool plain, uint32_t& lo, uint32_t& hi) {
+    float f[8];
+    if constexpr (FP8) {
+        // The conversion rounds to the nearest, ties to even, and z r is within two steps of 2^-24 of the quotient: only what lies
+        // that near a border, half way between neighbours (a one and 19 zeros below the three bits that stay), is looked at again.
+        // Below 2^-6 the borders are those of the numbers 2^-6 higher.
+        uint32_t near = 0xffffffffu;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        if constexpr (FP8) {
-            // the values are e4m3 numbers: the conversion rounds nothing
-            int p = __builtin_amdgcn_cvt_pk_fp8_f32(value_e4m3(z[4 * q], s, r), value_e4m3(z[4 * q + 1], s, r), 0, false);
-            w[q] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(value_e4m3(z[4 * q + 2], s, r), value_e4m3(z[4 * q + 3], s, r), p, true));
-        } else {
-            w[q] = code_int8(z[4 * q], s, r) | code_int8(z[4 * q + 1], s, r) << 8 | code_int8(z[4 * q + 2], s, r) << 16 |
-                   code_int8(z[4 * q + 3], s, r) << 24;
+        for (int e = 0; e < 8; ++e) {
+            f[e] = z[e] * r;
+            const float m = __builtin_fabsf(f[e]);
+            const uint32_t bits = __float_as_uint(m < 0x1p-6f ? m + 0x1p-6f : m);
+            near = min(near, (bits & 0xfffffu) - 0x7fff8u);
         }
+        if (near <= 16u || !plain) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = value_e4m3(z[e], s, r);
+        }
+        int p = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+        lo = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], p, true));
+        p = __builtin_amdgcn_cvt_pk_fp8_f32(f[4], f[5], 0, false);
+        hi = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(f[6], f[7], p, true));
+    } else {
+        round8(z, s, r, f);
+        if (!plain) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = __builtin_amdgcn_fmed3f(f[e], kRoundToInt - 127.0f, kRoundToInt + 127.0f);
+        }
+        lo = low_bytes(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        hi = low_bytes(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
     }
-    lo = w[0];
-    hi = w[1];
 }
 
-// Sum over the lanes of a wavefront, the same value in every lane (a fixed butterfly).
-__device__ __forceinline__ double wave_sum_all(double v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-    return v;
+// Reductions over a wavefront whose result every lane holds: within rows of 16 by data-parallel moves, across them by lane
+// swaps; no LDS traffic.  Sums are taken in a fixed tree, in which the two sides of an addition only trade places from lane to lane.
+template <int N>
+__device__ __forceinline__ uint32_t row_turned(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(v), static_cast<int>(v), 0x120 + N, 0xf, 0xf, false));     // row_ror:N
+}
+template <int N> __device__ __forceinline__ float row_turned(float v) { return __uint_as_float(row_turned<N>(__float_as_uint(v))); }
+template <int N> __device__ __forceinline__ double row_turned(double v) {
+    const long long b = __double_as_longlong(v);
+    const uint32_t lo = row_turned<N>(static_cast<uint32_t>(b)), hi = row_turned<N>(static_cast<uint32_t>(b >> 32));
+    return __longlong_as_double(static_cast<long long>(hi) << 32 | lo);
+}
+// f(v of one half, v of the other), likewise for neighbouring rows of 16.
+template <typename F> __device__ __forceinline__ uint32_t across_rows(uint32_t v, F&& f) {
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t w = f(static_cast<uint32_t>(h[0]), static_cast<uint32_t>(h[1]));
+    const auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    return f(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
 }
 __device__ __forceinline__ float wave_sum_all(float v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-    return v;
+    v += row_turned<8>(v);
+    v += row_turned<4>(v);
+    v += row_turned<2>(v);
+    v += row_turned<1>(v);
+    return __uint_as_float(across_rows(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+__device__ __forceinline__ double wave_sum_all(double v) {
+    v += row_turned<8>(v);
+    v += row_turned<4>(v);
+    v += row_turned<2>(v);
+    v += row_turned<1>(v);
+    auto join = [](uint32_t hi, uint32_t lo) { return __longlong_as_double(static_cast<long long>(hi) << 32 | lo); };
+    long long b = __double_as_longlong(v);
+    const auto l = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(b), static_cast<uint32_t>(b), false, false);
+    const auto h = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(b >> 32), static_cast<uint32_t>(b >> 32), false, false);
+    v = join(h[0], l[0]) + join(h[1], l[1]);
+    b = __double_as_longlong(v);
+    const auto m = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(b), static_cast<uint32_t>(b), false, false);
+    const auto n = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(b >> 32), static_cast<uint32_t>(b >> 32), false, false);
+    return join(n[0], m[0]) + join(n[1], m[1]);
 }
 __device__ __forceinline__ uint32_t wave_max_all(uint32_t v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, 64)));
-    return v;
+    v = max(v, row_turned<8>(v));
+    v = max(v, row_turned<4>(v));
+    v = max(v, row_turned<2>(v));
+    v = max(v, row_turned<1>(v));
+    return across_rows(v, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
 struct NormArgs {
@@ -226,10 +303,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_row_kernel(Nor
         if (i >= a.dim) break;
         uint32_t lo = 0, hi = 0;
         if (!q.none) {
+            const bool plain = q.up == 1.0f;
+            if (!plain) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[j][e] *= q.up;
-            if (a.fp8) codes8<true>(z[j], q.s, q.r, lo, hi);
-            else codes8<false>(z[j], q.s, q.r, lo, hi);
+                for (int e = 0; e < 8; ++e) z[j][e] *= q.up;
+            }
+            if (a.fp8) codes8<true>(z[j], q.s, q.r, plain, lo, hi);
+            else codes8<false>(z[j], q.s, q.r, plain, lo, hi);
         }
         store8_codes(cr, i, a.dim, lo, hi);
     }
@@ -285,8 +365,8 @@ __global__ __launch_bounds__(1024) void rms_norm_loop_kernel(NormArgs a) {
             load8(wr, i, a.dim, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) z[e] = z[e] * w[e] * q.up;
-            if (a.fp8) codes8<true>(z, q.s, q.r, lo, hi);
-            else codes8<false>(z, q.s, q.r, lo, hi);
+            if (a.fp8) codes8<true>(z, q.s, q.r, q.up == 1.0f, lo, hi);
+            else codes8<false>(z, q.s, q.r, q.up == 1.0f, lo, hi);
         }
         store8_codes(cr, i, a.dim, lo, hi);
     }
@@ -310,12 +390,35 @@ struct NormGradArgs {
     int dim;
 };
 
-// A workgroup of TPR lanes takes rows blockIdx.x, + gridDim.x, ...; a lane keeps its columns' share of dw in
-// registers over all of them, so dw costs one store of a row per workgroup.
+// A workgroup of TPR lanes takes rows blockIdx.x, + gridDim.x, ...; a lane keeps its columns' share of dw in registers over
+// all of them, so dw costs one store of a row per workgroup.  The next row is on its way while one is worked on.
 template <typename XT, typename WT, int TPR, int V>
 __global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
     __shared__ float sh[2][TPR / 64];
+    typedef typename Eight<XT>::type eight;
     const int lane = threadIdx.x;
+    const XT* grad = static_cast<const XT*>(a.grad);
+    const XT* hidden = static_cast<const XT*>(a.hidden);
+    const XT* grad_hidden = static_cast<const XT*>(a.grad_hidden);
+    eight g0[V], h0[V], d0[V];
+    float inv0;
+    auto fetch = [&](int64_t row) {
+        inv0 = a.inv_rms[row];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            g0[j] = take8(grad + row * a.g_stride, (lane + j * TPR) * 8, a.dim);
+            h0[j] = take8(hidden + row * a.h_stride, (lane + j * TPR) * 8, a.dim);
+        }
+        if (grad_hidden) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) d0[j] = take8(grad_hidden + row * a.gh_stride, (lane + j * TPR) * 8, a.dim);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d0[j][e] = static_cast<XT>(0.0f);
+    fetch(blockIdx.x);
     float dw[V][8], w[V][8];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -323,21 +426,27 @@ __global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) dw[j][e] = 0.0f;
     }
+    const float over_dim = 1.0f / static_cast<float>(a.dim);
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-        const float inv = a.inv_rms[row];
+        const float inv = inv0;
         float g[V][8], h[V][8];
+        eight d[V];
         float c = 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            load8(static_cast<const XT*>(a.grad) + row * a.g_stride, (lane + j * TPR) * 8, a.dim, g[j]);
-            load8(static_cast<const XT*>(a.hidden) + row * a.h_stride, (lane + j * TPR) * 8, a.dim, h[j]);
+            d[j] = d0[j];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                g[j][e] = static_cast<float>(g0[j][e]);
+                h[j][e] = static_cast<float>(h0[j][e]) * inv;      // the normalised row
+            }
         }
+        fetch(row + gridDim.x < a.rows ? row + gridDim.x : row);
 #pragma unroll
         for (int j = 0; j < V; ++j)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                h[j][e] *= inv;                                    // the normalised row
                 dw[j][e] = fmaf(g[j][e], h[j][e], dw[j][e]);
                 g[j][e] *= w[j][e];
                 c = fmaf(g[j][e], h[j][e], c);
@@ -351,15 +460,12 @@ __global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
 #pragma unroll
             for (int q = 1; q < TPR / 64; ++q) c += sh[turn][q];
         }
-        c /= static_cast<float>(a.dim);
+        c *= over_dim;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int i = (lane + j * TPR) * 8;
-            float dh[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (a.grad_hidden) load8(static_cast<const XT*>(a.grad_hidden) + row * a.gh_stride, i, a.dim, dh);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) g[j][e] = fmaf(inv, fmaf(-h[j][e], c, g[j][e]), dh[e]);
-            store8(static_cast<XT*>(a.grad_x) + row * a.dim, i, a.dim, g[j]);
+            for (int e = 0; e < 8; ++e) g[j][e] = fmaf(inv, fmaf(-h[j][e], c, g[j][e]), static_cast<float>(d[j][e]));
+            store8(static_cast<XT*>(a.grad_x) + row * a.dim, (lane + j * TPR) * 8, a.dim, g[j]);
         }
     }
 #pragma unroll
@@ -414,20 +520,29 @@ __global__ __launch_bounds__(256) void rms_norm_grad_apply_kernel(NormGradArgs a
     store8(a.partials + static_cast<int64_t>(band) * a.dim, i, a.dim, dw);
 }
 
-// dw[i] = the sum of the workgroups' shares in their order: 16 columns a workgroup, 16 lanes a column.
+// dw[i] = the sum of the workgroups' shares: 32 columns a workgroup, each by 32 lanes whose sums are added in their order.
 template <typename WT>
-__global__ __launch_bounds__(256) void column_sum_kernel(const float* __restrict__ partials, int groups, int dim, WT* __restrict__ out) {
-    __shared__ double sh[16][17];
-    const int c = threadIdx.x & 15, part = threadIdx.x >> 4;
-    const int64_t col = static_cast<int64_t>(blockIdx.x) * 16 + c;
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restrict__ partials, int groups, int dim, WT* __restrict__ out) {
+    __shared__ double sh[32][33];
+    const int c = threadIdx.x & 31, part = threadIdx.x >> 5;
+    const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + c;
     double s = 0.0;
-    if (col < dim)
-        for (int g = part; g < groups; g += 16) s += static_cast<double>(partials[static_cast<int64_t>(g) * dim + col]);
+    if (col < dim) {
+        const float* p = partials + col;
+        int g = part;
+        // four on their way at a time
+        for (; g + 96 < groups; g += 128) {
+            const float a = p[static_cast<int64_t>(g) * dim], b = p[static_cast<int64_t>(g + 32) * dim], d = p[static_cast<int64_t>(g + 64) * dim],
+                        e = p[static_cast<int64_t>(g + 96) * dim];
+            s += (static_cast<double>(a) + b) + (static_cast<double>(d) + e);
+        }
+        for (; g < groups; g += 32) s += static_cast<double>(p[static_cast<int64_t>(g) * dim]);
+    }
     sh[part][c] = s;
     __syncthreads();
     if (part == 0 && col < dim) {
 #pragma unroll
-        for (int q = 1; q < 16; ++q) s += sh[q][c];
+        for (int q = 1; q < 32; ++q) s += sh[q][c];
         out[col] = static_cast<WT>(static_cast<float>(s));
     }
 }
