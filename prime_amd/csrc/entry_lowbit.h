@@ -255,7 +255,7 @@ int prime_quantize_4bit(const void* weight, int64_t stride, int64_t n, int64_t k
                 PackArgs a{static_cast<const T*>(weight) + at * stride, stride, packed + at * eights * 4, static_cast<ST*>(scales) + at * groups,
                            static_cast<uint32_t>(vectors), static_cast<int>(k), group / 8, group_shift(group) - 3, FastDiv(static_cast<uint32_t>(eights))};
                 launch(kIdGroupPack, static_cast<double>(rows) * (k * sizeof(T) + eights * 4 + groups * sizeof(ST)), group4_pack_kernel<T, ST>,
-                       static_cast<int>((vectors + 255) / 256), 256, static_cast<hipStream_t>(stream), a);
+                       static_cast<int>((vectors + 256 * kPackEach - 1) / (256 * kPackEach)), 256, static_cast<hipStream_t>(stream), a);
             });
         });
         if (int rc = launch_check("group4_pack_kernel")) return rc;
@@ -280,7 +280,7 @@ int prime_dequantize_4bit(const uint8_t* packed, int64_t packed_stride, const vo
                 UnpackArgs a{packed + at * packed_stride, static_cast<const ST*>(scales) + at * scale_stride, static_cast<T*>(out) + at * k, packed_stride,
                              scale_stride, static_cast<uint32_t>(vectors), static_cast<int>(k), group_shift(group) - 3, FastDiv(static_cast<uint32_t>(eights))};
                 launch(kIdGroupUnpack, static_cast<double>(rows) * (k * (sizeof(T) + 0.5)), group4_unpack_kernel<T, ST>,
-                       static_cast<int>((vectors + 255) / 256), 256, static_cast<hipStream_t>(stream), a);
+                       static_cast<int>((vectors + 256 * kUnpackEach - 1) / (256 * kUnpackEach)), 256, static_cast<hipStream_t>(stream), a);
             });
         });
         if (int rc = launch_check("group4_unpack_kernel")) return rc;

@@ -34,15 +34,15 @@ struct PackArgs {
     FastDiv per_row;            // eights of a row
 };
 
-// A lane takes eight elements, a group's lanes sit side by side in a wavefront.
+constexpr int kPackEach = 2;
+
+// One eight of the matrix (number t, the v-th of its row) to codes, and its group's scale.
 template <typename T, typename ST>
-__global__ __launch_bounds__(256) void group4_pack_kernel(PackArgs a) {
-    const uint32_t t = blockIdx.x * 256u + threadIdx.x;
+__device__ __forceinline__ void pack8(const PackArgs& a, uint32_t t, uint32_t v, const typename Eight<T>::type& raw) {
     const bool live = t < a.vectors;
-    const uint32_t row = a.per_row.quotient(live ? t : 0u);
-    const uint32_t v = (live ? t : 0u) - row * a.per_row.d;
     float w[8];
-    load8(static_cast<const T*>(a.weight) + row * a.stride, static_cast<int>(v * 8), a.k, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = static_cast<float>(raw[e]);
     uint32_t top = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(w[e]) & 0x7fffffffu);
@@ -78,6 +78,22 @@ __global__ __launch_bounds__(256) void group4_pack_kernel(PackArgs a) {
     if ((v & (a.lanes - 1)) == 0) static_cast<ST*>(a.scales)[t >> a.lane_shift] = stored;
 }
 
+// A lane takes eight elements at a time, a group's lanes sit side by side in a wavefront; two loads are on their way at a time.
+template <typename T, typename ST>
+__global__ __launch_bounds__(256) void group4_pack_kernel(PackArgs a) {
+    typename Eight<T>::type raw[kPackEach];
+    uint32_t col[kPackEach];
+#pragma unroll
+    for (int i = 0; i < kPackEach; ++i) {
+        const uint32_t t = (blockIdx.x * kPackEach + i) * 256u + threadIdx.x, in = t < a.vectors ? t : 0u;
+        const uint32_t row = a.per_row.quotient(in);
+        col[i] = in - row * a.per_row.d;
+        raw[i] = take8(static_cast<const T*>(a.weight) + row * a.stride, static_cast<int>(col[i] * 8), a.k);
+    }
+#pragma unroll
+    for (int i = 0; i < kPackEach; ++i) pack8<T, ST>(a, (blockIdx.x * kPackEach + i) * 256u + threadIdx.x, col[i], raw[i]);
+}
+
 struct UnpackArgs {
     const uint8_t* packed;
     const void* scales;
@@ -90,20 +106,31 @@ struct UnpackArgs {
     FastDiv per_row;            // eights of a row of the output
 };
 
+constexpr int kUnpackEach = 2;       // eights of a lane, all on their way together
+
 // Code e of a word of eight, as an integer.
 __device__ __forceinline__ int code4(uint32_t word, int e) { return static_cast<int>(word << (28 - 4 * e)) >> 28; }
 
 template <typename T, typename ST>
 __global__ __launch_bounds__(256) void group4_unpack_kernel(UnpackArgs a) {
-    const uint32_t t = blockIdx.x * 256u + threadIdx.x;
-    if (t >= a.vectors) return;
-    const uint32_t row = a.per_row.quotient(t), v = t - row * a.per_row.d;
-    const uint32_t word = reinterpret_cast<const U32U*>(a.packed + row * a.p_stride)[v].v;
-    const float s = load_scale(static_cast<const ST*>(a.scales) + row * a.s_stride + (v >> a.lane_shift));
-    float o[8];
+    uint32_t row[kUnpackEach], v[kUnpackEach], word[kUnpackEach];
+    float s[kUnpackEach];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(code4(word, e)) * s;
-    store8(static_cast<T*>(a.out) + static_cast<int64_t>(row) * a.k, static_cast<int>(v * 8), a.k, o);
+    for (int i = 0; i < kUnpackEach; ++i) {
+        const uint32_t t = min((blockIdx.x * kUnpackEach + i) * 256u + threadIdx.x, a.vectors - 1);
+        row[i] = a.per_row.quotient(t);
+        v[i] = t - row[i] * a.per_row.d;
+        word[i] = reinterpret_cast<const U32U*>(a.packed + row[i] * a.p_stride)[v[i]].v;
+        s[i] = load_scale(static_cast<const ST*>(a.scales) + row[i] * a.s_stride + (v[i] >> a.lane_shift));
+    }
+#pragma unroll
+    for (int i = 0; i < kUnpackEach; ++i) {
+        if ((blockIdx.x * kUnpackEach + i) * 256u + threadIdx.x >= a.vectors) return;
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(code4(word[i], e)) * s[i];
+        store8(static_cast<T*>(a.out) + static_cast<int64_t>(row[i]) * a.k, static_cast<int>(v[i] * 8), a.k, o);
+    }
 }
 
 // ---- products of a few rows with 4-bit weights, on the matrix cores ----

@@ -396,6 +396,7 @@ template <typename XT, typename WT, int TPR, int V>
 __global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
     __shared__ float sh[2][TPR / 64];
     typedef typename Eight<XT>::type eight;
+    constexpr bool kAhead = TPR < 1024;        // the 128 registers of 1024 lanes do not hold another row
     const int lane = threadIdx.x;
     const XT* grad = static_cast<const XT*>(a.grad);
     const XT* hidden = static_cast<const XT*>(a.hidden);
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
     for (int j = 0; j < V; ++j)
 #pragma unroll
         for (int e = 0; e < 8; ++e) d0[j][e] = static_cast<XT>(0.0f);
-    fetch(blockIdx.x);
+    if (kAhead) fetch(blockIdx.x);
     float dw[V][8], w[V][8];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -429,6 +430,7 @@ __global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
     const float over_dim = 1.0f / static_cast<float>(a.dim);
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        if (!kAhead) fetch(row);
         const float inv = inv0;
         float g[V][8], h[V][8];
         eight d[V];
@@ -442,7 +444,7 @@ __global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
                 h[j][e] = static_cast<float>(h0[j][e]) * inv;      // the normalised row
             }
         }
-        fetch(row + gridDim.x < a.rows ? row + gridDim.x : row);
+        if (kAhead) fetch(row + gridDim.x < a.rows ? row + gridDim.x : row);
 #pragma unroll
         for (int j = 0; j < V; ++j)
 #pragma unroll
