@@ -36,16 +36,38 @@ struct PackArgs {
 
 constexpr int kPackEach = 2;
 
+// The largest magnitude of eight elements, as the bits of a float; a NaN compares above all numbers.
+template <typename T>
+__device__ __forceinline__ uint32_t largest_bits(const typename Eight<T>::type& v);
+template <>
+__device__ __forceinline__ uint32_t largest_bits<float>(const Eight<float>::type& v) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+    return top;
+}
+// 16-bit types: two at a time, as whole numbers.
+template <typename T>
+__device__ __forceinline__ uint32_t largest_bits(const typename Eight<T>::type& v) {
+    typedef uint16_t __attribute__((ext_vector_type(2))) u16x2;
+    typedef uint32_t __attribute__((ext_vector_type(4))) words;
+    T one[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) one[e] = v[e];
+    words w;
+    __builtin_memcpy(&w, one, 16);
+    u16x2 top = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+    const uint16_t m = top[0] > top[1] ? top[0] : top[1];
+    return __float_as_uint(static_cast<float>(__builtin_bit_cast(T, m)));
+}
+
 // One eight of the matrix (number t, the v-th of its row) to codes, and its group's scale.
 template <typename T, typename ST>
 __device__ __forceinline__ void pack8(const PackArgs& a, uint32_t t, uint32_t v, const typename Eight<T>::type& raw) {
     const bool live = t < a.vectors;
-    float w[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = static_cast<float>(raw[e]);
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(w[e]) & 0x7fffffffu);
+    uint32_t top = largest_bits<T>(raw);
     // the largest of the group's 4, 8 or 16 lanes, in all of them
     auto turned = [](uint32_t v, auto n) {
         return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(v), static_cast<int>(v), decltype(n)::value, 0xf, 0xf, false));
@@ -55,24 +77,36 @@ __device__ __forceinline__ void pack8(const PackArgs& a, uint32_t t, uint32_t v,
     if (a.lanes > 4) top = max(top, turned(top, std::integral_constant<int, 0x141>{}));     // row_half_mirror: the other four of eight
     if (a.lanes > 8) top = max(top, turned(top, std::integral_constant<int, 0x140>{}));     // row_mirror: the other eight
     if (!live) return;
-    const bool bad = top >= 0x7f800000u;
-    const ST stored = bad ? static_cast<ST>(__builtin_nanf("")) : static_cast<ST>(__uint_as_float(top) / 7.0f);
-    float s = static_cast<float>(stored);
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = static_cast<float>(raw[e]);
+    const float largest = __uint_as_float(top);
+    ST stored;
     uint32_t codes = 0;
-    if (s > 0.0f && s < __builtin_inff()) {
-        if (s < 0x1p-90f) {      // keeps the reciprocal and a residual inside fp32's range
-            s *= 0x1p64f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] *= 0x1p64f;
-        }
+    if (largest > 0x1p-80f && largest < 0x1p126f) {
+        // largest / 7, correctly rounded: the product with 1/7, put right by what it leaves (Markstein's division)
+        const float q = largest * (1.0f / 7.0f);
+        stored = static_cast<ST>(__builtin_fmaf(__builtin_fmaf(-7.0f, q, largest), 1.0f / 7.0f, q));
+        const float s = static_cast<float>(stored);
         float f[8];
-        round8(w, s, 1.0f / s, f);
-        uint32_t c[8];
+        round8<8>(w, s, __builtin_amdgcn_rcpf(s), f);      // the scale's own rounding puts a quotient up to 7.03: nearest 7
+        const uint32_t even = low_bytes(__float_as_uint(f[0]), __float_as_uint(f[2]), __float_as_uint(f[4]), __float_as_uint(f[6])) & 0x0f0f0f0fu;
+        const uint32_t odd = low_bytes(__float_as_uint(f[1]), __float_as_uint(f[3]), __float_as_uint(f[5]), __float_as_uint(f[7]));
+        codes = even | (odd << 4 & 0xf0f0f0f0u);
+    } else {
+        // zeros, what is not finite, and magnitudes so small or large that a step above would leave fp32's normal numbers
+        stored = top >= 0x7f800000u ? static_cast<ST>(__builtin_nanf("")) : static_cast<ST>(largest / 7.0f);
+        float s = static_cast<float>(stored);
+        if (s > 0.0f && s < __builtin_inff()) {
+            const float by = s < 1.0f ? 0x1p64f : 0x1p-64f;
+            s *= by;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)      // the scale's own rounding can put a quotient above 7, far from 8 unless it is a subnormal number
-            c[e] = __float_as_uint(__builtin_amdgcn_fmed3f(f[e], kRoundToInt - 7.0f, kRoundToInt + 7.0f));
-        const uint32_t even = low_bytes(c[0], c[2], c[4], c[6]) & 0x0f0f0f0fu, odd = low_bytes(c[1], c[3], c[5], c[7]) & 0x0f0f0f0fu;
-        codes = even | odd << 4;
+            for (int e = 0; e < 8; ++e) {
+                // a subnormal scale is rounded coarsely: quotients beyond 7 are taken to 7
+                const float k = __builtin_amdgcn_fmed3f(nearest_int(w[e] * by, s, 1.0f / s), -7.0f, 7.0f);
+                codes |= (static_cast<uint32_t>(static_cast<int>(k)) & 15u) << (4 * e);
+            }
+        }
     }
     reinterpret_cast<U32U*>(a.packed)[t].v = codes;
     if ((v & (a.lanes - 1)) == 0) static_cast<ST*>(a.scales)[t >> a.lane_shift] = stored;

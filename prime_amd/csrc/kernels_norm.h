@@ -83,11 +83,13 @@ __device__ __forceinline__ float nearest_int(float z, float unit, float r) {
 
 // 1.5 * 2^23: adding it rounds to a whole number, ties to even, which the sum's low byte then holds in two's complement.
 constexpr float kRoundToInt = 12582912.0f;
-constexpr float kNearBorder = 0.5f - 0x1p-14f;
 
-// Eight whole numbers z / unit to the nearest, as what they are plus kRoundToInt.  Elements near a border are rare (one in ten
-// thousand), so all eight share one test, and only then each is looked at on its own.
+// Eight whole numbers z / unit to the nearest, as what they are plus kRoundToInt, for |z / unit| < TOP.  Elements near a border
+// are rare, so all eight share one test, and only then each is looked at on its own.  z r is off by at most 2^-22 of it with r
+// within one step of 1 / unit, and what is left of it after rounding by another 2^-25.
+template <int TOP>
 __device__ __forceinline__ void round8(const float (&z)[8], float unit, float r, float (&f)[8]) {
+    constexpr float kNearBorder = 0.5f - TOP * 0x1p-21f;
     float d[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -143,7 +145,7 @@ __device__ __forceinline__ void codes8(const float (&z)[8], float s, float r, bo
         p = __builtin_amdgcn_cvt_pk_fp8_f32(f[4], f[5], 0, false);
         hi = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(f[6], f[7], p, true));
     } else {
-        round8(z, s, r, f);
+        round8<128>(z, s, r, f);
         if (!plain) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = __builtin_amdgcn_fmed3f(f[e], kRoundToInt - 127.0f, kRoundToInt + 127.0f);
