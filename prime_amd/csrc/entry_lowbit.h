@@ -30,18 +30,30 @@ void with_weight_type(int weight_type, int type, F&& f) {
 }
 
 constexpr int64_t kMaxDim = int64_t(1) << 30;
+
 constexpr int64_t kRowsPerLaunch = int64_t(1) << 21;    // a dispatch counts its work-items in 32 bits: 1024 a row at most
 
-template <typename XT, typename WT>
+// Rows are read with the hint that leaves them out of the caches when a call moves more than the last-level cache holds anyway
+// (256 MiB): norm of 16384 x 4096 bf16 with residual (470 MB) 74 us with it and 82 without, its gradient (537 MB) 89 and 98; a quarter of those
+// rows (117 and 134 MB) 23.6 and 20.3, 31.1 and 29.4.  Packing gains from half of that up: 16384 x 4096 bf16 (134 MB) 30.5 and 33.8 us,
+// 4096 x 4096 fp32 (67 MB) 16.1 and 13.7.
+constexpr double kOnceNormBytes = 300e6, kOncePackBytes = 128e6;
+template <typename F>
+void with_once(bool once, F&& f) {
+    if (once) f(std::true_type{});
+    else f(std::false_type{});
+}
+
+template <typename XT, typename WT, bool ONCE>
 void launch_rms_norm(const NormArgs& a, double bytes, hipStream_t st) {
     const int64_t r = a.rows;
     const int quads = static_cast<int>((r + 3) / 4), all = static_cast<int>(r);
-    if (a.dim <= 512) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 64, 1>, quads, 256, st, a);
-    else if (a.dim <= 1024) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 64, 2>, quads, 256, st, a);
-    else if (a.dim <= 2048) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 256, 1>, all, 256, st, a);
-    else if (a.dim <= 4096) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 256, 2>, all, 256, st, a);
-    else if (a.dim <= 8192) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 512, 2>, all, 512, st, a);
-    else if (a.dim <= 16384) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 1024, 2>, all, 1024, st, a);
+    if (a.dim <= 512) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 64, 1, ONCE>, quads, 256, st, a);
+    else if (a.dim <= 1024) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 64, 2, ONCE>, quads, 256, st, a);
+    else if (a.dim <= 2048) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 256, 1, ONCE>, all, 256, st, a);
+    else if (a.dim <= 4096) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 256, 2, ONCE>, all, 256, st, a);
+    else if (a.dim <= 8192) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 512, 2, ONCE>, all, 512, st, a);
+    else if (a.dim <= 16384) launch(kIdRmsNorm, bytes, rms_norm_row_kernel<XT, WT, 1024, 2, ONCE>, all, 1024, st, a);
     else launch(kIdRmsNorm, bytes, rms_norm_loop_kernel<XT, WT>, all, 1024, st, a);
 }
 
@@ -59,15 +71,15 @@ int64_t grad_scratch_bytes(int64_t rows, int64_t dim) {
     return grad_groups(rows, dim) * dim * 4 + (dim > kGradRegisterDim ? rows * 4 : 0);
 }
 
-template <typename XT, typename WT>
+template <typename XT, typename WT, bool ONCE>
 void launch_rms_norm_grad(const NormGradArgs& a, int groups, WT* grad_weight, double bytes, hipStream_t st) {
     if (a.rows > 0) {
-        if (a.dim <= 512) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 64, 1>, groups, 64, st, a);
-        else if (a.dim <= 1024) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 64, 2>, groups, 64, st, a);
-        else if (a.dim <= 2048) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 128, 2>, groups, 128, st, a);
-        else if (a.dim <= 4096) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 256, 2>, groups, 256, st, a);
-        else if (a.dim <= 8192) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 512, 2>, groups, 512, st, a);
-        else if (a.dim <= kGradRegisterDim) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 1024, 2>, groups, 1024, st, a);
+        if (a.dim <= 512) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 64, 1, ONCE>, groups, 64, st, a);
+        else if (a.dim <= 1024) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 64, 2, ONCE>, groups, 64, st, a);
+        else if (a.dim <= 2048) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 128, 2, ONCE>, groups, 128, st, a);
+        else if (a.dim <= 4096) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 256, 2, ONCE>, groups, 256, st, a);
+        else if (a.dim <= 8192) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 512, 2, ONCE>, groups, 512, st, a);
+        else if (a.dim <= kGradRegisterDim) launch(kIdRmsNormGrad, bytes, rms_norm_grad_kernel<XT, WT, 1024, 2, ONCE>, groups, 1024, st, a);
         else {
             float* dots = a.partials + static_cast<int64_t>(groups) * a.dim;
             for (int64_t at = 0; at < a.rows; at += kRowsPerLaunch) {
@@ -201,7 +213,11 @@ int prime_rms_norm_quantize(const void* x, int64_t x_stride, const void* residua
             NormArgs a{static_cast<const XT*>(x) + at * x_stride, residual ? static_cast<const XT*>(residual) + at * residual_stride : nullptr, weight,
                        hidden ? static_cast<XT*>(hidden) + at * dim : nullptr, static_cast<uint8_t*>(codes) + at * dim, scales + at, inv_rms + at,
                        x_stride, residual_stride, part, static_cast<int>(dim), code_type == PRIME_F8E4M3, eps};
-            with_weight_type<XT>(weight_type, type, [&](auto w) { launch_rms_norm<XT, decltype(w)>(a, row_bytes * part, static_cast<hipStream_t>(stream)); });
+            with_weight_type<XT>(weight_type, type, [&](auto w) {
+                with_once(row_bytes * rows >= kOnceNormBytes, [&](auto once) {
+                    launch_rms_norm<XT, decltype(w), decltype(once)::value>(a, row_bytes * part, static_cast<hipStream_t>(stream));
+                });
+            });
         });
         if (int rc = launch_check("rms_norm_row_kernel")) return rc;
     }
@@ -231,7 +247,10 @@ int prime_rms_norm_quantize_backward(const void* grad, int64_t grad_stride, cons
         NormGradArgs a{grad, hidden, weight, inv_rms, grad_hidden, grad_x, static_cast<float*>(scratch), grad_stride, hidden_stride, grad_hidden_stride,
                        rows, static_cast<int>(dim)};
         with_weight_type<XT>(weight_type, type, [&](auto w) {
-            launch_rms_norm_grad<XT>(a, static_cast<int>(grad_groups(rows, dim)), static_cast<decltype(w)*>(grad_weight), bytes, static_cast<hipStream_t>(stream));
+            with_once(bytes >= kOnceNormBytes, [&](auto once) {
+                launch_rms_norm_grad<XT, decltype(w), decltype(once)::value>(a, static_cast<int>(grad_groups(rows, dim)), static_cast<decltype(w)*>(grad_weight),
+                                                                             bytes, static_cast<hipStream_t>(stream));
+            });
         });
     });
     return launch_check("rms_norm_grad_kernel");
@@ -244,18 +263,24 @@ int prime_quantize_4bit(const void* weight, int64_t stride, int64_t n, int64_t k
     if (bad_group(group)) return fail(PRIME_EINVAL, "prime_quantize_4bit: group must be 32, 64 or 128");
     if (n == 0) return 0;
     if (!weight || !packed || !scales) return fail(PRIME_EINVAL, "prime_quantize_4bit: null operand");
-    const int64_t groups = (k + group - 1) / group, eights = groups * group / 8;
-    const int64_t step = std::max<int64_t>(1, ((int64_t(1) << 30) - 1) / eights);      // rows a launch: indexes in 31 bits
+    const int64_t groups = (k + group - 1) / group, row_codes = groups * group;
+    const int64_t step = std::max<int64_t>(1, ((int64_t(1) << 30) - 1) / (row_codes / 4));      // rows a launch: indexes in 31 bits
     for (int64_t at = 0; at < n; at += step) {
-        const int64_t rows = std::min(n - at, step), vectors = rows * eights;
+        const int64_t rows = std::min(n - at, step);
         with_float_type(type, [&](auto t) {
             using T = decltype(t);
+            constexpr int E = kUnit<T>;
             with_scale_type(scale_type, [&](auto s) {
                 using ST = decltype(s);
-                PackArgs a{static_cast<const T*>(weight) + at * stride, stride, packed + at * eights * 4, static_cast<ST*>(scales) + at * groups,
-                           static_cast<uint32_t>(vectors), static_cast<int>(k), group / 8, group_shift(group) - 3, FastDiv(static_cast<uint32_t>(eights))};
-                launch(kIdGroupPack, static_cast<double>(rows) * (k * sizeof(T) + eights * 4 + groups * sizeof(ST)), group4_pack_kernel<T, ST>,
-                       static_cast<int>((vectors + 256 * kPackEach - 1) / (256 * kPackEach)), 256, static_cast<hipStream_t>(stream), a);
+                const int64_t units = rows * (row_codes / E);
+                PackArgs a{static_cast<const T*>(weight) + at * stride, stride, packed + at * row_codes / 2, static_cast<ST*>(scales) + at * groups,
+                           static_cast<uint32_t>(units), static_cast<int>(k), group / E, group_shift(group) - (E == 8 ? 3 : 2),
+                           FastDiv(static_cast<uint32_t>(row_codes / E))};
+                with_once(static_cast<double>(n) * k * sizeof(T) >= kOncePackBytes, [&](auto once) {
+                    launch(kIdGroupPack, static_cast<double>(rows) * (k * sizeof(T) + row_codes / 2 + groups * sizeof(ST)),
+                           group4_pack_kernel<T, ST, decltype(once)::value>, static_cast<int>((units + 256 * kPackEach - 1) / (256 * kPackEach)), 256,
+                           static_cast<hipStream_t>(stream), a);
+                });
             });
         });
         if (int rc = launch_check("group4_pack_kernel")) return rc;
@@ -270,17 +295,20 @@ int prime_dequantize_4bit(const uint8_t* packed, int64_t packed_stride, const vo
     if (bad_group(group)) return fail(PRIME_EINVAL, "prime_dequantize_4bit: group must be 32, 64 or 128");
     if (n == 0) return 0;
     if (!packed || !scales || !out) return fail(PRIME_EINVAL, "prime_dequantize_4bit: null operand");
-    const int64_t eights = (k + 7) / 8, step = std::max<int64_t>(1, ((int64_t(1) << 30) - 1) / eights);
+    const int64_t step = std::max<int64_t>(1, ((int64_t(1) << 30) - 1) / ((k + 3) / 4));
     for (int64_t at = 0; at < n; at += step) {
-        const int64_t rows = std::min(n - at, step), vectors = rows * eights;
+        const int64_t rows = std::min(n - at, step);
         with_float_type(out_type, [&](auto t) {
             using T = decltype(t);
+            constexpr int E = kUnit<T>;
             with_scale_type(scale_type, [&](auto s) {
                 using ST = decltype(s);
+                const int64_t row_units = (k + E - 1) / E, units = rows * row_units;
                 UnpackArgs a{packed + at * packed_stride, static_cast<const ST*>(scales) + at * scale_stride, static_cast<T*>(out) + at * k, packed_stride,
-                             scale_stride, static_cast<uint32_t>(vectors), static_cast<int>(k), group_shift(group) - 3, FastDiv(static_cast<uint32_t>(eights))};
+                             scale_stride, static_cast<uint32_t>(units), static_cast<int>(k), group_shift(group) - (E == 8 ? 3 : 2),
+                             FastDiv(static_cast<uint32_t>(row_units))};
                 launch(kIdGroupUnpack, static_cast<double>(rows) * (k * (sizeof(T) + 0.5)), group4_unpack_kernel<T, ST>,
-                       static_cast<int>((vectors + 256 * kUnpackEach - 1) / (256 * kUnpackEach)), 256, static_cast<hipStream_t>(stream), a);
+                       static_cast<int>((units + 256 * kUnpackEach - 1) / (256 * kUnpackEach)), 256, static_cast<hipStream_t>(stream), a);
             });
         });
         if (int rc = launch_check("group4_unpack_kernel")) return rc;

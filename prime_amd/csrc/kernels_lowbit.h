@@ -19,67 +19,88 @@ struct FastDiv {
     __device__ __forceinline__ uint32_t quotient(uint32_t t) const { return (__umulhi(t, mul) + t) >> shift; }
 };
 
+struct __attribute__((packed)) U16U { uint16_t v; };
+
 __device__ __forceinline__ float load_scale(const float* p) { return *p; }
 __device__ __forceinline__ float load_scale(const __bf16* p) { return static_cast<float>(*p); }
+
+// Elements of a lane: 16 bytes of the matrix, so that a wavefront's access covers 1 KiB without gaps (fp32 elements eight a lane, in
+// two accesses that each touch every second 16 bytes: 22528 x 8192 packed in 164 us and widened in 189).
+template <typename T> constexpr int kUnit = 16 / static_cast<int>(sizeof(T));
+template <typename T> struct Unit;
+template <> struct Unit<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Unit<__bf16> { typedef Eight<__bf16>::type type; };
+template <> struct Unit<_Float16> { typedef Eight<_Float16>::type type; };
+
+template <typename T, bool ONCE>
+__device__ __forceinline__ typename Unit<T>::type take_unit(const T* __restrict__ row, int i, int n) {
+    typename Unit<T>::type t;
+    if (i + kUnit<T> <= n) {
+        const typename Unit<T>::type* p = reinterpret_cast<const typename Unit<T>::type*>(row + i);
+        if constexpr (ONCE) t = __builtin_nontemporal_load(p);
+        else t = *p;
+    } else {
+#pragma unroll
+        for (int e = 0; e < kUnit<T>; ++e) t[e] = i + e < n ? row[i + e] : static_cast<T>(0.0f);
+    }
+    return t;
+}
 
 struct PackArgs {
     const void* weight;
     int64_t stride;             // elements from row to row of the weight
     uint8_t* packed;            // dense rows of groups * group / 2 bytes
     void* scales;               // dense rows of `groups`
-    uint32_t vectors;           // eights of this launch: rows * groups * group / 8
+    uint32_t units;             // of this launch: rows * groups * group / kUnit
     int k;
-    int lanes;                  // eights of a group: 4, 8 or 16
+    int lanes;                  // units of a group: 4, 8, 16 or 32
     int lane_shift;
-    FastDiv per_row;            // eights of a row
+    FastDiv per_row;            // units of a row
 };
 
-constexpr int kPackEach = 2;
-
-// The largest magnitude of eight elements, as the bits of a float; a NaN compares above all numbers.
+// The largest magnitude of a unit, as the bits of a float; a NaN compares above all numbers.  16-bit elements two at a time, as whole numbers.
 template <typename T>
-__device__ __forceinline__ uint32_t largest_bits(const typename Eight<T>::type& v);
-template <>
-__device__ __forceinline__ uint32_t largest_bits<float>(const Eight<float>::type& v) {
-    uint32_t top = 0;
+__device__ __forceinline__ uint32_t largest_bits(const typename Unit<T>::type& v) {
+    if constexpr (sizeof(T) == 4) {
+        return max(max(__float_as_uint(v[0]) & 0x7fffffffu, __float_as_uint(v[1]) & 0x7fffffffu),
+                   max(__float_as_uint(v[2]) & 0x7fffffffu, __float_as_uint(v[3]) & 0x7fffffffu));
+    } else {
+        typedef uint16_t __attribute__((ext_vector_type(2))) u16x2;
+        typedef uint32_t __attribute__((ext_vector_type(4))) words;
+        T one[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
-    return top;
-}
-// 16-bit types: two at a time, as whole numbers.
-template <typename T>
-__device__ __forceinline__ uint32_t largest_bits(const typename Eight<T>::type& v) {
-    typedef uint16_t __attribute__((ext_vector_type(2))) u16x2;
-    typedef uint32_t __attribute__((ext_vector_type(4))) words;
-    T one[8];
+        for (int e = 0; e < 8; ++e) one[e] = v[e];
+        words w;
+        __builtin_memcpy(&w, one, 16);
+        u16x2 top = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) one[e] = v[e];
-    words w;
-    __builtin_memcpy(&w, one, 16);
-    u16x2 top = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
-#pragma unroll
-    for (int i = 1; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
-    const uint16_t m = top[0] > top[1] ? top[0] : top[1];
-    return __float_as_uint(static_cast<float>(__builtin_bit_cast(T, m)));
+        for (int i = 1; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+        const uint16_t m = top[0] > top[1] ? top[0] : top[1];
+        return __float_as_uint(static_cast<float>(__builtin_bit_cast(T, m)));
+    }
 }
 
-// One eight of the matrix (number t, the v-th of its row) to codes, and its group's scale.
+// One unit of the matrix (number t, the v-th of its row) to codes, and its group's scale.
 template <typename T, typename ST>
-__device__ __forceinline__ void pack8(const PackArgs& a, uint32_t t, uint32_t v, const typename Eight<T>::type& raw) {
-    const bool live = t < a.vectors;
+__device__ __forceinline__ void pack_unit(const PackArgs& a, uint32_t t, uint32_t v, const typename Unit<T>::type& raw) {
+    constexpr int E = kUnit<T>;
     uint32_t top = largest_bits<T>(raw);
-    // the largest of the group's 4, 8 or 16 lanes, in all of them
-    auto turned = [](uint32_t v, auto n) {
-        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(v), static_cast<int>(v), decltype(n)::value, 0xf, 0xf, false));
+    // the largest of the group's lanes, in all of them
+    auto turned = [](uint32_t x, auto n) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(x), static_cast<int>(x), decltype(n)::value, 0xf, 0xf, false));
     };
     top = max(top, turned(top, std::integral_constant<int, 0xb1>{}));                       // quad_perm 1 0 3 2
     top = max(top, turned(top, std::integral_constant<int, 0x4e>{}));                       // quad_perm 2 3 0 1
     if (a.lanes > 4) top = max(top, turned(top, std::integral_constant<int, 0x141>{}));     // row_half_mirror: the other four of eight
     if (a.lanes > 8) top = max(top, turned(top, std::integral_constant<int, 0x140>{}));     // row_mirror: the other eight
-    if (!live) return;
+    if (E == 4 && a.lanes > 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(top, top, false, false);            // the neighbouring row of 16
+        top = max(static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1]));
+    }
+    if (t >= a.units) return;
     float w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = static_cast<float>(raw[e]);
+    for (int e = 0; e < 8; ++e) w[e] = e < E ? static_cast<float>(raw[e % E]) : 0.0f;
     const float largest = __uint_as_float(top);
     ST stored;
     uint32_t codes = 0;
@@ -101,31 +122,34 @@ __device__ __forceinline__ void pack8(const PackArgs& a, uint32_t t, uint32_t v,
             const float by = s < 1.0f ? 0x1p64f : 0x1p-64f;
             s *= by;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < E; ++e) {
                 // a subnormal scale is rounded coarsely: quotients beyond 7 are taken to 7
                 const float k = __builtin_amdgcn_fmed3f(nearest_int(w[e] * by, s, 1.0f / s), -7.0f, 7.0f);
                 codes |= (static_cast<uint32_t>(static_cast<int>(k)) & 15u) << (4 * e);
             }
         }
     }
-    reinterpret_cast<U32U*>(a.packed)[t].v = codes;
+    if constexpr (E == 8) reinterpret_cast<U32U*>(a.packed)[t].v = codes;
+    else reinterpret_cast<U16U*>(a.packed)[t].v = static_cast<uint16_t>(codes);
     if ((v & (a.lanes - 1)) == 0) static_cast<ST*>(a.scales)[t >> a.lane_shift] = stored;
 }
 
-// A lane takes eight elements at a time, a group's lanes sit side by side in a wavefront; two loads are on their way at a time.
-template <typename T, typename ST>
+constexpr int kPackEach = 2;         // units of a lane, all on their way together
+
+// A group's lanes sit side by side in a wavefront.
+template <typename T, typename ST, bool ONCE>
 __global__ __launch_bounds__(256) void group4_pack_kernel(PackArgs a) {
-    typename Eight<T>::type raw[kPackEach];
+    typename Unit<T>::type raw[kPackEach];
     uint32_t col[kPackEach];
 #pragma unroll
     for (int i = 0; i < kPackEach; ++i) {
-        const uint32_t t = (blockIdx.x * kPackEach + i) * 256u + threadIdx.x, in = t < a.vectors ? t : 0u;
+        const uint32_t t = (blockIdx.x * kPackEach + i) * 256u + threadIdx.x, in = t < a.units ? t : 0u;
         const uint32_t row = a.per_row.quotient(in);
         col[i] = in - row * a.per_row.d;
-        raw[i] = take8(static_cast<const T*>(a.weight) + row * a.stride, static_cast<int>(col[i] * 8), a.k);
+        raw[i] = take_unit<T, ONCE>(static_cast<const T*>(a.weight) + row * a.stride, static_cast<int>(col[i] * kUnit<T>), a.k);
     }
 #pragma unroll
-    for (int i = 0; i < kPackEach; ++i) pack8<T, ST>(a, (blockIdx.x * kPackEach + i) * 256u + threadIdx.x, col[i], raw[i]);
+    for (int i = 0; i < kPackEach; ++i) pack_unit<T, ST>(a, (blockIdx.x * kPackEach + i) * 256u + threadIdx.x, col[i], raw[i]);
 }
 
 struct UnpackArgs {
@@ -134,36 +158,51 @@ struct UnpackArgs {
     void* out;                  // dense rows of k
     int64_t p_stride;           // bytes from row to row of the codes
     int64_t s_stride;           // elements from row to row of the scales
-    uint32_t vectors;
+    uint32_t units;
     int k;
-    int lane_shift;             // log2 of a group's eights
-    FastDiv per_row;            // eights of a row of the output
+    int lane_shift;             // log2 of a group's units
+    FastDiv per_row;            // units of a row of the output
 };
 
-constexpr int kUnpackEach = 2;       // eights of a lane, all on their way together
+constexpr int kUnpackEach = 2;       // units of a lane, all on their way together
 
 // Code e of a word of eight, as an integer.
 __device__ __forceinline__ int code4(uint32_t word, int e) { return static_cast<int>(word << (28 - 4 * e)) >> 28; }
 
 template <typename T, typename ST>
 __global__ __launch_bounds__(256) void group4_unpack_kernel(UnpackArgs a) {
+    constexpr int E = kUnit<T>;
     uint32_t row[kUnpackEach], v[kUnpackEach], word[kUnpackEach];
     float s[kUnpackEach];
 #pragma unroll
     for (int i = 0; i < kUnpackEach; ++i) {
-        const uint32_t t = min((blockIdx.x * kUnpackEach + i) * 256u + threadIdx.x, a.vectors - 1);
+        const uint32_t t = min((blockIdx.x * kUnpackEach + i) * 256u + threadIdx.x, a.units - 1);
         row[i] = a.per_row.quotient(t);
         v[i] = t - row[i] * a.per_row.d;
-        word[i] = reinterpret_cast<const U32U*>(a.packed + row[i] * a.p_stride)[v[i]].v;
+        const uint8_t* p = a.packed + row[i] * a.p_stride;
+        if constexpr (E == 8) word[i] = reinterpret_cast<const U32U*>(p)[v[i]].v;
+        else word[i] = reinterpret_cast<const U16U*>(p)[v[i]].v;
         s[i] = load_scale(static_cast<const ST*>(a.scales) + row[i] * a.s_stride + (v[i] >> a.lane_shift));
     }
 #pragma unroll
     for (int i = 0; i < kUnpackEach; ++i) {
-        if ((blockIdx.x * kUnpackEach + i) * 256u + threadIdx.x >= a.vectors) return;
-        float o[8];
+        if ((blockIdx.x * kUnpackEach + i) * 256u + threadIdx.x >= a.units) return;
+        T* out = static_cast<T*>(a.out) + static_cast<int64_t>(row[i]) * a.k;
+        const int at = static_cast<int>(v[i] * E);
+        typename Unit<T>::type o;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(code4(word[i], e)) * s[i];
-        store8(static_cast<T*>(a.out) + static_cast<int64_t>(row[i]) * a.k, static_cast<int>(v[i] * 8), a.k, o);
+        for (int e = 0; e < E; ++e) {
+            float p = static_cast<float>(code4(word[i], e)) * s[i];
+            if constexpr (std::is_same<T, _Float16>::value) asm("" : "+v"(p));      // keeps the product's own rounding: else it is fused with the conversion
+            o[e] = static_cast<T>(p);
+        }
+        if (at + E <= a.k) {
+            *reinterpret_cast<typename Unit<T>::type*>(out + at) = o;
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (at + e < a.k) out[at + e] = o[e];
+        }
     }
 }
 

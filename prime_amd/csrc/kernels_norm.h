@@ -20,12 +20,15 @@ template <> struct Eight<__bf16> { typedef __bf16 type __attribute__((ext_vector
 template <> struct Eight<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(8), aligned(2))); };
 struct __attribute__((packed, aligned(1))) U64U { uint32_t lo, hi; };
 
-// Elements i .. i + 7 of a row of n as they are, zero behind its end.
-template <typename T>
+// Elements i .. i + 7 of a row of n as they are, zero behind its end.  ONCE: nobody reads them again soon (a hinted load
+// leaves room in the caches for what is).
+template <typename T, bool ONCE = false>
 __device__ __forceinline__ typename Eight<T>::type take8(const T* __restrict__ row, int i, int n) {
     typename Eight<T>::type t;
     if (i + 8 <= n) {
-        t = *reinterpret_cast<const typename Eight<T>::type*>(row + i);
+        const typename Eight<T>::type* p = reinterpret_cast<const typename Eight<T>::type*>(row + i);
+        if constexpr (ONCE) t = __builtin_nontemporal_load(p);
+        else t = *p;
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) t[e] = i + e < n ? row[i + e] : static_cast<T>(0.0f);
@@ -41,6 +44,90 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int i, int n, f
     for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(t[e]);
 }
 
+// The `lane`-th eight elements of a row, dealt to lanes as the memory likes it: 16-bit elements eight side by side; fp32 elements
+// four side by side, twice (a wavefront's two loads then cover whole lines of 1 KiB each, where eight side by side
+// would have each load touch every second 16 bytes of 2 KiB).
+template <typename T>
+__device__ __forceinline__ void place8(int lane, int (&at)[2]) {
+    if constexpr (sizeof(T) == 4) {
+        at[0] = (lane >> 6) * 512 + (lane & 63) * 4;
+        at[1] = at[0] + 256;
+    } else {
+        at[0] = lane * 8;
+        at[1] = at[0] + 4;
+    }
+}
+typedef float __attribute__((ext_vector_type(4), aligned(4))) four_floats;
+struct __attribute__((packed, aligned(1))) U32Any { uint32_t v; };
+
+template <bool ONCE, typename T>
+__device__ __forceinline__ typename Eight<T>::type row_take8(const T* __restrict__ row, int lane, int n) {
+    if constexpr (sizeof(T) == 4) {
+        typename Eight<T>::type t;
+        int at[2];
+        place8<T>(lane, at);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (at[h] + 4 <= n) {
+                const four_floats* p = reinterpret_cast<const four_floats*>(row + at[h]);
+                four_floats v;
+                if constexpr (ONCE) v = __builtin_nontemporal_load(p);
+                else v = *p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[4 * h + e] = v[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[4 * h + e] = at[h] + e < n ? row[at[h] + e] : 0.0f;
+            }
+        }
+        return t;
+    } else {
+        return take8<T, ONCE>(row, lane * 8, n);
+    }
+}
+// A norm's weight for the elements that row_take8<XT> gives: read again by every row.
+template <typename XT, typename WT>
+__device__ __forceinline__ void weight8(const WT* __restrict__ weight, int lane, int n, float (&w)[8]) {
+    if constexpr (sizeof(XT) == 4 || sizeof(WT) == 2) {
+        const typename Eight<WT>::type t = row_take8<false>(weight, lane, n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = static_cast<float>(t[e]);
+    } else {
+        load8(weight, lane * 8, n, w);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void row_store8(T* __restrict__ row, int lane, int n, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        int at[2];
+        place8<T>(lane, at);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (at[h] + 4 <= n) {
+                *reinterpret_cast<four_floats*>(row + at[h]) = four_floats{v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (at[h] + e < n) row[at[h] + e] = v[4 * h + e];
+            }
+        }
+    } else {
+        const int i = lane * 8;
+        if (i + 8 <= n) {
+            typename Eight<T>::type t;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] = static_cast<T>(v[e]);
+            *reinterpret_cast<typename Eight<T>::type*>(row + i) = t;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (i + e < n) row[i + e] = static_cast<T>(v[e]);
+        }
+    }
+}
+
+// Eight consecutive elements.
 template <typename T>
 __device__ __forceinline__ void store8(T* __restrict__ row, int i, int n, const float (&v)[8]) {
     if (i + 8 <= n) {
@@ -55,14 +142,25 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int i, int n, const 
     }
 }
 
-// Eight one-byte codes, lowest byte first.
-__device__ __forceinline__ void store8_codes(uint8_t* __restrict__ row, int i, int n, uint32_t lo, uint32_t hi) {
-    if (i + 8 <= n) {
-        *reinterpret_cast<U64U*>(row + i) = U64U{lo, hi};
-    } else {
+// The one-byte codes of the elements that row_take8<T> gives, lowest byte first.
+template <typename T>
+__device__ __forceinline__ void row_store_codes(uint8_t* __restrict__ row, int lane, int n, uint32_t lo, uint32_t hi) {
+    int at[2];
+    place8<T>(lane, at);
+    if (sizeof(T) == 2 && at[1] + 4 <= n) {
+        *reinterpret_cast<U64U*>(row + at[0]) = U64U{lo, hi};
+        return;
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (i + e < n) row[i + e] = static_cast<uint8_t>((e < 4 ? lo : hi) >> (8 * (e & 3)));
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t w = h ? hi : lo;
+        if (at[h] + 4 <= n) {
+            reinterpret_cast<U32Any*>(row + at[h])->v = w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (at[h] + e < n) row[at[h] + e] = static_cast<uint8_t>(w >> (8 * e));
+        }
     }
 }
 
@@ -244,7 +342,7 @@ __device__ __forceinline__ void store_row_statistics(const NormArgs& a, int64_t 
 
 // One row per TPR lanes (64: four rows a workgroup; else a workgroup), held in registers between the statistics and
 // the codes: every byte is read once and written once.  V vectors of eight per lane.
-template <typename XT, typename WT, int TPR, int V>
+template <typename XT, typename WT, int TPR, int V, bool ONCE>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_row_kernel(NormArgs a) {
     constexpr int kRows = TPR < 256 ? 256 / TPR : 1;
     const int lane = threadIdx.x % TPR;
@@ -258,23 +356,27 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_row_kernel(Nor
     if (live) {
         float w[V][8];
 #pragma unroll
-        for (int j = 0; j < V; ++j) load8(xr, (lane + j * TPR) * 8, a.dim, z[j]);
+        for (int j = 0; j < V; ++j) {
+            const typename Eight<XT>::type t = row_take8<ONCE>(xr, lane + j * TPR, a.dim);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[j][e] = static_cast<float>(t[e]);
+        }
         if (a.residual) {
             const XT* rr = static_cast<const XT*>(a.residual) + row * a.r_stride;
             XT* hr = static_cast<XT*>(a.hidden) + row * a.dim;
-            float r[V][8];
+            typename Eight<XT>::type r[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) load8(rr, (lane + j * TPR) * 8, a.dim, r[j]);
+            for (int j = 0; j < V; ++j) r[j] = row_take8<ONCE>(rr, lane + j * TPR, a.dim);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) z[j][e] = static_cast<float>(static_cast<XT>(z[j][e] + r[j][e]));
-                store8(hr, (lane + j * TPR) * 8, a.dim, z[j]);
+                for (int e = 0; e < 8; ++e) z[j][e] = static_cast<float>(static_cast<XT>(z[j][e] + static_cast<float>(r[j][e])));
+                row_store8(hr, lane + j * TPR, a.dim, z[j]);
             }
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            load8(wr, (lane + j * TPR) * 8, a.dim, w[j]);
+            weight8<XT>(wr, lane + j * TPR, a.dim, w[j]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const double h = z[j][e];
@@ -301,8 +403,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_row_kernel(Nor
     uint8_t* cr = a.codes + row * a.dim;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int i = (lane + j * TPR) * 8;
-        if (i >= a.dim) break;
+        if ((lane + j * TPR) / 64 * 512 >= a.dim) break;      // the same for a wavefront
         uint32_t lo = 0, hi = 0;
         if (!q.none) {
             const bool plain = q.up == 1.0f;
@@ -313,7 +414,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_row_kernel(Nor
             if (a.fp8) codes8<true>(z[j], q.s, q.r, plain, lo, hi);
             else codes8<false>(z[j], q.s, q.r, plain, lo, hi);
         }
-        store8_codes(cr, i, a.dim, lo, hi);
+        row_store_codes<XT>(cr, lane + j * TPR, a.dim, lo, hi);
     }
     if (lane == 0) store_row_statistics(a, row, sq, top);
 }
@@ -331,15 +432,19 @@ __global__ __launch_bounds__(1024) void rms_norm_loop_kernel(NormArgs a) {
     const WT* wr = static_cast<const WT*>(a.weight);
     double sq = 0.0;
     uint32_t top = 0;
-    for (int64_t i = static_cast<int64_t>(threadIdx.x) * 8; i < a.dim; i += 8192) {
-        float h[8], r[8], w[8];
-        load8(xr, i, a.dim, h);
-        load8(wr, i, a.dim, w);
-        if (rr) {
-            load8(rr, i, a.dim, r);
+    const int turns = (a.dim + 8191) / 8192;
+    for (int turn = 0; turn < turns; ++turn) {
+        const int l = turn * 1024 + threadIdx.x;
+        float h[8], w[8];
+        const typename Eight<XT>::type x = row_take8<false>(xr, l, a.dim);
+        weight8<XT>(wr, l, a.dim, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = static_cast<float>(static_cast<XT>(h[e] + r[e]));
-            store8(hr, i, a.dim, h);
+        for (int e = 0; e < 8; ++e) h[e] = static_cast<float>(x[e]);
+        if (rr) {
+            const typename Eight<XT>::type r = row_take8<false>(rr, l, a.dim);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = static_cast<float>(static_cast<XT>(h[e] + static_cast<float>(r[e])));
+            row_store8(hr, l, a.dim, h);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -359,18 +464,19 @@ __global__ __launch_bounds__(1024) void rms_norm_loop_kernel(NormArgs a) {
     const RowScale q = row_scale(top, a.fp8);
     uint8_t* cr = a.codes + row * a.dim;
     const XT* back = hr ? hr : xr;
-    for (int64_t i = static_cast<int64_t>(threadIdx.x) * 8; i < a.dim; i += 8192) {
-        float z[8], w[8];
+    for (int turn = 0; turn < turns; ++turn) {
+        const int l = turn * 1024 + threadIdx.x;
         uint32_t lo = 0, hi = 0;
         if (!q.none) {
-            load8(back, i, a.dim, z);
-            load8(wr, i, a.dim, w);
+            float z[8], w[8];
+            const typename Eight<XT>::type h = row_take8<false>(back, l, a.dim);
+            weight8<XT>(wr, l, a.dim, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z[e] = z[e] * w[e] * q.up;
+            for (int e = 0; e < 8; ++e) z[e] = static_cast<float>(h[e]) * w[e] * q.up;
             if (a.fp8) codes8<true>(z, q.s, q.r, q.up == 1.0f, lo, hi);
             else codes8<false>(z, q.s, q.r, q.up == 1.0f, lo, hi);
         }
-        store8_codes(cr, i, a.dim, lo, hi);
+        row_store_codes<XT>(cr, l, a.dim, lo, hi);
     }
     if (threadIdx.x == 0) store_row_statistics(a, row, sq, top);
 }
@@ -394,7 +500,7 @@ struct NormGradArgs {
 
 // A workgroup of TPR lanes takes rows blockIdx.x, + gridDim.x, ...; a lane keeps its columns' share of dw in registers over
 // all of them, so dw costs one store of a row per workgroup.  The next row is on its way while one is worked on.
-template <typename XT, typename WT, int TPR, int V>
+template <typename XT, typename WT, int TPR, int V, bool ONCE>
 __global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
     __shared__ float sh[2][TPR / 64];
     typedef typename Eight<XT>::type eight;
@@ -409,12 +515,12 @@ __global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
         inv0 = a.inv_rms[row];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            g0[j] = take8(grad + row * a.g_stride, (lane + j * TPR) * 8, a.dim);
-            h0[j] = take8(hidden + row * a.h_stride, (lane + j * TPR) * 8, a.dim);
+            g0[j] = row_take8<ONCE>(grad + row * a.g_stride, lane + j * TPR, a.dim);
+            h0[j] = row_take8<ONCE>(hidden + row * a.h_stride, lane + j * TPR, a.dim);
         }
         if (grad_hidden) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) d0[j] = take8(grad_hidden + row * a.gh_stride, (lane + j * TPR) * 8, a.dim);
+            for (int j = 0; j < V; ++j) d0[j] = row_take8<ONCE>(grad_hidden + row * a.gh_stride, lane + j * TPR, a.dim);
         }
     };
 #pragma unroll
@@ -425,7 +531,7 @@ __global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
     float dw[V][8], w[V][8];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        load8(static_cast<const WT*>(a.weight), (lane + j * TPR) * 8, a.dim, w[j]);
+        weight8<XT>(static_cast<const WT*>(a.weight), lane + j * TPR, a.dim, w[j]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) dw[j][e] = 0.0f;
     }
@@ -469,11 +575,15 @@ __global__ __launch_bounds__(TPR) void rms_norm_grad_kernel(NormGradArgs a) {
         for (int j = 0; j < V; ++j) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) g[j][e] = fmaf(inv, fmaf(-h[j][e], c, g[j][e]), static_cast<float>(d[j][e]));
-            store8(static_cast<XT*>(a.grad_x) + row * a.dim, (lane + j * TPR) * 8, a.dim, g[j]);
+            row_store8(static_cast<XT*>(a.grad_x) + row * a.dim, lane + j * TPR, a.dim, g[j]);
         }
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) store8(a.partials + static_cast<int64_t>(blockIdx.x) * a.dim, (lane + j * TPR) * 8, a.dim, dw[j]);
+    for (int j = 0; j < V; ++j) {
+        float* to = a.partials + static_cast<int64_t>(blockIdx.x) * a.dim;
+        if constexpr (sizeof(XT) == 4) row_store8(to, lane + j * TPR, a.dim, dw[j]);
+        else store8(to, (lane + j * TPR) * 8, a.dim, dw[j]);
+    }
 }
 
 // Rows too long for that: the row's c first, ...
