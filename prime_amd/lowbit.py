@@ -68,10 +68,26 @@ def _check_inputs(name: str, dev: torch.device, *tensors: Optional[torch.Tensor]
             _fail(name, "records no gradient; call it inside a torch.autograd.Function or under torch.no_grad()")
 
 
-def _rows(t: torch.Tensor, dim: int) -> torch.Tensor:
-    """``t`` as rows of ``dim`` consecutive elements: a view wherever the strides allow it."""
+def _wants_gradient(*tensors: Optional[torch.Tensor]) -> bool:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
+
+
+def _rows(t: torch.Tensor, dim: int) -> Tuple[torch.Tensor, int]:
+    """(``t``, or a copy where its strides ask for one, elements from row to row): rows of ``dim`` consecutive elements."""
+    if t.is_contiguous():
+        return t, dim
     v = t if t.dim() == 2 else t.reshape(-1, dim)
-    return v if v.stride(1) == 1 or dim == 1 else v.contiguous()
+    if v.stride(1) != 1 and dim > 1:
+        v = v.contiguous()
+    return v, v.stride(0)
+
+
+def _like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """An uninitialised dense tensor of ``t``'s shape (from a dense one in half the time)."""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else torch.empty(t.shape, dtype=dtype, device=t.device)
 
 
 def _check_norm(name: str, x: torch.Tensor, weight: torch.Tensor, like: Tuple[Tuple[str, Optional[torch.Tensor]], ...] = ()) -> int:
@@ -91,27 +107,37 @@ def _check_norm(name: str, x: torch.Tensor, weight: torch.Tensor, like: Tuple[Tu
 
 
 def _norm(name: str, x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float, dtype: torch.dtype):
-    dim = _check_norm(name, x, weight, (("residual", residual),))
-    if dtype not in CODE_DTYPES:
-        _fail(name, f"codes are torch.int8 or torch.float8_e4m3fn, got {dtype}")
-    if not eps >= 0.0:
-        _fail(name, f"eps must not be negative, got {eps}")
-    dev = x.device
-    _check_inputs(name, dev, x, residual, weight)
+    xt, wt, shape, dev = x.dtype, weight.dtype, x.shape, x.device
+    # one expression for the calls that are right; the checks that say what is wrong run only for the others
+    if not (xt in _FLOATS and len(shape) > 0 and weight.shape == shape[-1:] and 0 < shape[-1] <= MAX_DIM and (wt is xt or wt is torch.float32)
+            and dtype in CODE_DTYPES and eps >= 0.0 and weight.device == dev
+            and (residual is None or (residual.shape == shape and residual.dtype is xt and residual.device == dev))
+            and not _wants_gradient(x, weight, residual)):
+        _check_norm(name, x, weight, (("residual", residual),))
+        if dtype not in CODE_DTYPES:
+            _fail(name, f"codes are torch.int8 or torch.float8_e4m3fn, got {dtype}")
+        if not eps >= 0.0:
+            _fail(name, f"eps must not be negative, got {eps}")
+        _check_inputs(name, dev, x, residual, weight)
+    dim = shape[-1]
     lib = _lib.load()
     with _on(dev):
-        lead = x.shape[:-1]
-        x2 = _rows(x, dim)
-        r2 = None if residual is None else _rows(residual, dim)
-        weight = weight.contiguous()
-        codes = torch.empty(x.shape, dtype=dtype, device=dev)
-        scales = torch.empty(lead, dtype=torch.float32, device=dev)
-        inv_rms = torch.empty(lead, dtype=torch.float32, device=dev)
-        hidden = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-        rc = lib.prime_rms_norm_quantize(x2.data_ptr(), x2.stride(0), None if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0),
-                                         weight.data_ptr(), x2.shape[0], dim, _TYPE[x.dtype], _TYPE[weight.dtype], _TYPE[dtype], float(eps),
-                                         codes.data_ptr(), scales.data_ptr(), None if hidden is None else hidden.data_ptr(),
-                                         inv_rms.data_ptr(), _stream(dev))
+        lead = shape[:-1]
+        x2, xs = _rows(x, dim)
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        codes = _like(x, dtype)
+        scales = x.new_empty(lead, dtype=torch.float32)
+        inv_rms = x.new_empty(lead, dtype=torch.float32)
+        hidden = None
+        rp = hp = None
+        rs = 0
+        if residual is not None:
+            r2, rs = _rows(residual, dim)
+            hidden = _like(x, xt)
+            rp, hp = r2.data_ptr(), hidden.data_ptr()
+        rc = lib.prime_rms_norm_quantize(x2.data_ptr(), xs, rp, rs, weight.data_ptr(), x.numel() // dim, dim, _TYPE[xt], _TYPE[wt], _TYPE[dtype], eps,
+                                         codes.data_ptr(), scales.data_ptr(), hp, inv_rms.data_ptr(), _stream(dev))
         if rc:
             _lib.check(rc, "prime_rms_norm_quantize")
     return codes, scales, hidden, inv_rms
@@ -128,26 +154,37 @@ def _add_rms_norm_quantize(x, residual, weight, eps=1e-6, dtype=torch.int8):
 
 def _rms_norm_quantize_backward(grad, hidden, weight, inv_rms, grad_hidden=None):
     name = "rms_norm_quantize_backward"
-    dim = _check_norm(name, hidden, weight, (("grad", grad), ("grad_hidden", grad_hidden)))
-    if inv_rms.dtype != torch.float32 or inv_rms.shape != hidden.shape[:-1]:
-        _fail(name, f"inv_rms must be Float of shape {tuple(hidden.shape[:-1])}, got {inv_rms.dtype} of {tuple(inv_rms.shape)}")
-    dev = hidden.device
-    _check_inputs(name, dev, grad, hidden, weight, inv_rms, grad_hidden)
+    ht, wt, shape, dev = hidden.dtype, weight.dtype, hidden.shape, hidden.device
+    if not (ht in _FLOATS and len(shape) > 0 and weight.shape == shape[-1:] and 0 < shape[-1] <= MAX_DIM and (wt is ht or wt is torch.float32)
+            and grad.shape == shape and grad.dtype is ht and inv_rms.dtype is torch.float32 and inv_rms.shape == shape[:-1]
+            and grad.device == dev and weight.device == dev and inv_rms.device == dev
+            and (grad_hidden is None or (grad_hidden.shape == shape and grad_hidden.dtype is ht and grad_hidden.device == dev))
+            and not _wants_gradient(grad, hidden, weight, inv_rms, grad_hidden)):
+        _check_norm(name, hidden, weight, (("grad", grad), ("grad_hidden", grad_hidden)))
+        if inv_rms.dtype != torch.float32 or inv_rms.shape != shape[:-1]:
+            _fail(name, f"inv_rms must be Float of shape {tuple(shape[:-1])}, got {inv_rms.dtype} of {tuple(inv_rms.shape)}")
+        _check_inputs(name, dev, grad, hidden, weight, inv_rms, grad_hidden)
+    dim = shape[-1]
     lib = _lib.load()
     with _on(dev):
-        g2, h2 = _rows(grad, dim), _rows(hidden, dim)
-        d2 = None if grad_hidden is None else _rows(grad_hidden, dim)
-        weight, inv_rms = weight.contiguous(), inv_rms.contiguous()
-        rows = h2.shape[0]
-        grad_x = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev)
-        grad_weight = torch.empty(dim, dtype=weight.dtype, device=dev)
+        g2, gs = _rows(grad, dim)
+        h2, hs = _rows(hidden, dim)
+        dp, ds = None, 0
+        if grad_hidden is not None:
+            d2, ds = _rows(grad_hidden, dim)
+            dp = d2.data_ptr()
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        if not inv_rms.is_contiguous():
+            inv_rms = inv_rms.contiguous()
+        rows = hidden.numel() // dim
+        grad_x = _like(hidden, ht)
+        grad_weight = torch.empty_like(weight)
         # the call's own scratch and no workspace of the stream: a captured call keeps it in its graph's memory
-        nbytes = int(lib.prime_rms_norm_backward_scratch_bytes(rows, dim))
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        rc = lib.prime_rms_norm_quantize_backward(g2.data_ptr(), g2.stride(0), h2.data_ptr(), h2.stride(0), weight.data_ptr(),
-                                                  inv_rms.data_ptr(), None if d2 is None else d2.data_ptr(), 0 if d2 is None else d2.stride(0),
-                                                  rows, dim, _TYPE[hidden.dtype], _TYPE[weight.dtype], grad_x.data_ptr(),
-                                                  grad_weight.data_ptr(), scratch.data_ptr(), nbytes, _stream(dev))
+        nbytes = lib.prime_rms_norm_backward_scratch_bytes(rows, dim)
+        scratch = hidden.new_empty((nbytes,), dtype=torch.uint8)
+        rc = lib.prime_rms_norm_quantize_backward(g2.data_ptr(), gs, h2.data_ptr(), hs, weight.data_ptr(), inv_rms.data_ptr(), dp, ds, rows, dim,
+                                                  _TYPE[ht], _TYPE[wt], grad_x.data_ptr(), grad_weight.data_ptr(), scratch.data_ptr(), nbytes, _stream(dev))
         if rc:
             _lib.check(rc, "prime_rms_norm_quantize_backward")
     return grad_x, grad_weight
@@ -174,13 +211,14 @@ def _quantize_4bit(weight, group_size=128, scale_dtype=torch.bfloat16):
     n, k = weight.shape
     groups = _groups(name, k, group_size)
     dev = weight.device
-    _check_inputs(name, dev, weight)
+    if _wants_gradient(weight):
+        _check_inputs(name, dev, weight)
     lib = _lib.load()
     with _on(dev):
-        w = _rows(weight, k)
-        packed = torch.empty((n, groups * group_size // 2), dtype=torch.uint8, device=dev)
-        scales = torch.empty((n, groups), dtype=scale_dtype, device=dev)
-        rc = lib.prime_quantize_4bit(w.data_ptr(), w.stride(0), n, k, _TYPE[w.dtype], group_size, _TYPE[scale_dtype], packed.data_ptr(),
+        w, stride = _rows(weight, k)
+        packed = weight.new_empty((n, groups * group_size // 2), dtype=torch.uint8)
+        scales = weight.new_empty((n, groups), dtype=scale_dtype)
+        rc = lib.prime_quantize_4bit(w.data_ptr(), stride, n, k, _TYPE[w.dtype], group_size, _TYPE[scale_dtype], packed.data_ptr(),
                                      scales.data_ptr(), _stream(dev))
         if rc:
             _lib.check(rc, "prime_quantize_4bit")
@@ -189,6 +227,15 @@ def _quantize_4bit(weight, group_size=128, scale_dtype=torch.bfloat16):
 
 def _check_packed(name: str, packed: torch.Tensor, scales: torch.Tensor, columns: Optional[int]) -> Tuple[int, int, int]:
     """(rows, columns, group size) of a 4-bit matrix."""
+    if packed.dtype is torch.uint8 and scales.dtype in _SCALES and packed.dim() == 2 and scales.dim() == 2:
+        n, held = packed.shape
+        rows, groups = scales.shape
+        held *= 2
+        if rows == n and groups > 0:
+            group = held // groups
+            k = held if columns is None else columns
+            if group in GROUP_SIZES and group * groups == held <= MAX_DIM and held - group < k <= held:
+                return n, k, group
     if packed.dtype != torch.uint8 or scales.dtype not in _SCALES:
         _fail(name, f"expected Byte codes and Float or BFloat16 scales but found {packed.dtype} and {scales.dtype}")
     if packed.dim() != 2 or scales.dim() != 2 or packed.shape[0] != scales.shape[0] or scales.shape[1] < 1:
@@ -204,7 +251,7 @@ def _check_packed(name: str, packed: torch.Tensor, scales: torch.Tensor, columns
 
 
 def _dense_rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
 def _dequantize_4bit(packed, scales, columns=None, dtype=torch.float32):
@@ -213,11 +260,12 @@ def _dequantize_4bit(packed, scales, columns=None, dtype=torch.float32):
     if dtype not in _FLOATS:
         _fail(name, f"weights are Float, BFloat16 or Half, got {dtype}")
     dev = packed.device
-    _check_inputs(name, dev, packed, scales)
+    if scales.device != dev or _wants_gradient(scales):
+        _check_inputs(name, dev, packed, scales)
     lib = _lib.load()
     with _on(dev):
         packed, scales = _dense_rows(packed), _dense_rows(scales)
-        out = torch.empty((n, k), dtype=dtype, device=dev)
+        out = packed.new_empty((n, k), dtype=dtype)
         rc = lib.prime_dequantize_4bit(packed.data_ptr(), packed.stride(0), scales.data_ptr(), scales.stride(0), n, k, group, _TYPE[scales.dtype],
                                        out.data_ptr(), _TYPE[dtype], _stream(dev))
         if rc:
@@ -247,16 +295,20 @@ def _matvec_4bit(x, packed, scales, x_scales=None, dtype=None):
     name = "matvec_4bit"
     n, k, group, dtype = _check_matvec(name, x, packed, scales, x_scales, dtype)
     dev = x.device
-    _check_inputs(name, dev, x, packed, scales, x_scales)
+    if packed.device != dev or scales.device != dev or (x_scales is not None and x_scales.device != dev) or _wants_gradient(x, scales, x_scales):
+        _check_inputs(name, dev, x, packed, scales, x_scales)
     lib = _lib.load()
     with _on(dev):
-        x2 = _rows(x, k)
+        x2, stride = _rows(x, k)
         packed, scales = _dense_rows(packed), _dense_rows(scales)
-        xs = None if x_scales is None else x_scales.contiguous()
-        out = torch.empty(x.shape[:-1] + (n,), dtype=dtype, device=dev)
-        rc = lib.prime_matvec_4bit(x2.data_ptr(), x2.stride(0), _TYPE[x.dtype], None if xs is None else xs.data_ptr(), packed.data_ptr(),
-                                   packed.stride(0), scales.data_ptr(), scales.stride(0), x2.shape[0], n, k, group, _TYPE[scales.dtype],
-                                   out.data_ptr(), _TYPE[dtype], _stream(dev))
+        xp = None
+        if x_scales is not None:
+            x_scales = x_scales.contiguous()
+            xp = x_scales.data_ptr()
+        shape = x.shape
+        out = x.new_empty((shape[0], n) if len(shape) == 2 else shape[:-1] + (n,), dtype=dtype)
+        rc = lib.prime_matvec_4bit(x2.data_ptr(), stride, _TYPE[x.dtype], xp, packed.data_ptr(), packed.stride(0), scales.data_ptr(), scales.stride(0),
+                                   x.numel() // k, n, k, group, _TYPE[scales.dtype], out.data_ptr(), _TYPE[dtype], _stream(dev))
         if rc:
             _lib.check(rc, "prime_matvec_4bit")
     return out
