@@ -141,11 +141,20 @@ void launch_matvec_few(MatvecArgs a, double bytes, hipStream_t st) {
     }
 }
 
-template <typename XT, int GS, int MT, int SPLIT>
-void launch_matvec_many_as(MatvecArgs a, bool scale_bf16, double bytes, hipStream_t st) {
-    a.sets = (a.n + 32 * (8 / SPLIT) - 1) / (32 * (8 / SPLIT));
-    constexpr int kRows = 16 * MT;
-    const int64_t row_tiles = (a.rows + kRows - 1) / kRows, step = std::max<int64_t>(1, (int64_t(1) << 22) / a.sets);
+template <typename XT, typename ST, int GS, int MT, int B, int NT>
+void launch_matvec_many_as(MatvecArgs a, double bytes, hipStream_t st) {
+    constexpr int kRows = 16 * MT, kPart = NT * MT * 256 * 4;
+    a.sets = (a.n + 16 * NT - 1) / (16 * NT);
+    const int64_t row_tiles = (a.rows + kRows - 1) / kRows;
+    const int visits = ((a.k + 127) / 128 + 8 * B - 1) / (8 * B);
+    // workgroups that stay for all their rounds, one a compute unit, all with as many (within one); with several visits LDS keeps the
+    // sums of at most 48 KiB of rounds
+    const int64_t most = visits > 1 ? (48 << 10) / kPart : int64_t(1) << 30;
+    const int64_t wanted = std::max<int64_t>(1, cu_count() / row_tiles), rounds = std::min<int64_t>(most, (a.sets + wanted - 1) / wanted);
+    const int per_row_tile = static_cast<int>((a.sets + rounds - 1) / rounds);
+    const int lds = visits > 1 ? static_cast<int>(rounds) * kPart : 0;
+    // a dispatch counts its work-items in 32 bits: 2^22 workgroups at a time
+    const int64_t step = std::max<int64_t>(1, (int64_t(1) << 22) / per_row_tile);
     const int type = a.out_type, rows = a.rows;
     for (int64_t at = 0; at < row_tiles; at += step) {
         MatvecArgs part = a;
@@ -154,23 +163,18 @@ void launch_matvec_many_as(MatvecArgs a, bool scale_bf16, double bytes, hipStrea
         part.x = static_cast<const XT*>(a.x) + row * a.x_stride;
         if (a.x_scales) part.x_scales = a.x_scales + row;
         part.out = static_cast<uint8_t*>(a.out) + row * a.n * type_bytes(type);
-        launch(kIdMatvec4, bytes, matvec4_many_kernel<XT, GS, MT, SPLIT>, static_cast<int>(a.sets * ((part.rows + kRows - 1) / kRows)), 512, st, part,
-               static_cast<int>(scale_bf16));
+        launch_lds(kIdMatvec4, bytes, matvec4_many_kernel<XT, ST, GS, MT, B, NT>, static_cast<int>(per_row_tile * ((part.rows + kRows - 1) / kRows)), 512, lds,
+                   st, part);
     }
 }
 
-template <typename XT, int GS>
-void launch_matvec_many(const MatvecArgs& a, bool scale_bf16, double bytes, hipStream_t st) {
-    const int64_t pairs = (a.n + 31) / 32;
-    if (a.rows <= 16) {
-        if (pairs * 2 >= cu_count() * 8) launch_matvec_many_as<XT, GS, 1, 2>(a, scale_bf16, bytes, st);
-        else launch_matvec_many_as<XT, GS, 1, sizeof(XT) == 4 ? 4 : 8>(a, scale_bf16, bytes, st);
-    } else if (a.rows <= 32 || sizeof(XT) == 4) {
-        if (pairs * 2 >= cu_count() * 8) launch_matvec_many_as<XT, GS, 2, 1>(a, scale_bf16, bytes, st);
-        else launch_matvec_many_as<XT, GS, 2, sizeof(XT) == 4 ? 2 : 4>(a, scale_bf16, bytes, st);
-    } else if constexpr (sizeof(XT) < 4) {
-        launch_matvec_many_as<XT, GS, 4, 2>(a, scale_bf16, bytes, st);
-    }
+// Tiles of rows, blocks of columns and tiles of outputs of a wavefront: what 256 registers hold.
+template <typename XT, typename ST, int GS>
+void launch_matvec_many(const MatvecArgs& a, double bytes, hipStream_t st) {
+    constexpr bool k32 = sizeof(XT) == 4, k8 = sizeof(XT) == 1;
+    if (a.rows <= 16) launch_matvec_many_as<XT, ST, GS, 1, k32 ? 2 : 4, 2>(a, bytes, st);
+    else if (a.rows <= 32 || k32) launch_matvec_many_as<XT, ST, GS, 2, k32 ? 1 : 4, k32 || k8 ? 2 : 1>(a, bytes, st);
+    else if constexpr (!k32) launch_matvec_many_as<XT, ST, GS, 4, 2, k8 ? 2 : 1>(a, bytes, st);
 }
 
 template <typename XT>
@@ -179,11 +183,8 @@ void launch_matvec(const MatvecArgs& a, int group, int scale_type, double bytes,
         constexpr int GS = decltype(gs)::value;
         with_scale_type(scale_type, [&](auto s) {
             if (a.rows <= 4) launch_matvec_few<XT, decltype(s), GS, 4>(a, bytes, st);
-            else if constexpr (sizeof(XT) == 1) {
-                if (a.rows <= 16) launch_matvec_few<XT, decltype(s), GS, 16>(a, bytes, st);
-            }
+            else launch_matvec_many<XT, decltype(s), GS>(a, bytes, st);
         });
-        if (a.rows > (sizeof(XT) == 1 ? 16 : 4)) launch_matvec_many<XT, GS>(a, scale_type == PRIME_BF16, bytes, st);
     };
     if (group == 32) go(std::integral_constant<int, 5>{});
     else if (group == 64) go(std::integral_constant<int, 6>{});

@@ -515,52 +515,60 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
 
 // ---- more rows: 16, 32 or 64 at a time ----
 // Here the matrix cores' work grows with the rows and the rows are taken as they are: bf16 and fp16 codes are widened beside an
-// offset (widen_word()), the sums of a group start from what the offset adds, taken off; fp32 rows are three bf16 rows,
-// which together are exact; int8 as above.  A wavefront takes 32 outputs, and every SPLIT-th stretch of 256 columns; the rows of
-// the workgroup's next stretches are on their way to registers while LDS holds the ones that are multiplied.
+// offset (widen_word()), and the sums of a group start from what the offset adds, taken off; fp32 rows are three bf16 rows,
+// which together are exact; int8 as above.  The rows stay where they are and the codes pass by: the eight wavefronts of a
+// workgroup split the columns, each holds its share of the rows in registers for all of the workgroup's outputs, and
+// only codes and scales are loaded in the loop, a round of outputs ahead (registers hold 8 to 16 KiB of them a wavefront).  The
+// wavefronts' sums of a round meet in LDS.  Rows too long for the registers take several visits, whose sums LDS keeps.
+// (The first form kept the rows in LDS and a barrier for every 256 columns: each stretch waited for its loads, 64 x 8192 x 22528 bf16
+// 91 us, 7 x 5604 x 11263 fp16 37 us.)
 
 template <typename XT> constexpr int kPlanes = sizeof(XT) == 4 ? 3 : 1;
-template <typename XT> constexpr int kPlaneBytes = sizeof(XT) == 1 ? 1 : 2;      // of an element in LDS
 
 __device__ __forceinline__ uint32_t pair16(uint32_t lo, uint32_t hi) { return (lo & 0xffffu) | hi << 16; }
 
-// Eight columns of a row as read.
-template <typename XT> struct Raw8 { uint32_t w[8 * sizeof(XT) / 4]; };
+// Eight columns of a row as the A operand wants them: 16-bit values in the order 0 4 1 5 2 6 3 7 (fp32 in three planes, each the
+// leading bits of what the ones before leave), bytes in the order 0 2 4 6 1 3 5 7.
+template <typename XT> struct Frag { typedef u32x4 type; };
+template <> struct Frag<int8_t> { typedef u32x2 type; };
 
 template <typename XT>
-__device__ __forceinline__ Raw8<XT> load_raw8(const XT* row, int64_t i, int n) {
-    struct __attribute__((packed, aligned(sizeof(XT)))) Loose { uint32_t w[8 * sizeof(XT) / 4]; };
-    Raw8<XT> r;
-    if (i + 8 <= n) {
-        const Loose t = *reinterpret_cast<const Loose*>(row + i);
+__device__ __forceinline__ void rows8(const XT* __restrict__ row, int64_t i, int n, typename Frag<XT>::type (&out)[kPlanes<XT>]) {
+    if constexpr (sizeof(XT) == 1) {
+        u32x2 v[1];
+        digits8<int8_t>(row, i, n, v);
+        out[0] = v[0];
+    } else if constexpr (sizeof(XT) == 2) {
+        typename Eight<XT>::type t;
+        if (i < n) {
+            t = take8(row, static_cast<int>(i), n);
+        } else {
 #pragma unroll
-        for (unsigned e = 0; e < 8 * sizeof(XT) / 4; ++e) r.w[e] = t.w[e];
+            for (int e = 0; e < 8; ++e) t[e] = static_cast<XT>(0.0f);
+        }
+        uint32_t b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = __builtin_bit_cast(uint16_t, static_cast<XT>(t[e]));
+        out[0] = u32x4{pair16(b[0], b[4]), pair16(b[1], b[5]), pair16(b[2], b[6]), pair16(b[3], b[7])};
     } else {
+        float v[8];
+        if (i < n) {
+            load8(row, static_cast<int>(i), n, v);
+        } else {
 #pragma unroll
-        for (unsigned e = 0; e < 8 * sizeof(XT) / 4; ++e) r.w[e] = 0;
+            for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+        }
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (i + e < n) {
-                if constexpr (sizeof(XT) == 4) r.w[e] = __builtin_bit_cast(uint32_t, row[i + e]);
-                else if constexpr (sizeof(XT) == 2) r.w[e >> 1] |= static_cast<uint32_t>(__builtin_bit_cast(uint16_t, row[i + e])) << (16 * (e & 1));
-                else r.w[e >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[i + e])) << (8 * (e & 3));
+        for (int p = 0; p < 3; ++p) {
+            uint32_t b[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                b[e] = __float_as_uint(v[e]) >> 16;
+                v[e] -= __uint_as_float(b[e] << 16);      // exact: the bits that are left
             }
+            out[p] = u32x4{pair16(b[0], b[4]), pair16(b[1], b[5]), pair16(b[2], b[6]), pair16(b[3], b[7])};
+        }
     }
-    return r;
-}
-
-// The sum of neighbouring lanes' values over a group's eights (4, 8 or 16 lanes of a row of 16), in all of them.
-template <int GS>
-__device__ __forceinline__ float group_sum(float v) {
-    auto turned = [](float f, auto n) {
-        return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(__float_as_uint(f)), static_cast<int>(__float_as_uint(f)),
-                                                                                 decltype(n)::value, 0xf, 0xf, false)));
-    };
-    v += turned(v, std::integral_constant<int, 0xb1>{});            // quad_perm 1 0 3 2
-    v += turned(v, std::integral_constant<int, 0x4e>{});            // quad_perm 2 3 0 1
-    if constexpr (GS >= 6) v += turned(v, std::integral_constant<int, 0x141>{});     // row_half_mirror: the other four of eight
-    if constexpr (GS == 7) v += turned(v, std::integral_constant<int, 0x140>{});     // row_mirror: the other eight
-    return v;
 }
 
 // f(0), f(1), ... with the index a constant: registers are indexed by it.
@@ -569,273 +577,187 @@ __device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>)
 template <int N, typename F>
 __device__ __forceinline__ void each(F&& f) { each_of<N>(static_cast<F&&>(f), std::make_integer_sequence<int, N>{}); }
 
-template <typename XT, int GS, int MT, int SPLIT>
-__global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a, int scale_bf16) {
+// MT tiles of 16 rows; B blocks of 128 columns a wavefront; NT tiles of 16 outputs a round.
+template <typename XT, typename ST, int GS, int MT, int B, int NT>
+__global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
     constexpr bool kInt = sizeof(XT) == 1;
-    constexpr int P = kPlanes<XT>, E8 = 8 * kPlaneBytes<XT>;               // bytes of eight columns in LDS
-    constexpr int NG = 1 << (7 - GS), NT = 2, BW = 2;
-    constexpr int kBlocks = BW * SPLIT;                                    // blocks of 128 columns in LDS
-    constexpr int kRows = 16 * MT;
-    constexpr int kRowBytes = kBlocks * 16 * E8 + 16;                      // 16 bytes more: rows start on other banks
-    constexpr int kEach = kRows * kBlocks * 16 / 512;                      // eights of x a lane brings
-    constexpr int kSide = 8 / SPLIT;
-    static_assert(kEach >= 1 && kRows * kBlocks * 16 % 512 == 0, "whole rounds of the workgroup");
-    constexpr int kRowArea = P * kRows * kRowBytes, kSumArea = 8 * NT * 256 * 4 * (SPLIT > 1);
-    __shared__ __align__(16) uint8_t lds[kRowArea > kSumArea ? kRowArea : kSumArea];
-    __shared__ __align__(16) float starts[kInt ? 1 : kBlocks * NG * kRows];       // [group][row]: -24 times the sum of its columns
+    constexpr int P = kPlanes<XT>, NG = 1 << (7 - GS), kRows = 16 * MT;
+    constexpr int RUN = B < 2 ? B : 2;                       // blocks side by side: whole lines of codes
+    constexpr int kPart = NT * MT * 256;                     // values of a round
+    typedef typename Frag<XT>::type frag;
+    typedef ST __attribute__((ext_vector_type(RUN * NG), aligned(sizeof(ST)))) run_scales;
+    __shared__ __align__(16) float part[8 * kPart];
+    __shared__ __align__(16) float starts[kInt ? 1 : 8 * B * NG * MT * 16];      // [wavefront][block][group][tile][row]: -24 times the sum of its columns
+    extern __shared__ __align__(16) float kept[];            // [own round][value], for rows that take several visits
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4, v16 = lane & 15;
-    const int kpart = wave % SPLIT, col = wave / SPLIT;
-    const int set = blockIdx.x % a.sets, row0 = blockIdx.x / a.sets * kRows;
+    const int per_row_tile = gridDim.x / ((a.rows + kRows - 1) / kRows);
+    const int row0 = blockIdx.x / per_row_tile * kRows, set0 = blockIdx.x % per_row_tile;
     const int rows = min(a.rows - row0, kRows);
-    const int blocks = (a.k + 127) >> 7, chunks = (blocks + kBlocks - 1) / kBlocks;
+    const int blocks = (a.k + 127) >> 7, visits = (blocks + 8 * B - 1) / (8 * B);
     const XT* x = static_cast<const XT*>(a.x) + static_cast<int64_t>(row0) * a.x_stride;
-    typedef u32x4 __attribute__((aligned(1))) u32x4u;
-    int n0[NT];
-    const uint8_t* codes[NT];
-    int64_t scale_row[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        n0[t] = ((set * kSide + col) * NT + t) * 16 + v16;
-        const int64_t n = min(n0[t], a.n - 1);
-        codes[t] = a.packed + n * a.p_stride + quarter * 16;
-        scale_row[t] = n * a.s_stride;
-    }
-    auto fetch_codes = [&](int chunk, u32x4 (&w)[NT][BW], uint32_t (&s)[NT][BW * NG]) {
-        const int b = chunk * kBlocks + kpart * BW;
-        const int there = a.groups - b * NG;
+    const ST* scales = static_cast<const ST*>(a.scales);
+    auto block_of = [&](int visit, int u) { return visit * 8 * B + u / RUN * (8 * RUN) + wave * RUN + u % RUN; };
+    auto fetch = [&](int visit, int set, u32x4 (&w)[NT][B], run_scales (&s)[NT][B / RUN]) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            if ((b + BW) * 64 <= a.row_bytes) {
+            const int64_t n = min((set * NT + t) * 16 + v16, a.n - 1);
+            const uint8_t* codes = a.packed + n * a.p_stride + quarter * 16;
+            const ST* sp = scales + n * a.s_stride;
 #pragma unroll
-                for (int u = 0; u < BW; ++u) w[t][u] = *reinterpret_cast<const u32x4u*>(codes[t] + static_cast<int64_t>(b + u) * 64);
-            } else {
+            for (int r = 0; r < B / RUN; ++r) {
+                typedef u32x4 __attribute__((aligned(1))) u32x4u;
+                const int b = block_of(visit, r * RUN);
+                if ((b + RUN) * 64 <= a.row_bytes) {
 #pragma unroll
-                for (int u = 0; u < BW; ++u)
-                    w[t][u] = (b + u) * 64 + quarter * 16 < a.row_bytes ? *reinterpret_cast<const u32x4u*>(codes[t] + static_cast<int64_t>(b + u) * 64) : u32x4{0, 0, 0, 0};
-            }
-            // scales as stored; behind the last group zeros
-            if (scale_bf16) {
-                const uint16_t* p = static_cast<const uint16_t*>(a.scales) + scale_row[t] + static_cast<int64_t>(b) * NG;
-                if (there >= BW * NG) {
-                    typedef uint16_t __attribute__((ext_vector_type(BW * NG), aligned(2))) some;
-                    const some v = *reinterpret_cast<const some*>(p);
-#pragma unroll
-                    for (int g = 0; g < BW * NG; ++g) s[t][g] = v[g];
+                    for (int u = 0; u < RUN; ++u) w[t][r * RUN + u] = *reinterpret_cast<const u32x4u*>(codes + static_cast<int64_t>(b + u) * 64);
+                    s[t][r] = *reinterpret_cast<const run_scales*>(sp + static_cast<int64_t>(b) * NG);
                 } else {
+                    // behind the row's end codes and scales are zero
 #pragma unroll
-                    for (int g = 0; g < BW * NG; ++g) s[t][g] = g < there ? p[g] : 0u;
-                }
-            } else {
-                const uint32_t* p = static_cast<const uint32_t*>(a.scales) + scale_row[t] + static_cast<int64_t>(b) * NG;
-                if (there >= BW * NG) {
-                    typedef uint32_t __attribute__((ext_vector_type(BW * NG), aligned(4))) some;
-                    const some v = *reinterpret_cast<const some*>(p);
+                    for (int u = 0; u < RUN; ++u)
+                        w[t][r * RUN + u] = (b + u) * 64 + quarter * 16 < a.row_bytes ? *reinterpret_cast<const u32x4u*>(codes + static_cast<int64_t>(b + u) * 64) : u32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int g = 0; g < BW * NG; ++g) s[t][g] = v[g];
-                } else {
-#pragma unroll
-                    for (int g = 0; g < BW * NG; ++g) s[t][g] = g < there ? p[g] : 0u;
+                    for (int g = 0; g < RUN * NG; ++g) s[t][r][g] = b * NG + g < a.groups ? sp[static_cast<int64_t>(b) * NG + g] : static_cast<ST>(0.0f);
                 }
             }
         }
     };
-    const int scale_shift = scale_bf16 ? 16 : 0;
-    auto widen_scales = [&](const uint32_t (&from)[NT][BW * NG], float (&to)[NT][BW * NG]) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int g = 0; g < BW * NG; ++g) to[t][g] = __uint_as_float(from[t][g] << scale_shift);
-    };
-    // A lane's eights of x: 16 lanes side by side take 128 columns of a row.
-    auto fetch_rows = [&](int chunk, Raw8<XT> (&r)[kEach]) {
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int i = threadIdx.x + e * 512, m = i / (kBlocks * 16), c = i % (kBlocks * 16);
-            r[e] = load_raw8(x + static_cast<int64_t>(min(m, rows - 1)) * a.x_stride, static_cast<int64_t>(chunk) * (kBlocks * 128) + c * 8, a.k);
-        }
-    };
-    auto put_rows = [&](const Raw8<XT> (&r)[kEach]) {
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const int i = threadIdx.x + e * 512, m = i / (kBlocks * 16), c = i % (kBlocks * 16), in = c & 15;
-            uint8_t* to = lds + m * kRowBytes + ((c & ~15) | (GS == 7 ? in : (in & 3) * 4 + (in >> 2))) * E8;
-            const auto& w = r[e].w;
-            if constexpr (kInt) {
-                *reinterpret_cast<u32x2*>(to) = u32x2{__builtin_amdgcn_perm(w[1], w[0], 0x06040200u), __builtin_amdgcn_perm(w[1], w[0], 0x07050301u)};
-            } else {
-                float v[8];
-                if constexpr (sizeof(XT) == 2) {
-                    // 0 4, 1 5, 2 6, 3 7
-                    *reinterpret_cast<u32x4*>(to) = u32x4{__builtin_amdgcn_perm(w[2], w[0], 0x05040100u), __builtin_amdgcn_perm(w[2], w[0], 0x07060302u),
-                                                          __builtin_amdgcn_perm(w[3], w[1], 0x05040100u), __builtin_amdgcn_perm(w[3], w[1], 0x07060302u)};
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        v[k] = static_cast<float>(__builtin_bit_cast(XT, static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1)))));
-                } else {
-                    float left[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) left[k] = v[k] = __uint_as_float(w[k]);
-#pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        uint32_t b[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            b[k] = __float_as_uint(left[k]) >> 16;
-                            left[k] -= __uint_as_float(b[k] << 16);      // exact: the bits that are left
-                        }
-                        *reinterpret_cast<u32x4*>(to + p * kRows * kRowBytes) = u32x4{pair16(b[0], b[4]), pair16(b[1], b[5]), pair16(b[2], b[6]), pair16(b[3], b[7])};
-                    }
-                }
-                const float sum = group_sum<GS>(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])));
-                if (in % (1 << (GS - 3)) == 0) starts[(c >> (GS - 3)) * kRows + m] = -24.0f * sum;
-            }
-        }
-    };
-    float y[NT][MT][4];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[t][m][i] = 0.0f;
-    u32x4 w[NT][BW];
-    uint32_t s2[NT][BW * NG];
-    float s[NT][BW * NG];
-    Raw8<XT> r[kEach];
-    fetch_codes(0, w, s2);
-    fetch_rows(0, r);
-    for (int chunk = 0; chunk < chunks; ++chunk) {
-        if (chunk) __syncthreads();
-        put_rows(r);
-        __syncthreads();
-        u32x4 w2[NT][BW];
-        widen_scales(s2, s);
-        const int next = min(chunk + 1, chunks - 1);
-        fetch_codes(next, w2, s2);
-        fetch_rows(next, r);
-        each<BW>([&](auto uc) {
+    u32x4 w[NT][B], w2[NT][B];
+    run_scales s[NT][B / RUN], s2[NT][B / RUN];
+    fetch(0, set0, w, s);
+    for (int visit = 0; visit < visits; ++visit) {
+        // this wavefront's columns of the rows; rows that do not exist repeat the last one, their sums are dropped
+        frag xa[B][P][MT][4];
+        each<B>([&](auto uc) {
             constexpr int u = decltype(uc)::value;
-            const int b = kpart * BW + u;
-            u32x4 v[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                v[t] = w[t][u];
-                if constexpr (GS < 7) transpose_quarters(v[t]);
-            }
-            const uint8_t* mine = lds + v16 * kRowBytes + (b * 16 + quarter * 4) * E8;
-            each<NG>([&](auto gc) {
-                constexpr int g = decltype(gc)::value;
-                constexpr int kSteps = 4 / NG;                       // words of a lane in a group
-                if constexpr (kInt) {
-                    i32x4 acc[NT][MT];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) acc[t][m] = i32x4{0, 0, 0, 0};
-                    constexpr int kPairs = kSteps >= 2 ? kSteps / 2 : 1;
-                    each<kPairs>([&](auto jc) {
-                        u32x4 cb[NT];
-                        constexpr int at = GS == 5 ? g : g * kSteps + 2 * decltype(jc)::value;
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            const uint32_t w0 = v[t][at], w1 = GS == 5 ? 0u : v[t][GS == 5 ? at : at + 1];
-                            cb[t] = u32x4{(w0 << 4) & 0xf0f0f0f0u, w0 & 0xf0f0f0f0u, (w1 << 4) & 0xf0f0f0f0u, w1 & 0xf0f0f0f0u};
-                        }
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            if constexpr (GS == 5) {
-                                const u32x2 xa = *reinterpret_cast<const u32x2*>(mine + m * 16 * kRowBytes + at * E8);
-#pragma unroll
-                                for (int t = 0; t < NT; ++t)
-                                    acc[t][m] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, xa), __builtin_bit_cast(long, u32x2{cb[t][0], cb[t][1]}),
-                                                                                      acc[t][m], 0, 0, 0);
-                            } else {
-                                const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + m * 16 * kRowBytes + at * E8);
-#pragma unroll
-                                for (int t = 0; t < NT; ++t)
-                                    acc[t][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, xa), __builtin_bit_cast(i32x4, cb[t]), acc[t][m], 0, 0, 0);
-                            }
-                        }
-                    });
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const float f = s[t][u * NG + g];
-#pragma unroll
-                        for (int m = 0; m < MT; ++m)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) y[t][m][i] = fmaf(static_cast<float>(acc[t][m][i]), f, y[t][m][i]);
-                    }
-                } else {
-                    f32x4 acc[NT][MT];
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        const f32x4 start = *reinterpret_cast<const f32x4*>(starts + (b * NG + g) * kRows + m * 16 + quarter * 4);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) acc[t][m] = start;
-                    }
-                    each<kSteps>([&](auto jc) {
-                        constexpr int j = g * kSteps + decltype(jc)::value;
-                        u32x4 cb[NT];
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) cb[t] = widen_word<!std::is_same<XT, _Float16>::value>(v[t][j]);
-#pragma unroll
-                        for (int p = 0; p < P; ++p)
-#pragma unroll
-                            for (int m = 0; m < MT; ++m) {
-                                const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + (p * kRows + m * 16) * kRowBytes + j * E8);
-#pragma unroll
-                                for (int t = 0; t < NT; ++t) acc[t][m] = product<XT>(xa, cb[t], acc[t][m]);
-                            }
-                    });
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const float f = s[t][u * NG + g];
-#pragma unroll
-                        for (int m = 0; m < MT; ++m)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) y[t][m][i] = fmaf(acc[t][m][i], f, y[t][m][i]);
-                    }
-                }
-            });
-        });
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int u = 0; u < BW; ++u) w[t][u] = w2[t][u];
-    }
-    auto put = [&](int t, int m, int i, float v) {
-        const int row = m * 16 + quarter * 4 + i;
-        if (row < rows && n0[t] < a.n) store_product(a, static_cast<int64_t>(row0 + row) * a.n + n0[t], kInt ? v * (a.x_scales[row0 + row] * 0.0625f) : v);
-    };
-    if constexpr (SPLIT == 1) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
+            const int64_t b = block_of(visit, u);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) put(t, m, i, y[t][m][i]);
-    } else {
-        // the wavefronts' sums, added in their order, 16 rows at a time
-        float* part = reinterpret_cast<float*>(lds);
+                for (int j = 0; j < 4; ++j) {
+                    frag f[P];
+                    rows8(x + static_cast<int64_t>(min(m * 16 + v16, rows - 1)) * a.x_stride, b * 128 + (GS == 7 ? quarter * 4 + j : j * 4 + quarter) * 8, a.k, f);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            __syncthreads();
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) part[((wave * NT + t) * 4 + i) * 64 + lane] = y[t][m][i];
-            __syncthreads();
-            // the wavefronts of a tile pair share its eight values a lane
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if ((t * 4 + i) % SPLIT != kpart) continue;
-                    float v = 0.0f;
-#pragma unroll
-                    for (int p = 0; p < SPLIT; ++p) v += part[(((col * SPLIT + p) * NT + t) * 4 + i) * 64 + lane];
-                    put(t, m, i, v);
+                    for (int p = 0; p < P; ++p) xa[u][p][m][j] = f[p];
                 }
+        });
+        if constexpr (!kInt) {
+            // what the offset of the codes adds to each group's sums, in the layout of the sums; a wavefront writes and reads its own
+            constexpr uint32_t kOff = std::is_same<XT, _Float16>::value ? 0xce00ce00u : 0xc1c0c1c0u;      // -24 twice
+            each<B>([&](auto uc) {
+                constexpr int u = decltype(uc)::value;
+                each<NG>([&](auto gc) {
+                    constexpr int g = decltype(gc)::value;
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        f32x4 acc{0, 0, 0, 0};
+                        each<4 / NG>([&](auto jc) {
+                            constexpr int j = g * (4 / NG) + decltype(jc)::value;
+#pragma unroll
+                            for (int p = 0; p < P; ++p) acc = product<XT>(xa[u][p][m][j], u32x4{kOff, kOff, kOff, kOff}, acc);
+                        });
+                        if (v16 == 0) *reinterpret_cast<f32x4*>(starts + (((wave * B + u) * NG + g) * MT + m) * 16 + quarter * 4) = acc;
+                    }
+                });
+            });
+            __builtin_amdgcn_wave_barrier();
+        }
+        int own = 0;
+        for (int set = set0; set < a.sets; set += per_row_tile, ++own) {
+            const bool more = set + per_row_tile < a.sets;
+            fetch(more ? visit : min(visit + 1, visits - 1), more ? set + per_row_tile : set0, w2, s2);
+            float y[NT][MT][4];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[t][m][i] = 0.0f;
+            each<B>([&](auto uc) {
+                constexpr int u = decltype(uc)::value;
+                if (block_of(visit, u) >= blocks) return;      // the same for the whole wavefront
+                each<NT>([&](auto tc) {
+                    constexpr int t = decltype(tc)::value;
+                    u32x4 v = w[t][u];
+                    if constexpr (GS < 7) transpose_quarters(v);
+                    each<NG>([&](auto gc) {
+                        constexpr int g = decltype(gc)::value, kSteps = 4 / NG;      // words of a lane in a group
+                        const float f = static_cast<float>(s[t][u / RUN][u % RUN * NG + g]);
+                        if constexpr (kInt) {
+                            i32x4 acc[MT];
+#pragma unroll
+                            for (int m = 0; m < MT; ++m) acc[m] = i32x4{0, 0, 0, 0};
+                            if constexpr (GS == 5) {
+                                const u32x2 cb{(v[g] << 4) & 0xf0f0f0f0u, v[g] & 0xf0f0f0f0u};
+#pragma unroll
+                                for (int m = 0; m < MT; ++m)
+                                    acc[m] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, xa[u][0][m][g]), __builtin_bit_cast(long, cb), acc[m], 0, 0, 0);
+                            } else {
+                                each<kSteps / 2>([&](auto jc) {
+                                    constexpr int j = g * kSteps + 2 * decltype(jc)::value;
+                                    const u32x4 cb{(v[j] << 4) & 0xf0f0f0f0u, v[j] & 0xf0f0f0f0u, (v[j + 1] << 4) & 0xf0f0f0f0u, v[j + 1] & 0xf0f0f0f0u};
+#pragma unroll
+                                    for (int m = 0; m < MT; ++m) {
+                                        const frag lo = xa[u][0][m][j], hi = xa[u][0][m][j + 1];
+                                        acc[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(i32x4{static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(hi[0]), static_cast<int>(hi[1])},
+                                                                                       __builtin_bit_cast(i32x4, cb), acc[m], 0, 0, 0);
+                                    }
+                                });
+                            }
+#pragma unroll
+                            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) y[t][m][i] = fmaf(static_cast<float>(acc[m][i]), f, y[t][m][i]);
+                        } else {
+                            f32x4 acc[MT];
+#pragma unroll
+                            for (int m = 0; m < MT; ++m) acc[m] = *reinterpret_cast<const f32x4*>(starts + (((wave * B + u) * NG + g) * MT + m) * 16 + quarter * 4);
+                            each<kSteps>([&](auto jc) {
+                                constexpr int j = g * kSteps + decltype(jc)::value;
+                                const u32x4 cb = widen_word<!std::is_same<XT, _Float16>::value>(v[j]);
+#pragma unroll
+                                for (int p = 0; p < P; ++p)
+#pragma unroll
+                                    for (int m = 0; m < MT; ++m) acc[m] = product<XT>(xa[u][p][m][j], cb, acc[m]);
+                            });
+#pragma unroll
+                            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) y[t][m][i] = fmaf(acc[m][i], f, y[t][m][i]);
+                        }
+                    });
+                });
+            });
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    *reinterpret_cast<f32x4*>(part + wave * kPart + ((t * MT + m) * 64 + lane) * 4) = f32x4{y[t][m][0], y[t][m][1], y[t][m][2], y[t][m][3]};
+            __syncthreads();
+            // the wavefronts' sums, added in their order, to those of the visits before
+            for (int i = threadIdx.x; i < kPart; i += 512) {
+                float v = part[i];
+#pragma unroll
+                for (int q = 1; q < 8; ++q) v += part[q * kPart + i];
+                if (visits > 1) {
+                    if (visit) v += kept[own * kPart + i];
+                    if (visit + 1 < visits) {
+                        kept[own * kPart + i] = v;
+                        continue;
+                    }
+                }
+                const int l = i >> 2 & 63, m = (i >> 8) % MT, t = (i >> 8) / MT;
+                const int row = m * 16 + (l >> 4) * 4 + (i & 3), n = (set * NT + t) * 16 + (l & 15);
+                if (row < rows && n < a.n) store_product(a, static_cast<int64_t>(row0 + row) * a.n + n, kInt ? v * (a.x_scales[row0 + row] * 0.0625f) : v);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                for (int u = 0; u < B; ++u) w[t][u] = w2[t][u];
+#pragma unroll
+                for (int r = 0; r < B / RUN; ++r) s[t][r] = s2[t][r];
+            }
         }
     }
 }
