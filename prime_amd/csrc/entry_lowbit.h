@@ -101,11 +101,11 @@ bool bad_group(int group) { return group != 32 && group != 64 && group != 128; }
 bool bad_matrix(int64_t n, int64_t k) { return n < 0 || n >= (int64_t(1) << 40) || k < 1 || k > kMaxDim; }
 int group_shift(int group) { return group == 32 ? 5 : group == 64 ? 6 : 7; }
 
-// Up to four floating rows at a time, or 16 of int8.
-template <typename XT, typename ST, int GS, int ROWS>
+// Up to four rows.
+template <typename XT, typename ST, int GS>
 void launch_matvec_few(MatvecArgs a, double bytes, hipStream_t st) {
     constexpr int kMostLds = 56 << 10;
-    const int held = std::min(a.rows, ROWS), quads = (a.k + 511) / 512, quad_bytes = 4 * kFewBlock<XT> + 16;
+    const int held = a.rows, quads = (a.k + 511) / 512, quad_bytes = 4 * kFewBlock<XT> + 16;
     a.tiles = (a.n + 15) / 16;
     // wavefronts that share a tile's columns: enough for 16 wavefronts a compute unit, but not more than it has stretches
     const int wanted = cu_count() * 16;
@@ -119,34 +119,25 @@ void launch_matvec_few(MatvecArgs a, double bytes, hipStream_t st) {
     const int side = waves >> a.split_shift;
     a.sets = (a.tiles + side - 1) / side;
     const int lds = held * (a.chunk_quads * quad_bytes + kFewPad<XT>);
-    int per_row_tile = a.sets;
+    int grid = a.sets;
     if (quads <= most && a.sets > cu_count()) {
         // workgroups that stay for all their tiles: as many as the device holds
         int fit = 0;
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&fit, matvec4_few_kernel<XT, ST, GS, ROWS>, waves * 64, lds) != hipSuccess || fit < 1) fit = 1;
-        per_row_tile = std::min(a.sets, cu_count() * fit);
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&fit, matvec4_few_kernel<XT, ST, GS>, waves * 64, lds) != hipSuccess || fit < 1) fit = 1;
+        grid = std::min(a.sets, cu_count() * fit);
     }
-    // a dispatch counts its work-items in 32 bits: 2^22 workgroups at a time
-    const int64_t row_tiles = (a.rows + ROWS - 1) / ROWS, step = std::max<int64_t>(1, (int64_t(1) << 22) / per_row_tile);
-    const int type = a.out_type, rows = a.rows;
-    for (int64_t at = 0; at < row_tiles; at += step) {
-        MatvecArgs part = a;
-        const int64_t row = at * ROWS;
-        part.rows = static_cast<int>(std::min<int64_t>(rows - row, step * ROWS));
-        part.x = static_cast<const XT*>(a.x) + row * a.x_stride;
-        if (a.x_scales) part.x_scales = a.x_scales + row;
-        part.out = static_cast<uint8_t*>(a.out) + row * a.n * type_bytes(type);
-        launch_lds(kIdMatvec4, bytes, matvec4_few_kernel<XT, ST, GS, ROWS>, static_cast<int>(per_row_tile * ((part.rows + ROWS - 1) / ROWS)), waves * 64, lds,
-                   st, part);
-    }
+    launch_lds(kIdMatvec4, bytes, matvec4_few_kernel<XT, ST, GS>, grid, waves * 64, lds, st, a);
 }
+
+// Times that rows of k columns are taken up by eight wavefronts of `blocks` blocks each.
+int visits_of(int k, int blocks) { return ((k + 127) / 128 + 8 * blocks - 1) / (8 * blocks); }
 
 template <typename XT, typename ST, int GS, int MT, int B, int NT>
 void launch_matvec_many_as(MatvecArgs a, double bytes, hipStream_t st) {
     constexpr int kRows = 16 * MT, kPart = NT * MT * 256 * 4;
     a.sets = (a.n + 16 * NT - 1) / (16 * NT);
     const int64_t row_tiles = (a.rows + kRows - 1) / kRows;
-    const int visits = ((a.k + 127) / 128 + 8 * B - 1) / (8 * B);
+    const int visits = visits_of(a.k, B);
     // workgroups that stay for all their rounds, one a compute unit, all with as many (within one); with several visits LDS keeps the
     // sums of at most 48 KiB of rounds
     const int64_t most = visits > 1 ? (48 << 10) / kPart : int64_t(1) << 30;
@@ -168,13 +159,21 @@ void launch_matvec_many_as(MatvecArgs a, double bytes, hipStream_t st) {
     }
 }
 
-// Tiles of rows, blocks of columns and tiles of outputs of a wavefront: what 256 registers hold.
+// Tiles of rows, blocks of columns and tiles of outputs of a wavefront: what 256 registers hold, next to the scales of a round (which
+// groups of 32 have four times as many of).  Up to 16 rows take six blocks and half the outputs where that saves a visit: 7 x 5604 x 11263
+// fp16 groups of 32 19 us against 23; where it does not, four blocks: 16 x 8192 x 22528 bf16 36 us (eight blocks do not fit: 40).
 template <typename XT, typename ST, int GS>
 void launch_matvec_many(const MatvecArgs& a, double bytes, hipStream_t st) {
-    constexpr bool k32 = sizeof(XT) == 4, k8 = sizeof(XT) == 1;
-    if (a.rows <= 16) launch_matvec_many_as<XT, ST, GS, 1, k32 ? 2 : 4, 2>(a, bytes, st);
-    else if (a.rows <= 32 || k32) launch_matvec_many_as<XT, ST, GS, 2, k32 ? 1 : 4, k32 || k8 ? 2 : 1>(a, bytes, st);
-    else if constexpr (!k32) launch_matvec_many_as<XT, ST, GS, 4, 2, k8 ? 2 : 1>(a, bytes, st);
+    constexpr bool k32 = sizeof(XT) == 4, k8 = sizeof(XT) == 1, kWide = GS == 5 && sizeof(ST) == 4 && !k8;
+    if (a.rows <= 16) {
+        if constexpr (k32) launch_matvec_many_as<XT, ST, GS, 1, 2, 2>(a, bytes, st);
+        else if (visits_of(a.k, 6) < visits_of(a.k, 4)) launch_matvec_many_as<XT, ST, GS, 1, 6, 1>(a, bytes, st);
+        else launch_matvec_many_as<XT, ST, GS, 1, 4, kWide ? 1 : 2>(a, bytes, st);
+    } else if (a.rows <= 32 || k32) {
+        launch_matvec_many_as<XT, ST, GS, 2, k32 ? 1 : kWide ? 2 : 4, k32 || k8 ? 2 : 1>(a, bytes, st);
+    } else if constexpr (!k32) {
+        launch_matvec_many_as<XT, ST, GS, 4, 2, k8 ? 2 : 1>(a, bytes, st);
+    }
 }
 
 template <typename XT>
@@ -182,7 +181,7 @@ void launch_matvec(const MatvecArgs& a, int group, int scale_type, double bytes,
     auto go = [&](auto gs) {
         constexpr int GS = decltype(gs)::value;
         with_scale_type(scale_type, [&](auto s) {
-            if (a.rows <= 4) launch_matvec_few<XT, decltype(s), GS, 4>(a, bytes, st);
+            if (a.rows <= 4) launch_matvec_few<XT, decltype(s), GS>(a, bytes, st);
             else launch_matvec_many<XT, decltype(s), GS>(a, bytes, st);
         });
     };
@@ -329,7 +328,9 @@ int prime_matvec_4bit(const void* x, int64_t x_stride, int x_type, const float* 
     if (!x || !packed || !scales || !out || (x_type == PRIME_I8) != (x_scales != nullptr))
         return fail(PRIME_EINVAL, "prime_matvec_4bit: null operand, or scales without int8 rows");
     const int64_t groups = (k + group - 1) / group;
-    MatvecArgs a{x, x_scales, packed, scales, out, x_stride, packed_stride, scale_stride, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k),
+    const int64_t scale_bytes = scale_stride * type_bytes(scale_type);
+    if (packed_stride > 0xffffffffLL || scale_bytes > 0xffffffffLL) return fail(PRIME_EINVAL, "prime_matvec_4bit: rows of codes or scales 4 GiB apart");
+    MatvecArgs a{x, x_scales, packed, scales, out, x_stride, static_cast<uint32_t>(packed_stride), static_cast<uint32_t>(scale_bytes), static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k),
                  static_cast<int>(groups * group / 2), static_cast<int>(groups), out_type, 0, 0, 0, 0};
     const double bytes = static_cast<double>(n) * k / 2 + static_cast<double>(n) * groups * type_bytes(scale_type) +
                          static_cast<double>(rows) * (k * type_bytes(x_type) + n * type_bytes(out_type));

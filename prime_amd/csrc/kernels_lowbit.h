@@ -237,7 +237,8 @@ struct MatvecArgs {
     const uint8_t* packed;
     const void* scales;
     void* out;                  // dense rows of n
-    int64_t x_stride, p_stride, s_stride;
+    int64_t x_stride;           // elements
+    uint32_t p_stride, s_stride; // bytes, from row to row of the codes and of the scales
     int rows;
     int n;
     int k;
@@ -297,7 +298,7 @@ __device__ __forceinline__ void store_product(const MatvecArgs& a, int64_t at, f
     else static_cast<_Float16*>(a.out)[at] = static_cast<_Float16>(v);
 }
 
-// ---- up to four floating rows, or 16 of int8: whole numbers up to the end of a group ----
+// ---- up to four rows: whole numbers up to the end of a group ----
 
 // Digits in base 256 that a value is taken to.
 template <typename XT> constexpr int kDigits = sizeof(XT) == 1 ? 1 : 4;
@@ -373,37 +374,33 @@ __device__ __forceinline__ float digits8(const XT* __restrict__ row, int64_t i, 
     }
 }
 
-template <typename XT, typename ST, int GS, int ROWS>
+template <typename XT, typename ST, int GS>
 __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
     constexpr bool kInt = sizeof(XT) == 1;
     constexpr int NG = 1 << (7 - GS);
     constexpr int kBlock = kFewBlock<XT>, D = kDigits<XT>;
-    constexpr int IR = ROWS / 4;                                         // sums of a lane
-    static_assert(kInt || ROWS == 4, "a row of four digits takes four rows of the A operand");
     extern __shared__ __align__(16) uint8_t few_lds[];
-    __shared__ float part[2][8 * IR * 64];
+    __shared__ float part[2][8 * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4, v16 = lane & 15;
     const int split = 1 << a.split_shift, kpart = wave & (split - 1);
     const int side = static_cast<int>(blockDim.x >> 6) >> a.split_shift;                    // tiles at a time
-    const int per_row_tile = gridDim.x / ((a.rows + ROWS - 1) / ROWS);                       // workgroups of a row tile
-    const int row0 = blockIdx.x / per_row_tile * ROWS, set0 = blockIdx.x % per_row_tile;
-    const int rows = min(a.rows - row0, ROWS);
+    const int stride = gridDim.x, set0 = blockIdx.x, rows = a.rows;
     const int quads = (a.k + 511) >> 9;
     const int row_stride = a.chunk_quads * 4 * kBlock + kFewPad<XT>;
     float* units = reinterpret_cast<float*>(few_lds + rows * row_stride);                    // [row][block of 128 columns]
-    // a lane's row of the A operand: digit v16 & 3 of row v16 >> 2; with 16 int8 rows the row v16.  Rows that do not exist repeat
-    // the last one; their sums are dropped
-    const int my_row = min(ROWS == 16 ? v16 : v16 >> 2, rows - 1);
+    // a lane's row of the A operand: digit v16 & 3 of row v16 >> 2 (int8: the row, four times).  Rows that do not exist repeat the
+    // last one; their sums are dropped
+    const int my_row = min(v16 >> 2, rows - 1);
     const uint8_t* mine = few_lds + my_row * row_stride + (kInt ? quarter * 32 : quarter * 128 + (v16 & 3) * 16);
     const float* unit = units + min(quarter, rows - 1) * (a.chunk_quads * 4);
-    const ST* scales = static_cast<const ST*>(a.scales);
+    const uint8_t* scales = static_cast<const uint8_t*>(a.scales);
     u32x4 w[4], w2[4];
     QuadScales<ST, GS> s, s2;
     auto fetch = [&](int set, int q, u32x4 (&to)[4], QuadScales<ST, GS>& sc) {
-        const int64_t n = min((set * side + (wave >> a.split_shift)) * 16 + v16, a.n - 1);
+        const uint32_t n = min((set * side + (wave >> a.split_shift)) * 16 + v16, a.n - 1);
         typedef u32x4 __attribute__((aligned(1))) u32x4u;
-        const uint8_t* p = a.packed + n * a.p_stride + static_cast<int64_t>(q) * 256 + quarter * 16;
-        const ST* sp = scales + n * a.s_stride + static_cast<int64_t>(q) * (4 * NG);
+        const uint8_t* p = a.packed + (static_cast<uint64_t>(n) * a.p_stride + static_cast<uint32_t>(q * 256 + quarter * 16));
+        const ST* sp = reinterpret_cast<const ST*>(scales + static_cast<uint64_t>(n) * a.s_stride) + q * (4 * NG);
         if ((q + 1) * 256 <= a.row_bytes) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) to[u] = *reinterpret_cast<const u32x4u*>(p + 64 * u);
@@ -415,7 +412,7 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
             sc.load_some(sp, a.groups - q * (4 * NG));
         }
     };
-    const XT* x = static_cast<const XT*>(a.x) + static_cast<int64_t>(row0) * a.x_stride;
+    const XT* x = static_cast<const XT*>(a.x);
     // Where a wavefront starts in its tile's columns: tiles side by side start at different ones, else all rows of
     // a matrix whose row length is a power of two would be read at the same offset at a time, from the same memory channels.
     const bool whole = a.chunk_quads >= quads;
@@ -424,10 +421,8 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
     int at = start(set0);
     fetch(set0, at, w, s);
     int turn = 0;
-    for (int set = set0; set < a.sets; set += per_row_tile, turn ^= 1) {
-        float y[IR];
-#pragma unroll
-        for (int i = 0; i < IR; ++i) y[i] = 0.0f;
+    for (int set = set0; set < a.sets; set += stride, turn ^= 1) {
+        float y = 0.0f;
         for (int first = 0; first < quads; first += a.chunk_quads) {
             const int held = min(a.chunk_quads, quads - first);
             if (set == set0 || held < quads) {
@@ -449,7 +444,7 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
             for (int i = kpart; i < held; i += split) {
                 const int q = at - first;
                 const bool more = first + i + split < quads;
-                const int next_set = more ? set : min(set + per_row_tile, a.sets - 1);
+                const int next_set = more ? set : min(set + stride, a.sets - 1);
                 at = !more ? start(next_set) : at + split < quads ? at + split : kpart;
                 fetch(next_set, at, w2, s2);
 #pragma unroll
@@ -475,8 +470,7 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
                     if constexpr (kInt) {
 #pragma unroll
                         for (int g = 0; g < NG; ++g)
-#pragma unroll
-                            for (int r = 0; r < IR; ++r) y[r] = fmaf(static_cast<float>(acc[g][r]), s.at(u * NG + g), y[r]);
+                            y = fmaf(static_cast<float>(acc[g][0]), s.at(u * NG + g), y);
                     } else {
                         // a digit's sum stays below 2^21: two digits go together in 32 bits, exactly
                         float t = 0.0f;
@@ -485,7 +479,7 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
                             const float hi = static_cast<float>(acc[g][0] * 256 + acc[g][1]), lo = static_cast<float>(acc[g][2] * 256 + acc[g][3]);
                             t = fmaf(fmaf(hi, 65536.0f, lo), s.at(u * NG + g), t);
                         }
-                        y[0] = fmaf(t, unit[q * 4 + u], y[0]);
+                        y = fmaf(t, unit[q * 4 + u], y);
                     }
                 }
 #pragma unroll
@@ -496,20 +490,13 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
         const int n = (set * side + (wave >> a.split_shift)) * 16 + v16;
         if (split > 1) {
             // the wavefronts' sums, added in their order; two buffers in turn, so that one barrier a set is enough
-#pragma unroll
-            for (int i = 0; i < IR; ++i) part[turn][(wave * IR + i) * 64 + lane] = y[i];
+            part[turn][wave * 64 + lane] = y;
             __syncthreads();
             if (kpart) continue;
-#pragma unroll
-            for (int i = 0; i < IR; ++i)
-                for (int p = 1; p < split; ++p) y[i] += part[turn][((wave + p) * IR + i) * 64 + lane];
+            for (int p = 1; p < split; ++p) y += part[turn][(wave + p) * 64 + lane];
         }
-#pragma unroll
-        for (int i = 0; i < IR; ++i) {
-            const int m = quarter * IR + i;
-            // codes were multiplied as 16 q
-            if (m < rows && n < a.n) store_product(a, static_cast<int64_t>(row0 + m) * a.n + n, kInt ? y[i] * (a.x_scales[row0 + m] * 0.0625f) : y[i] * 0.0625f);
-        }
+        // codes were multiplied as 16 q
+        if (quarter < rows && n < a.n) store_product(a, static_cast<int64_t>(quarter) * a.n + n, kInt ? y * (a.x_scales[quarter] * 0.0625f) : y * 0.0625f);
     }
 }
 
@@ -546,10 +533,11 @@ __device__ __forceinline__ void rows8(const XT* __restrict__ row, int64_t i, int
 #pragma unroll
             for (int e = 0; e < 8; ++e) t[e] = static_cast<XT>(0.0f);
         }
-        uint32_t b[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) b[e] = __builtin_bit_cast(uint16_t, static_cast<XT>(t[e]));
-        out[0] = u32x4{pair16(b[0], b[4]), pair16(b[1], b[5]), pair16(b[2], b[6]), pair16(b[3], b[7])};
+        typedef XT __attribute__((ext_vector_type(8))) eight;
+        const u32x4 b = __builtin_bit_cast(u32x4, static_cast<eight>(t));
+        // 0 4, 1 5, 2 6, 3 7
+        out[0] = u32x4{__builtin_amdgcn_perm(b[2], b[0], 0x05040100u), __builtin_amdgcn_perm(b[2], b[0], 0x07060302u),
+                       __builtin_amdgcn_perm(b[3], b[1], 0x05040100u), __builtin_amdgcn_perm(b[3], b[1], 0x07060302u)};
     } else {
         float v[8];
         if (i < n) {
@@ -595,14 +583,14 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
     const int rows = min(a.rows - row0, kRows);
     const int blocks = (a.k + 127) >> 7, visits = (blocks + 8 * B - 1) / (8 * B);
     const XT* x = static_cast<const XT*>(a.x) + static_cast<int64_t>(row0) * a.x_stride;
-    const ST* scales = static_cast<const ST*>(a.scales);
+    const uint8_t* scales = static_cast<const uint8_t*>(a.scales);
     auto block_of = [&](int visit, int u) { return visit * 8 * B + u / RUN * (8 * RUN) + wave * RUN + u % RUN; };
     auto fetch = [&](int visit, int set, u32x4 (&w)[NT][B], run_scales (&s)[NT][B / RUN]) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const int64_t n = min((set * NT + t) * 16 + v16, a.n - 1);
-            const uint8_t* codes = a.packed + n * a.p_stride + quarter * 16;
-            const ST* sp = scales + n * a.s_stride;
+            const uint32_t n = min((set * NT + t) * 16 + v16, a.n - 1);
+            const uint8_t* codes = a.packed + (static_cast<uint64_t>(n) * a.p_stride + quarter * 16);
+            const ST* sp = reinterpret_cast<const ST*>(scales + static_cast<uint64_t>(n) * a.s_stride);
 #pragma unroll
             for (int r = 0; r < B / RUN; ++r) {
                 typedef u32x4 __attribute__((aligned(1))) u32x4u;
@@ -735,20 +723,25 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
                     *reinterpret_cast<f32x4*>(part + wave * kPart + ((t * MT + m) * 64 + lane) * 4) = f32x4{y[t][m][0], y[t][m][1], y[t][m][2], y[t][m][3]};
             __syncthreads();
             // the wavefronts' sums, added in their order, to those of the visits before
-            for (int i = threadIdx.x; i < kPart; i += 512) {
-                float v = part[i];
+            for (int i = threadIdx.x; i < kPart / 4; i += 512) {
+                f32x4 v = reinterpret_cast<const f32x4*>(part)[i];
 #pragma unroll
-                for (int q = 1; q < 8; ++q) v += part[q * kPart + i];
+                for (int q = 1; q < 8; ++q) v += reinterpret_cast<const f32x4*>(part)[q * (kPart / 4) + i];
                 if (visits > 1) {
-                    if (visit) v += kept[own * kPart + i];
+                    f32x4* keep = reinterpret_cast<f32x4*>(kept) + own * (kPart / 4) + i;
+                    if (visit) v += *keep;
                     if (visit + 1 < visits) {
-                        kept[own * kPart + i] = v;
+                        *keep = v;
                         continue;
                     }
                 }
-                const int l = i >> 2 & 63, m = (i >> 8) % MT, t = (i >> 8) / MT;
-                const int row = m * 16 + (l >> 4) * 4 + (i & 3), n = (set * NT + t) * 16 + (l & 15);
-                if (row < rows && n < a.n) store_product(a, static_cast<int64_t>(row0 + row) * a.n + n, kInt ? v * (a.x_scales[row0 + row] * 0.0625f) : v);
+                const int l = i & 63, m = (i >> 6) % MT, t = (i >> 6) / MT;
+                const int row = m * 16 + (l >> 4) * 4, n = (set * NT + t) * 16 + (l & 15);
+                if (n >= a.n) continue;
+                const int64_t at = static_cast<int64_t>(row0 + row) * a.n + n;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (row + r < rows) store_product(a, at + static_cast<int64_t>(r) * a.n, kInt ? v[r] * (a.x_scales[row0 + row + r] * 0.0625f) : v[r]);
             }
             __syncthreads();
 #pragma unroll
