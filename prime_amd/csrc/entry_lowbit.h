@@ -165,7 +165,10 @@ void launch_matvec_many_as(MatvecArgs a, double bytes, hipStream_t st) {
 template <typename XT, typename ST, int GS>
 void launch_matvec_many(const MatvecArgs& a, double bytes, hipStream_t st) {
     constexpr bool k32 = sizeof(XT) == 4, k8 = sizeof(XT) == 1, kWide = GS == 5 && sizeof(ST) == 4 && !k8;
-    if (a.rows <= 16) {
+    // more rows in tiles of 16 all the same where each tile finds a compute unit of its own: a wavefront's work is then a
+    // quarter as long, and the codes that every tile reads come from the caches: 59 x 6720 x 76 bf16 34 us with 64 rows a workgroup
+    const bool small = (a.rows + 15) / 16 * ((static_cast<int64_t>(a.n) + 31) / 32) <= cu_count();
+    if (a.rows <= 16 || small) {
         if constexpr (k32) launch_matvec_many_as<XT, ST, GS, 1, 2, 2>(a, bytes, st);
         else if (visits_of(a.k, 6) < visits_of(a.k, 4)) launch_matvec_many_as<XT, ST, GS, 1, 6, 1>(a, bytes, st);
         else launch_matvec_many_as<XT, ST, GS, 1, 4, kWide ? 1 : 2>(a, bytes, st);
