@@ -29,13 +29,13 @@ from __future__ import annotations
 
 import re
 from functools import lru_cache
-from typing import List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 import torch.distributed as dist
 from torch import nn
 
-from . import ops
+from . import lowbit, ops
 from .collectives import all_reduce
 from .config import Compression
 
@@ -174,6 +174,18 @@ class Diloco:
         ops.outer_sgd_nesterov_segmented_([v[0] for v in self._views], [v[2] for v in self._views], [v[1] for v in self._views],
                                           [p.data.view(-1) for p in ps], self.outer_lr, OUTER_MOMENTUM, self._first_step)
         self._first_step = False
+
+    @torch.no_grad()
+    def outer_weights_4bit(self, model: nn.Module, group_size: int = 128,
+                           scale_dtype: torch.dtype = torch.bfloat16) -> Dict[str, Tuple[torch.Tensor, torch.Tensor]]:
+        """The outer copy's matrices as 4-bit codes and group scales, by parameter name: the weights that the last outer
+        step agreed on, in the form ``lowbit.matvec_4bit`` takes, for evaluation or decoding between outer steps (the
+        inner weights drift from them).  Parameters of other than two dimensions (norm weights, biases) are left out."""
+        out = {}
+        for (name, p), view in zip(((n, p) for n, p in model.named_parameters() if p.requires_grad), self._views):
+            if p.dim() == 2:
+                out[name] = lowbit.quantize_4bit(view[0].view(p.shape), group_size, scale_dtype)
+        return out
 
     @torch.no_grad()
     def step(self, model: nn.Module, group: Optional[object] = None, world_size: Optional[int] = None, fake: bool = False,

@@ -274,6 +274,96 @@ def test_matvec_4bit_rows(dev, rows, xt):
             check_matvec(dev, x.to(xt), xs, codes, s, k, dt)
 
 
+@pytest.mark.parametrize("rows,n,k", [(24, 4200, 700), (64, 2090, 4300), (70, 2100, 2100), (9, 8300, 6000)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("xt", [BF16, F16, F32, I8], ids=NAMES.get)
+def test_matvec_4bit_many_rows_and_outputs(dev, rows, n, k, group, xt):
+    # more tiles of 16 rows by 32 outputs than compute units: the kernels that take 32 and 64 rows at a time, rows in several visits
+    g = gen("many", rows, n, k, group, str(xt))
+    for st in (F32, BF16):
+        announce(f"matvec {rows} x {k} x {n} group {group} {xt} {st}")
+        codes, s = four_bit(g, n, k, group, st)
+        x, xs = rows_like_activations(g, rows, k, F32), None
+        if xt == I8:
+            x, xs = torch.randint(-128, 128, (rows, k), generator=g).to(I8), torch.rand(rows, generator=g) * 0.05
+        check_matvec(dev, x.to(xt), xs, codes, s, k)
+
+
+def test_offsets_beyond_32_bits(dev):
+    g = gen("far")
+    announce("rows far apart")
+    base = torch.zeros(40, 1 << 27, dtype=torch.uint8, device=dev)          # 5 GiB: row 32 starts at 2^32
+    codes, s = four_bit(g, 40, 96, 32, F32)
+    packed = base[:, 1000:1048]
+    packed.copy_(ref.pack(codes))
+    x = rows_like_activations(g, 6, 96, BF16)
+    for rows in (1, 6):
+        got = lowbit.matvec_4bit(x[:rows].to(dev), packed, s.to(dev))
+        want, bound = ref.matvec(x[:rows], None, codes, s, 96)
+        assert ref.outside(got.cpu(), want, bound) <= 0
+    assert torch.equal(lowbit.dequantize_4bit(packed, s.to(dev)).cpu(), codes.float() * s.repeat_interleave(32, 1))
+    view = base.view(torch.bfloat16)[:, 512:812]
+    x = rows_like_activations(g, 40, 300, BF16)
+    view.copy_(x)
+    w = 1 + 0.1 * torch.randn(300, generator=g)
+    codes8, scales, inv = lowbit.rms_norm_quantize(view, w.to(dev))
+    check_norm((codes8, scales, None, inv), x, None, w, 1e-6, I8)
+    wx, ww, bx, bw = ref.norm_backward(x, x, w, inv.cpu())
+    gx, gw = lowbit.rms_norm_quantize_backward(view, view, w.to(dev), inv)
+    assert ref.outside(gx.cpu(), wx, bx) <= 0 and ref.outside(gw.cpu(), ww, bw) <= 0
+    want4, ws = ref.quantize_4bit(x, 64, BF16)
+    got4, gs = lowbit.quantize_4bit(view, 64, BF16)
+    assert torch.equal(got4.cpu(), ref.pack(want4)) and torch.equal(gs.cpu(), ws)
+
+
+def test_large_codes_and_outputs_leave_their_neighbours_alone(dev):
+    # outputs are written inside their own tensors only: guards on both sides of every output of the C calls
+    from prime_amd import _lib
+
+    lib = _lib.load()
+    st = torch.cuda.current_stream(dev).cuda_stream
+    g = gen("guards")
+    for rows, dim in ((3, 77), (5, 1030), (2, 5001)):
+        x, w = rows_like_activations(g, rows, dim, BF16).to(dev), torch.ones(dim, device=dev)
+        out = torch.full((rows * dim + 128,), 0x5A, dtype=torch.uint8, device=dev)
+        sc = torch.full((2 * rows + 128,), 7.0, device=dev)
+        hid = torch.full((rows * dim + 128,), 9.0, dtype=BF16, device=dev)
+        rc = lib.prime_rms_norm_quantize(x.data_ptr(), dim, x.data_ptr(), dim, w.data_ptr(), rows, dim, 1, 0, 3, 1e-6, out[64:].data_ptr(),
+                                         sc[64:].data_ptr(), hid[64:].data_ptr(), sc[64 + rows:].data_ptr(), st)
+        assert rc == 0
+        assert (out[:64] == 0x5A).all() and (out[64 + rows * dim:] == 0x5A).all()
+        assert (sc[:64] == 7).all() and (sc[64 + 2 * rows:] == 7).all() and (hid[:64] == 9).all() and (hid[64 + rows * dim:] == 9).all()
+    for rows, n, k in ((1, 37, 300), (9, 37, 300), (20, 4099, 130), (70, 2061, 200)):
+        codes, s = four_bit(g, n, k, 64, F32)
+        packed, sd, x = ref.pack(codes).to(dev), s.to(dev), rows_like_activations(g, rows, k, BF16).to(dev)
+        y = torch.full((rows * n + 128,), 3.0, device=dev)
+        rc = lib.prime_matvec_4bit(x.data_ptr(), k, 1, None, packed.data_ptr(), packed.stride(0), sd.data_ptr(), sd.stride(0), rows, n, k, 64, 0,
+                                   y[64:].data_ptr(), 0, st)
+        assert rc == 0 and (y[:64] == 3).all() and (y[64 + rows * n:] == 3).all()
+
+
+def test_outer_weights_in_4_bits(dev):
+    from prime_amd.diloco import Diloco
+
+    torch.manual_seed(3)
+    model = torch.nn.Sequential(torch.nn.Linear(130, 70), torch.nn.LayerNorm(70), torch.nn.Linear(70, 33, bias=False)).to(dev)
+    d = Diloco(0.7, model)
+    start = {n: p.detach().cpu().clone() for n, p in model.named_parameters()}
+    with torch.no_grad():
+        for p in model.parameters():
+            p.add_(0.1)                          # inner training: the outer copy stays
+    got = d.outer_weights_4bit(model, 64, F32)
+    assert set(got) == {"0.weight", "2.weight"}
+    for name, (packed, scales) in got.items():
+        codes, s = ref.quantize_4bit(start[name], 64, F32)
+        assert torch.equal(packed.cpu(), ref.pack(codes)) and torch.equal(scales.cpu(), s)
+    x = torch.randn(1, 130, generator=gen("outer"))
+    y = lowbit.matvec_4bit(x.to(dev), *got["0.weight"])
+    codes, s = ref.quantize_4bit(start["0.weight"], 64, F32)
+    want, bound = ref.matvec(x, None, codes, s, 130)
+    assert ref.outside(y.cpu(), want, bound) <= 0
+
+
 def test_matvec_4bit_rows_are_independent_and_each_sees_what_is_not_finite(dev):
     g = gen("special matvec")
     for xt in (BF16, F16, F32):

@@ -124,8 +124,11 @@ def test_c_abi_refuses_bad_arguments_before_any_launch():
 
     assert mv(rows=0, x=None) == 0 and mv(n=0, out=None) == 0
     for bad in (dict(x=None), dict(packed=None), dict(scales=None), dict(out=None), dict(xt=4), dict(xt=3), dict(xs=p), dict(rows=-1), dict(n=-1), dict(k=0),
-                dict(g=33), dict(st=2), dict(ot=3)):
+                dict(g=33), dict(st=2), dict(ot=3), dict(n=(1 << 26) + 1)):
         assert mv(**bad) == -1, bad
+    # rows of codes or scales 4 GiB apart
+    assert lib.prime_matvec_4bit(p, 64, 0, None, p, 1 << 32, p, 1, 2, 3, 64, 64, 0, p, 0, None) == -1
+    assert lib.prime_matvec_4bit(p, 64, 0, None, p, 32, p, 1 << 30, 2, 3, 64, 64, 0, p, 0, None) == -1
 
 
 def test_reference_rounds_to_e4m3_as_the_type_is_defined():
