@@ -399,8 +399,12 @@ int prime_dequantize_4bit(const uint8_t* packed, int64_t packed_stride, const vo
 /* Products of rows with such a matrix: out[m][i] = x_scales[m] * sum over groups of scale[i][g] * sum over the
  * group's j of code[i][j] * x[m][j], rounded once to out_type (dense rows of n).  x: PRIME_F32, PRIME_BF16 or PRIME_F16
  * rows (x_scales NULL), or PRIME_I8 codes with a scale per row, as prime_rms_norm_quantize gives them: the
- * sums within a group are then exact.  Meant for the few rows of a decoding step; many rows (hundreds) are better
- * served by prime_dequantize_4bit and a library product. */
+ * sums within a group are then exact.  Floating rows are summed in 32 bits: up to four rows as fixed point of 31 bits
+ * under the largest magnitude of each 128 columns, more rows as they are (the last bits can depend on the number of
+ * rows).  A row that holds a value that is not finite has no finite products; other rows are not touched.  Magnitudes
+ * beyond 2^120 may overflow before their group's scale is applied.  n <= 2^26; rows of codes and of scales less than
+ * 4 GiB apart.  Meant for the few rows of a decoding step; many rows (hundreds) are better served by
+ * prime_dequantize_4bit and a library product. */
 int prime_matvec_4bit(const void* x, int64_t x_stride, int x_type, const float* x_scales, const uint8_t* packed,
                       int64_t packed_stride, const void* scales, int64_t scale_stride, int64_t rows, int64_t n,
                       int64_t k, int group, int scale_type, void* out, int out_type, prime_stream_t stream);

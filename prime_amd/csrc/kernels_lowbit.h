@@ -210,19 +210,15 @@ __global__ __launch_bounds__(256) void group4_unpack_kernel(UnpackArgs a) {
 //
 //   y[m][n] = x_scale[m] * sum over groups g of scale[n][g] * sum over k in g of q[n][k] x[m][k]
 //
-// Everything is whole numbers up to the end of a group.  Codes become bytes by two masks and a shift a word of eight: a code in
-// the upper half of a byte is 16 q.  int8 rows are taken as they are.  Floating rows become fixed point under the largest
-// magnitude of each 128 columns, in base 256 digits of -128 .. 127: three digits for bf16 and fp16 (23 bits, so a value within
-// 2^-24 of a bound of the largest, what a 32-bit sum with it would keep), four for fp32 (31 bits).  A product's sums are
-// exact in each digit; the digits' sums are put together and scaled in fp32.
-// (The other way, codes widened to bf16 or fp16 for the rows as they are, takes 8 instructions a word instead of 3 and an offset's
-// second product: 1 x 8192 x 128000 bf16 114 us.)
+// Rows of x are the A operand of 16 x 16 matrix instructions, 16 outputs n the B operand.  A wavefront takes 128 columns of 16
+// outputs at a time: lane (n, quarter) loads 16 bytes of row n, so codes go from memory to the matrix cores through registers
+// alone.  With groups of 128 any order of k within them does; with smaller ones the words are transposed between the
+// quarters (four instructions for four words), so that an instruction's columns lie in one group and its sums can be scaled on
+// their own.  The rows are brought into the order in which codes come out of their words.
 //
-// Rows of x are the A operand of 16 x 16 x 64 matrix instructions, 16 outputs n the B operand.  A wavefront takes 128 columns
-// of 16 outputs at a time: lane (n, quarter) loads 16 bytes of row n, so codes go from memory to the matrix cores through
-// registers alone.  With groups of 128 any order of k within them does; with smaller ones the words are transposed between the
-// quarters (four instructions for four words), so that an instruction's columns lie in one group and its sums can be
-// scaled on their own.  The rows of x are brought to LDS once a workgroup, in the order in which codes come out of their words.
+// Two kernels.  Up to four rows are bound by the codes' way from memory: everything is whole numbers up to the end of a group, so
+// that a word of eight codes costs three instructions (a code in the upper half of a byte is 16 q).  More rows are bound by
+// instructions: they are multiplied as they are, at eight instructions a word.
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -299,6 +295,15 @@ __device__ __forceinline__ void store_product(const MatvecArgs& a, int64_t at, f
 }
 
 // ---- up to four rows: whole numbers up to the end of a group ----
+// int8 rows are taken as they are.  Floating rows become fixed point under the largest magnitude of each 128 columns: 31 bits, as
+// four digits of -128 .. 127 in base 256, so a value is off by at most 2^-31 of that largest (a 32-bit sum that holds both loses
+// more).  The four digits of a row are four rows of the A operand, so one matrix instruction takes them all; a group's sums are
+// exact in each digit, two digits are put together exactly in 32 bits, and the rest is fp32.
+//
+// Bound by memory from a few thousand outputs up: 1 x 8192 x 128000 int8 92 us (5.9 TB/s; with the products taken out and the loads left
+// in 97, with loads that cover whole lines instead of 64 bytes of 16 rows 90), bf16 104 us (5.2 TB/s); the same with the codes widened to
+// bf16, at eight instructions a word beside an offset's second product, 121.  Small products are a launch and two trips
+// to memory: 1 x 2048 x 2048 4.1 us, 1 x 4096 x 4096 5.0 us.
 
 // Digits in base 256 that a value is taken to.
 template <typename XT> constexpr int kDigits = sizeof(XT) == 1 ? 1 : 4;
@@ -505,10 +510,12 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
 // offset (widen_word()), and the sums of a group start from what the offset adds, taken off; fp32 rows are three bf16 rows,
 // which together are exact; int8 as above.  The rows stay where they are and the codes pass by: the eight wavefronts of a
 // workgroup split the columns, each holds its share of the rows in registers for all of the workgroup's outputs, and
-// only codes and scales are loaded in the loop, a round of outputs ahead (registers hold 8 to 16 KiB of them a wavefront).  The
-// wavefronts' sums of a round meet in LDS.  Rows too long for the registers take several visits, whose sums LDS keeps.
-// (The first form kept the rows in LDS and a barrier for every 256 columns: each stretch waited for its loads, 64 x 8192 x 22528 bf16
-// 91 us, 7 x 5604 x 11263 fp16 37 us.)
+// only codes and scales are loaded in the loop, a round of outputs ahead.  The wavefronts' sums of a round meet in LDS.  Rows too
+// long for the registers take several visits, whose sums LDS keeps.
+// Bound by instructions: 16 x 8192 x 22528 bf16 36 us, 64 rows 74 us (of each SIMD's cycles 38 % are vector and 16 % matrix
+// instructions, which do not overlap in two wavefronts; the rest is the rounds' ends and loads of the rows); a round more of codes on
+// their way changes nothing (76 us).  The first form kept the rows in LDS, with a barrier for every 256 columns: each stretch waited for
+// its loads, 64 x 8192 x 22528 91 us, 7 x 5604 x 11263 fp16 37 us against 19.
 
 template <typename XT> constexpr int kPlanes = sizeof(XT) == 4 ? 3 : 1;
 

@@ -11,6 +11,11 @@
 // value overflows fp32; at 8 bytes of traffic an element the fp64 additions cost nothing).
 // A row that holds a value that is not finite, or whose product with the weight is not, gets scale NaN and codes 0.
 //
+// Bound by memory: 16384 x 4096 bf16 with residual 74 us (6.35 TB/s; a plain copy reaches 6.8), its gradient with that of the sum 89 us
+// (6.0 TB/s, of which 4 us the second launch that adds up the weight's gradient).  A row is one visit: from registers, a
+// workgroup a row from 1025 elements up (four rows a workgroup below), and a workgroup that ends after its row, so that no wavefront
+// waits for its own stores.  Eight roundings to codes share one test for borders: one at a time they took 96 us instead of 82.
+//
 // Included by prime_hip.hip inside its anonymous namespace; not a translation unit of its own.
 
 // Eight consecutive elements of a row, at element alignment (a row of odd length starts anywhere).

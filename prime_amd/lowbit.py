@@ -420,9 +420,15 @@ def dequantize_4bit(packed: torch.Tensor, scales: torch.Tensor, columns: Optiona
 def matvec_4bit(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, x_scales: Optional[torch.Tensor] = None,
                 dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``x @ dequantize_4bit(packed, scales, k).T`` for ``x`` [..., k], without the matrix: [..., n].  ``x`` is Float, BFloat16 or
-    Half (32-bit sums, products exact), or int8 codes with ``x_scales`` (Float, one a row), as ``rms_norm_quantize`` gives them
-    (sums within a group exact).  ``dtype``: of the products, rounded once; default the rows' type, Float for int8 rows.
-    Meant for the rows of a decoding step; for hundreds of rows take ``dequantize_4bit`` and a library product."""
+    Half, or int8 codes with ``x_scales`` (Float, one a row), as ``rms_norm_quantize`` gives them (sums within a group exact).
+    ``dtype``: of the products, rounded once; default the rows' type, Float for int8 rows.
+
+    Floating rows are summed in 32 bits: up to four rows as fixed point of 31 bits under the largest magnitude of each 128
+    columns, more rows as they are, so the last bits of a row's products can depend on how many rows come with it.  A row that holds a
+    value that is not finite has no finite products (other rows are not touched), and magnitudes beyond 2^120 may overflow before their
+    group's scale is applied.  At most 2^26 outputs; rows of ``packed`` and ``scales`` may be slices of a larger matrix,
+    less than 4 GiB apart.  Meant for the rows of a decoding step; for hundreds of rows take ``dequantize_4bit`` and a library
+    product."""
     if _plain(x):
         return _matvec_4bit(x, packed, scales, x_scales, dtype)
     return torch.ops.prime_lowbit.matvec_4bit(x, packed, scales, x_scales, dtype)
