@@ -517,6 +517,7 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
 // their way changes nothing (76 us).  The first form kept the rows in LDS, with a barrier for every 256 columns: each stretch waited for
 // its loads, 64 x 8192 x 22528 91 us, 7 x 5604 x 11263 fp16 37 us against 19.
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 template <typename XT> constexpr int kPlanes = sizeof(XT) == 4 ? 3 : 1;
 
 __device__ __forceinline__ uint32_t pair16(uint32_t lo, uint32_t hi) { return (lo & 0xffffu) | hi << 16; }
@@ -581,7 +582,9 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
     constexpr int kPart = NT * MT * 256;                     // values of a round
     typedef typename Frag<XT>::type frag;
     typedef ST __attribute__((ext_vector_type(RUN * NG), aligned(sizeof(ST)))) run_scales;
-    __shared__ __align__(16) float part[8 * kPart];
+    constexpr int kBuffers = kPart > 1024 ? 1 : 2;
+    __shared__ __align__(16) float part_of[kBuffers][8 * kPart];
+    int turn = 0;
     __shared__ __align__(16) float starts[kInt ? 1 : 8 * B * NG * MT * 16];      // [wavefront][block][group][tile][row]: -24 times the sum of its columns
     extern __shared__ __align__(16) float kept[];            // [own round][value], for rows that take several visits
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4, v16 = lane & 15;
@@ -661,6 +664,8 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
         for (int set = set0; set < a.sets; set += per_row_tile, ++own) {
             const bool more = set + per_row_tile < a.sets;
             fetch(more ? visit : min(visit + 1, visits - 1), more ? set + per_row_tile : set0, w2, s2);
+            float* part = part_of[turn & (kBuffers - 1)];
+            ++turn;
             float y[NT][MT][4];
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -730,27 +735,27 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
                     *reinterpret_cast<f32x4*>(part + wave * kPart + ((t * MT + m) * 64 + lane) * 4) = f32x4{y[t][m][0], y[t][m][1], y[t][m][2], y[t][m][3]};
             __syncthreads();
             // the wavefronts' sums, added in their order, to those of the visits before
-            for (int i = threadIdx.x; i < kPart / 4; i += 512) {
-                f32x4 v = reinterpret_cast<const f32x4*>(part)[i];
+            for (int i = threadIdx.x; i < kPart / 2; i += 512) {
+                f32x2 v = reinterpret_cast<const f32x2*>(part)[i];
 #pragma unroll
-                for (int q = 1; q < 8; ++q) v += reinterpret_cast<const f32x4*>(part)[q * (kPart / 4) + i];
+                for (int q = 1; q < 8; ++q) v += reinterpret_cast<const f32x2*>(part)[q * (kPart / 2) + i];
                 if (visits > 1) {
-                    f32x4* keep = reinterpret_cast<f32x4*>(kept) + own * (kPart / 4) + i;
+                    f32x2* keep = reinterpret_cast<f32x2*>(kept) + own * (kPart / 2) + i;
                     if (visit) v += *keep;
                     if (visit + 1 < visits) {
                         *keep = v;
                         continue;
                     }
                 }
-                const int l = i & 63, m = (i >> 6) % MT, t = (i >> 6) / MT;
-                const int row = m * 16 + (l >> 4) * 4, n = (set * NT + t) * 16 + (l & 15);
+                const int l = i >> 1 & 63, m = (i >> 7) % MT, t = (i >> 7) / MT;
+                const int row = m * 16 + (l >> 4) * 4 + (i & 1) * 2, n = (set * NT + t) * 16 + (l & 15);
                 if (n >= a.n) continue;
                 const int64_t at = static_cast<int64_t>(row0 + row) * a.n + n;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
+                for (int r = 0; r < 2; ++r)
                     if (row + r < rows) store_product(a, at + static_cast<int64_t>(r) * a.n, kInt ? v[r] * (a.x_scales[row0 + row + r] * 0.0625f) : v[r]);
             }
-            __syncthreads();
+            if constexpr (kBuffers == 1) __syncthreads();
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
 #pragma unroll
