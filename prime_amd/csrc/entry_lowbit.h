@@ -161,7 +161,7 @@ void launch_matvec_many_as(MatvecArgs a, double bytes, hipStream_t st) {
 
 // Tiles of rows, blocks of columns and tiles of outputs of a wavefront: what 256 registers hold, next to the scales of a round (which
 // groups of 32 have four times as many of).  Up to 16 rows take six blocks and half the outputs where that saves a visit: 7 x 5604 x 11263
-// fp16 groups of 32 19 us against 23; where it does not, four blocks: 16 x 8192 x 22528 bf16 36 us (eight blocks do not fit: 40).
+// fp16 groups of 32 19 us against 23; where it does not, four blocks: 16 x 8192 x 22528 bf16 33 us (eight blocks do not fit: 40).
 template <typename XT, typename ST, int GS>
 void launch_matvec_many(const MatvecArgs& a, double bytes, hipStream_t st) {
     constexpr bool k32 = sizeof(XT) == 4, k8 = sizeof(XT) == 1, kWide = GS == 5 && sizeof(ST) == 4 && !k8;

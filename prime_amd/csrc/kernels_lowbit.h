@@ -217,8 +217,8 @@ __global__ __launch_bounds__(256) void group4_unpack_kernel(UnpackArgs a) {
 // their own.  The rows are brought into the order in which codes come out of their words.
 //
 // Two kernels.  Up to four rows are bound by the codes' way from memory: everything is whole numbers up to the end of a group, so
-// that a word of eight codes costs three instructions (a code in the upper half of a byte is 16 q).  More rows are bound by
-// instructions: they are multiplied as they are, at eight instructions a word.
+// that a word of eight codes costs three instructions (a code in the upper half of a byte is 16 q).  More rows are
+// multiplied as they are, at eight instructions a word.
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -512,10 +512,13 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
 // workgroup split the columns, each holds its share of the rows in registers for all of the workgroup's outputs, and
 // only codes and scales are loaded in the loop, a round of outputs ahead.  The wavefronts' sums of a round meet in LDS.  Rows too
 // long for the registers take several visits, whose sums LDS keeps.
-// Bound by instructions: 16 x 8192 x 22528 bf16 36 us, 64 rows 74 us (of each SIMD's cycles 38 % are vector and 16 % matrix
-// instructions, which do not overlap in two wavefronts; the rest is the rounds' ends and loads of the rows); a round more of codes on
-// their way changes nothing (76 us).  The first form kept the rows in LDS, with a barrier for every 256 columns: each stretch waited for
-// its loads, 64 x 8192 x 22528 91 us, 7 x 5604 x 11263 fp16 37 us against 19.
+// 16 x 8192 x 22528 bf16 33 us, 64 rows 74 us.  Up to 16 rows are bound by the loads' way through few, large rounds (without the
+// products 32 us, without the loads 22), 64 rows by both (58 and 68 us; without the sums' way through LDS 61 us; of each SIMD's cycles
+// 38 % are vector and 16 % matrix instructions).  What changes nothing or costs: three rounds in flight in registers of their own
+// (74 to 78 us, products of 2048 columns twice the time), the offsets' sums by fp32 matrix instructions instead of from LDS (70 to 75),
+// workgroups that begin at different columns (73 to 75).  One barrier a round is worth 3 us of the 64 rows.  The first form kept the rows
+// in LDS, with a barrier for every 256 columns: each stretch waited for its loads, 64 x 8192 x 22528 91 us, 7 x 5604 x 11263 fp16 37 us
+// against 18.
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 template <typename XT> constexpr int kPlanes = sizeof(XT) == 4 ? 3 : 1;
@@ -582,6 +585,7 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
     constexpr int kPart = NT * MT * 256;                     // values of a round
     typedef typename Frag<XT>::type frag;
     typedef ST __attribute__((ext_vector_type(RUN * NG), aligned(sizeof(ST)))) run_scales;
+    // two buffers in turn need one barrier a round; what 64 KiB do not hold twice has one and two
     constexpr int kBuffers = kPart > 1024 ? 1 : 2;
     __shared__ __align__(16) float part_of[kBuffers][8 * kPart];
     int turn = 0;
