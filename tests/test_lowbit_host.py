@@ -146,3 +146,33 @@ def test_reference_packing_is_its_own_inverse():
     codes = torch.randint(-8, 8, (3, 64), dtype=torch.int8)
     assert torch.equal(ref.unpack(ref.pack(codes)), codes)
     assert int(ref.pack(torch.tensor([[1, -1]], dtype=torch.int8))[0, 0]) == 0xF1
+
+
+@pytest.mark.parametrize("frozen, thawed", [((0,), ()), ((2,), ()), ((), (3,)), ((0,), (3,))], ids=["first", "last", "one more", "another one"])
+def test_outer_weights_are_refused_for_a_changed_set_of_parameters(frozen, thawed):
+    from prime_amd.diloco import Diloco
+
+    model = torch.nn.Sequential(*(torch.nn.Linear(64, 64, bias=False) for _ in range(4)))
+    model[3].weight.requires_grad_(False)
+    state = Diloco(0.7, model)
+    for i in frozen:
+        model[i].weight.requires_grad_(False)
+    for i in thawed:
+        model[i].weight.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="model does not match"):
+        state.outer_weights_4bit(model)
+
+
+def test_outer_weights_come_under_their_own_names(monkeypatch):
+    from prime_amd.diloco import Diloco
+
+    monkeypatch.setattr(lowbit, "quantize_4bit", lambda w, group, dtype: (w.clone(), None))
+    model = torch.nn.Sequential(torch.nn.Linear(64, 64), torch.nn.LayerNorm(64), torch.nn.Linear(64, 64, bias=False))
+    state = Diloco(0.7, model)
+    want = {"0.weight": model[0].weight.detach().clone(), "2.weight": model[2].weight.detach().clone()}
+    for p in model.parameters():
+        p.data.add_(1.0)
+    for wrapped, prefix in ((model, ""), (torch.compile(model, backend="eager"), "_orig_mod.")):
+        got = state.outer_weights_4bit(wrapped)
+        assert got.keys() == {prefix + n for n in want}
+        assert all(torch.equal(got[prefix + n][0], w) for n, w in want.items())
