@@ -31,7 +31,8 @@ void with_weight_type(int weight_type, int type, F&& f) {
 
 constexpr int64_t kMaxDim = int64_t(1) << 30;
 
-constexpr int64_t kRowsPerLaunch = int64_t(1) << 21;    // a dispatch counts its work-items in 32 bits: 1024 a row at most
+// A dispatch counts its work-items in 32 bits: 1024 a row at most, and 32 a column of a sum over rows.
+constexpr int64_t kRowsPerLaunch = int64_t(1) << 21, kColumnsPerLaunch = int64_t(1) << 26;
 
 // Rows are read with the hint that leaves them out of the caches when a call moves more than the last-level cache holds anyway
 // (256 MiB): norm of 16384 x 4096 bf16 with residual (470 MB) 74 us with it and 82 without, its gradient (537 MB) 89 and 98; a quarter of those
@@ -94,7 +95,10 @@ void launch_rms_norm_grad(const NormGradArgs& a, int groups, WT* grad_weight, do
             launch(kIdRmsNormGrad, bytes, rms_norm_grad_apply_kernel<XT, WT>, stretches * groups, 256, st, a, dots, stretches, groups);
         }
     }
-    launch(kIdColumnSum, 4.0 * groups * a.dim, column_sum_kernel<WT>, static_cast<int>((a.dim + 31) / 32), 1024, st, a.partials, groups, a.dim, grad_weight);
+    for (int64_t at = 0; at < a.dim; at += kColumnsPerLaunch) {
+        const int64_t columns = std::min(a.dim - at, kColumnsPerLaunch);
+        launch(kIdColumnSum, 4.0 * groups * columns, column_sum_kernel<WT>, static_cast<int>((columns + 31) / 32), 1024, st, a.partials, groups, a.dim, at, grad_weight);
+    }
 }
 
 bool bad_group(int group) { return group != 32 && group != 64 && group != 128; }

@@ -640,11 +640,12 @@ __global__ __launch_bounds__(256) void rms_norm_grad_apply_kernel(NormGradArgs a
 }
 
 // dw[i] = the sum of the workgroups' shares: 32 columns a workgroup, each by 32 lanes whose sums are added in their order.
+// `first`: this launch's first column.
 template <typename WT>
-__global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restrict__ partials, int groups, int dim, WT* __restrict__ out) {
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float* __restrict__ partials, int groups, int dim, int64_t first, WT* __restrict__ out) {
     __shared__ double sh[32][33];
     const int c = threadIdx.x & 31, part = threadIdx.x >> 5;
-    const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + c;
+    const int64_t col = first + static_cast<int64_t>(blockIdx.x) * 32 + c;
     double s = 0.0;
     if (col < dim) {
         const float* p = partials + col;

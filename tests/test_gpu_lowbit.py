@@ -538,3 +538,22 @@ def test_calls_that_record_gradients_are_refused_on_the_gpu(dev):
     with pytest.raises(RuntimeError, match="no gradient"):
         torch.ops.prime_lowbit.rms_norm_quantize(x, w)
     assert torch.equal(torch.ops.prime_lowbit.rms_norm_quantize(x, w.detach())[0], lowbit.rms_norm_quantize(x, w.detach())[0])
+
+
+def test_norm_and_gradients_of_one_very_long_row(dev):
+    # 2^27 columns: 32 work-items a column for the sum over rows are one dispatch more than 32 bits count
+    dim = (1 << 27) + 41
+    announce("norm gradient 1 x 2^27 + 41")
+    g = torch.Generator(device=dev).manual_seed(7)
+    h, dy = (torch.randn(1, dim, device=dev, generator=g).to(BF16) for _ in range(2))
+    w = torch.rand(dim, device=dev, generator=g) + 0.5
+    inv = (h.double().square().mean(-1) + 1e-6).rsqrt().float()
+    gx, gw = lowbit.rms_norm_quantize_backward(dy, h, w, inv)
+    assert torch.equal(gw, (dy.float() * (h.float() * inv))[0])            # one row: two roundings, the same ones
+    wx, _, bx, _ = ref.norm_backward(dy, h, w, inv)
+    assert ref.outside(gx, wx, bx) <= 0
+    del wx, bx
+    codes, scales, got_inv = lowbit.rms_norm_quantize(h, w)
+    unit = (h.float() * w).abs().max() / 127
+    assert torch.equal(got_inv, inv) and abs(float(scales[0]) - float(unit.double() * inv.double())) <= 2.0 ** -23 * float(scales[0])
+    assert torch.equal(codes, torch.round((h.float() * w).double() / unit.double()).clamp(-127, 127).to(I8))
