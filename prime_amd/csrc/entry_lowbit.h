@@ -140,7 +140,7 @@ template <typename XT, typename ST, int GS, int MT, int B, int NT>
 void launch_matvec_many_as(MatvecArgs a, double bytes, hipStream_t st) {
     constexpr int kRows = 16 * MT, kPart = NT * MT * 256 * 4;
     a.sets = (a.n + 16 * NT - 1) / (16 * NT);
-    const int64_t row_tiles = (a.rows + kRows - 1) / kRows;
+    const int64_t row_tiles = (static_cast<int64_t>(a.rows) + kRows - 1) / kRows;
     const int visits = visits_of(a.k, B);
     // workgroups that stay for all their rounds, one a compute unit, all with as many (within one); with several visits LDS keeps the
     // sums of at most 48 KiB of rounds
@@ -171,7 +171,7 @@ void launch_matvec_many(const MatvecArgs& a, double bytes, hipStream_t st) {
     constexpr bool k32 = sizeof(XT) == 4, k8 = sizeof(XT) == 1, kWide = GS == 5 && sizeof(ST) == 4 && !k8;
     // more rows in tiles of 16 all the same where each tile finds a compute unit of its own: a wavefront's work is then a
     // quarter as long, and the codes that every tile reads come from the caches: 59 x 6720 x 76 bf16 34 us with 64 rows a workgroup
-    const bool small = (a.rows + 15) / 16 * ((static_cast<int64_t>(a.n) + 31) / 32) <= cu_count();
+    const bool small = (static_cast<int64_t>(a.rows) + 15) / 16 * ((static_cast<int64_t>(a.n) + 31) / 32) <= cu_count();
     if (a.rows <= 16 || small) {
         if constexpr (k32) launch_matvec_many_as<XT, ST, GS, 1, 2, 2>(a, bytes, st);
         else if (visits_of(a.k, 6) < visits_of(a.k, 4)) launch_matvec_many_as<XT, ST, GS, 1, 6, 1>(a, bytes, st);

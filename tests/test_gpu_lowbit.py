@@ -557,3 +557,17 @@ def test_norm_and_gradients_of_one_very_long_row(dev):
     unit = (h.float() * w).abs().max() / 127
     assert torch.equal(got_inv, inv) and abs(float(scales[0]) - float(unit.double() * inv.double())) <= 2.0 ** -23 * float(scales[0])
     assert torch.equal(codes, torch.round((h.float() * w).double() / unit.double()).clamp(-127, 127).to(I8))
+
+
+@pytest.mark.parametrize("xt", [F16, F32], ids=NAMES.get)
+def test_matvec_4bit_of_the_most_rows(dev, xt):
+    # 2^31 - 1 rows, the most a call takes: their number of tiles is rounded up in 64 bits
+    rows = (1 << 31) - 1
+    announce(f"matvec of 2^31 - 1 rows {xt}")
+    codes = torch.arange(-8, 8, dtype=torch.int8).repeat(2).view(1, 32)
+    x = torch.arange(1, 33).to(xt)
+    got = lowbit.matvec_4bit(x.to(dev).expand(rows, 32), ref.pack(codes).to(dev), torch.ones(1, 1, device=dev), None, F16)
+    want = float((x.double() * codes.double()).sum())          # every sum of the products is a whole number, and fp16 holds it
+    assert got.shape == (rows, 1) and want == 416
+    for part in got.view(-1).split(1 << 28):
+        assert bool((part == want).all())
