@@ -256,17 +256,39 @@ __device__ __forceinline__ void transpose_quarters(u32x4& w) {
     w = u32x4{c[0], c[1], d[0], d[1]};
 }
 
-// Eight codes of a word as 24 + q in 16 bits, in the order 0 4 1 5 2 6 3 7.
+// Eight codes of a word as 16-bit numbers with their sign, in the order 0 4 1 5 2 6 3 7: bf16 holds q / 16, fp16 q, both exactly.  (Beside an
+// offset, as 24 + q, a word takes eight instructions instead of thirteen and nine.  But then a column passes through the sums at up to 24 times
+// its size whatever its code is, and what a large one leaves there as rounding hides the others, and beyond 2^116 as infinity all of them.)
 template <bool BF16>
 __device__ __forceinline__ u32x4 widen_word(uint32_t w) {
     if constexpr (BF16) {
-        constexpr uint32_t kMask = 0x00780078u, kBase = 0x41c041c0u;      // 16.0 with the code's sign bit flipped in
-        return u32x4{((w << 3) & kMask) ^ kBase, ((w >> 1) & kMask) ^ kBase, ((w >> 5) & kMask) ^ kBase, ((w >> 9) & kMask) ^ kBase};
+        uint32_t odd = w >> 4;
+        asm("" : "+v"(odd));                                // keeps the one shift: its bytes are then operands as they are
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __builtin_amdgcn_cvt_off_f32_i4(w >> (8 * i) & 0xff);
+            f[2 * i + 1] = __builtin_amdgcn_cvt_off_f32_i4(odd >> (8 * i) & 0xff);
+        }
+        auto pair = [&](int e) { return __builtin_amdgcn_perm(__float_as_uint(f[e + 4]), __float_as_uint(f[e]), 0x07060302u); };
+        return u32x4{pair(0), pair(1), pair(2), pair(3)};
     } else {
-        constexpr uint32_t kMask = 0x03c003c0u, kBase = 0x4e004e00u;
-        return u32x4{((w << 6) & kMask) ^ kBase, ((w << 2) & kMask) ^ kBase, ((w >> 2) & kMask) ^ kBase, ((w >> 6) & kMask) ^ kBase};
+        typedef _Float16 __attribute__((ext_vector_type(2))) half2;
+        // 1024 + u or 1024 + 16 u with u = q + 8, then q
+        auto low = [](uint32_t v) {
+            const half2 h = __builtin_bit_cast(half2, (v & 0x000f000fu) ^ 0x64086408u) + half2{static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
+            return __builtin_bit_cast(uint32_t, h);
+        };
+        auto high = [](uint32_t v) {
+            const half2 by{static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)}, off{static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
+            return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2, (v & 0x00f000f0u) ^ 0x64806480u), by, off));
+        };
+        const uint32_t v = w >> 8;
+        return u32x4{low(w), high(w), low(v), high(v)};
     }
 }
+// What products with widened codes are to be multiplied by.
+template <typename XT> constexpr float kWidenedUnit = std::is_same<XT, _Float16>::value ? 1.0f : 16.0f;
 template <typename XT>
 __device__ __forceinline__ f32x4 product(u32x4 rows, u32x4 codes, f32x4 c) {
     if constexpr (std::is_same<XT, _Float16>::value)
@@ -589,7 +611,6 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
     constexpr int kBuffers = kPart > 1024 ? 1 : 2;
     __shared__ __align__(16) float part_of[kBuffers][8 * kPart];
     int turn = 0;
-    __shared__ __align__(16) float starts[kInt ? 1 : 8 * B * NG * MT * 16];      // [wavefront][block][group][tile][row]: -24 times the sum of its columns
     extern __shared__ __align__(16) float kept[];            // [own round][value], for rows that take several visits
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4, v16 = lane & 15;
     const int per_row_tile = gridDim.x / ((a.rows + kRows - 1) / kRows);
@@ -643,27 +664,6 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
                     for (int p = 0; p < P; ++p) xa[u][p][m][j] = f[p];
                 }
         });
-        if constexpr (!kInt) {
-            // what the offset of the codes adds to each group's sums, in the layout of the sums; a wavefront writes and reads its own
-            constexpr uint32_t kOff = std::is_same<XT, _Float16>::value ? 0xce00ce00u : 0xc1c0c1c0u;      // -24 twice
-            each<B>([&](auto uc) {
-                constexpr int u = decltype(uc)::value;
-                each<NG>([&](auto gc) {
-                    constexpr int g = decltype(gc)::value;
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        f32x4 acc{0, 0, 0, 0};
-                        each<4 / NG>([&](auto jc) {
-                            constexpr int j = g * (4 / NG) + decltype(jc)::value;
-#pragma unroll
-                            for (int p = 0; p < P; ++p) acc = product<XT>(xa[u][p][m][j], u32x4{kOff, kOff, kOff, kOff}, acc);
-                        });
-                        if (v16 == 0) *reinterpret_cast<f32x4*>(starts + (((wave * B + u) * NG + g) * MT + m) * 16 + quarter * 4) = acc;
-                    }
-                });
-            });
-            __builtin_amdgcn_wave_barrier();
-        }
         int own = 0;
         for (int set = set0; set < a.sets; set += per_row_tile, ++own) {
             const bool more = set + per_row_tile < a.sets;
@@ -715,7 +715,7 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
                         } else {
                             f32x4 acc[MT];
 #pragma unroll
-                            for (int m = 0; m < MT; ++m) acc[m] = *reinterpret_cast<const f32x4*>(starts + (((wave * B + u) * NG + g) * MT + m) * 16 + quarter * 4);
+                            for (int m = 0; m < MT; ++m) acc[m] = f32x4{0, 0, 0, 0};
                             each<kSteps>([&](auto jc) {
                                 constexpr int j = g * kSteps + decltype(jc)::value;
                                 const u32x4 cb = widen_word<!std::is_same<XT, _Float16>::value>(v[j]);
@@ -757,7 +757,7 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
                 const int64_t at = static_cast<int64_t>(row0 + row) * a.n + n;
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
-                    if (row + r < rows) store_product(a, at + static_cast<int64_t>(r) * a.n, kInt ? v[r] * (a.x_scales[row0 + row + r] * 0.0625f) : v[r]);
+                    if (row + r < rows) store_product(a, at + static_cast<int64_t>(r) * a.n, v[r] * (kInt ? a.x_scales[row0 + row + r] * 0.0625f : kWidenedUnit<XT>));
             }
             if constexpr (kBuffers == 1) __syncthreads();
 #pragma unroll

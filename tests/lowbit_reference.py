@@ -108,3 +108,15 @@ def outside(got, want, bound):
     # the rounded value is compared, so the step is taken where the bound could carry it; 2^-150: fp32's smallest half step
     small = {torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}[got.dtype]
     return float((d - (STEP[got.dtype] * (want.abs() + bound) + bound + small)).max()) if d.numel() else 0.0
+
+
+def matvec_bound(x, codes, scales, k):
+    """Bound of the error of products of floating rows, from the roundings that 32-bit sums of the terms themselves make: relative to
+    sum |code x scale|, so that a column whose code is 0 counts for nothing.  Products with a code are exact (fp32 rows as three
+    parts, so three products).  Within a group each addition is off by at most a whole step (twice half of one, should the matrix
+    unit cut off what it does not hold); a group's scaling and each addition of groups, wavefronts and visits by half a step."""
+    group = codes.shape[1] // scales.shape[1]
+    parts = 3 if x.dtype == torch.float32 else 1
+    terms = x.reshape(-1, k).to(F64).abs() @ (codes[:, :k].to(F64) * scales.to(F64).repeat_interleave(group, 1)[:, :k]).abs().T
+    bound = 2.0 ** -24 * (2 * parts * group + scales.shape[1] + 24) * terms
+    return bound.view(*x.shape[:-1], codes.shape[0])

@@ -571,3 +571,107 @@ def test_matvec_4bit_of_the_most_rows(dev, xt):
     assert got.shape == (rows, 1) and want == 416
     for part in got.view(-1).split(1 << 28):
         assert bool((part == want).all())
+
+
+# ---- floating rows: more of them than are taken as a decoding step's few (5 and up), then few ----
+
+FLOATS = [BF16, F16, F32]
+
+
+def check_matvec_closely(dev, x, codes, s, k):
+    got = lowbit.matvec_4bit(x.to(dev), ref.pack(codes).to(dev), s.to(dev), None, F32)
+    want, _ = ref.matvec(x, None, codes, s, k)
+    assert torch.isfinite(got).all() and ref.outside(got.cpu(), want, ref.matvec_bound(x, codes, s, k)) <= 0
+    return got.cpu()
+
+
+def check_large_columns_under_zero_codes(dev, rows, xt):
+    # what a large column leaves where its code is 0 is nothing: neither its rounding nor its range shows in the other columns' sum
+    for n, k, group in ((40, 128, 128), (33, 700, 32), (70, 2100, 64)):
+        for far in (13, 20, 60) if xt != F16 else (13, 15):
+            g = gen("large columns", rows, str(xt), k, group, far)
+            announce(f"matvec {rows} x {k} x {n} group {group} {xt}: columns of 2^{far} under zeros")
+            codes, s = four_bit(g, n, k, group, F32)
+            x = torch.randn(rows, k, generator=g)
+            large = torch.randperm(k, generator=g)[: max(1, k // 50)]
+            x[:, large] = 2.0 ** far * (0.5 + torch.rand(rows, len(large), generator=g))
+            codes[:, large] = 0
+            codes[5] = 0                                                    # an output of zeros stays one
+            got = check_matvec_closely(dev, x.to(xt), codes, s, k)
+            assert not got[:, 5].any()
+    # one column of 1e10 (1e4) under a zero, 127 ones under ones
+    codes, s = torch.ones(3, 128, dtype=torch.int8), torch.ones(3, 1)
+    codes[:, 0] = 0
+    x = torch.ones(rows, 128)
+    x[:, 0] = 1e10 if xt != F16 else 6e4
+    assert bool((lowbit.matvec_4bit(x.to(xt).to(dev), ref.pack(codes).to(dev), s.to(dev), None, F32) == 127).all())
+
+
+def check_the_range_of_columns(dev, rows, xt):
+    # up to 2^120 in magnitude a finite product is finite, whatever the scale takes off afterwards; small columns keep their bits
+    for group in (32, 64, 128):
+        codes = torch.full((20, 256), 7, dtype=torch.int8)
+        codes[1::2] = -8
+        for top, scale in ((116.0, 0.5), (120.0, 2.0 ** -20), (15.0, 1.0), (-100.0, 2.0 ** 60), (-108.0, 2.0 ** 80)):
+            if xt == F16 and top != 15.0:
+                continue
+            announce(f"matvec {rows} x 256 x 20 group {group} {xt}: columns of 2^{top}")
+            s = torch.full((20, 256 // group), scale)
+            x = torch.full((rows, 256), 2.0 ** top)
+            want = x.double() @ (codes.double() * scale).T
+            got = lowbit.matvec_4bit(x.to(xt).to(dev), ref.pack(codes).to(dev), s.to(dev), None, F32)
+            assert torch.equal(got.cpu().double(), want)                    # equal columns: every sum has few bits
+            x = torch.randn(rows, 256, generator=gen("range", rows, str(xt), group)).clamp(-3, 3) * 2.0 ** (top - 2)
+            mixed, _ = four_bit(gen("range codes", group), 20, 256, group, F32)
+            check_matvec_closely(dev, x.to(xt), mixed, s, 256)
+
+
+def check_whole_numbers(dev, rows, xt, sizes):
+    # sixteenths up to 8 and scales of 1/2, 1 and 2: every sum, in every order, is a multiple of 2^-5 below 2^19, so nothing is rounded, and
+    # a column that is lost, doubled or met with another's code shows
+    for n, k, group in sizes:
+        g = gen("whole", rows, str(xt), n, k, group)
+        announce(f"matvec {rows} x {k} x {n} group {group} {xt}: whole numbers")
+        codes, _ = four_bit(g, n, k, group, F32)
+        s = 2.0 ** torch.randint(-1, 2, (n, codes.shape[1] // group), generator=g).float()
+        x = torch.randint(-127, 128, (rows, k), generator=g) / 16
+        weights = codes[:, :k].double() * s.double().repeat_interleave(group, 1)[:, :k]
+        assert float((x.double().abs() @ weights.abs().T).max()) < 2 ** 19
+        got = lowbit.matvec_4bit(x.to(xt).to(dev), ref.pack(codes).to(dev), s.to(dev), None, F32)
+        assert torch.equal(got.cpu().double(), x.double() @ weights.T)
+
+
+def check_single_columns(dev, rows, xt):
+    # one column that is not 0 a row, of as many bits as its type has.  16-bit columns: the product has at most 11 + 3 bits and is exact.  fp32: its
+    # three parts of 8 bits give products of 11; the first two add up to 19 bits, exactly, and the third addition alone is inexact.  The
+    # matrix unit is free to cut off what it does not hold, so that addition is off by less than a whole step of the sum, 2^-23 of it
+    # (half a step if it rounds); the factors behind it are powers of two
+    for group in (32, 64, 128):
+        g = gen("single", rows, str(xt), group)
+        codes, _ = four_bit(g, 50, 600, group, F32)
+        s = 2.0 ** torch.randint(-1, 2, (50, codes.shape[1] // group), generator=g).float()
+        x = torch.zeros(rows, 600, dtype=xt)
+        for m in range(rows):
+            x[m, int(torch.randint(0, 600, (1,), generator=g))] = torch.randn(1, generator=g).to(xt)[0]
+        got = lowbit.matvec_4bit(x.to(dev), ref.pack(codes).to(dev), s.to(dev), None, F32)
+        want, _ = ref.matvec(x, None, codes, s, 600)
+        assert bool(((got.cpu().double() - want).abs() <= (2.0 ** -23 * want.abs() if xt == F32 else 0.0)).all())
+
+
+@pytest.mark.parametrize("rows", [5, 16, 20, 40, 64])
+@pytest.mark.parametrize("xt", FLOATS, ids=NAMES.get)
+def test_matvec_4bit_many_rows_with_large_columns_under_zero_codes(dev, rows, xt):
+    check_large_columns_under_zero_codes(dev, rows, xt)
+
+
+@pytest.mark.parametrize("rows", [5, 40, 64])
+@pytest.mark.parametrize("xt", FLOATS, ids=NAMES.get)
+def test_matvec_4bit_many_rows_range_of_columns(dev, rows, xt):
+    check_the_range_of_columns(dev, rows, xt)
+
+
+@pytest.mark.parametrize("rows", [5, 16, 30, 64])
+@pytest.mark.parametrize("xt", FLOATS, ids=NAMES.get)
+def test_matvec_4bit_many_rows_of_whole_numbers(dev, rows, xt):
+    check_whole_numbers(dev, rows, xt, ((48, 20000, 32), (48, 20000, 128), (600, 6000, 64), (4200, 2100, 128)))
+    check_single_columns(dev, rows, xt)
