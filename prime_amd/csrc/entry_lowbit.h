@@ -109,7 +109,7 @@ int group_shift(int group) { return group == 32 ? 5 : group == 64 ? 6 : 7; }
 template <typename XT, typename ST, int GS>
 void launch_matvec_few(MatvecArgs a, double bytes, hipStream_t st) {
     constexpr int kMostLds = 56 << 10;
-    const int held = a.rows, quads = (a.k + 511) / 512, quad_bytes = 4 * kFewBlock<XT> + 16;
+    const int held = a.rows, quads = (a.k + 511) / 512, quad_bytes = 4 * kFewBlock<XT>;
     a.tiles = (a.n + 15) / 16;
     // wavefronts that share a tile's columns: enough for 16 wavefronts a compute unit, but not more than it has stretches
     const int wanted = cu_count() * 16;

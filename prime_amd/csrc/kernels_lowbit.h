@@ -316,46 +316,18 @@ __device__ __forceinline__ void store_product(const MatvecArgs& a, int64_t at, f
     else static_cast<_Float16*>(a.out)[at] = static_cast<_Float16>(v);
 }
 
-// ---- up to four rows: whole numbers up to the end of a group ----
-// int8 rows are taken as they are.  Floating rows become fixed point under the largest magnitude of each 128 columns: 31 bits, as
-// four digits of -128 .. 127 in base 256, so a value is off by at most 2^-31 of that largest (a 32-bit sum that holds both loses
-// more).  The four digits of a row are four rows of the A operand, so one matrix instruction takes them all; a group's sums are
-// exact in each digit, two digits are put together exactly in 32 bits, and the rest is fp32.
-//
-// Bound by memory from a few thousand outputs up: 1 x 8192 x 128000 int8 92 us (5.9 TB/s; with the products taken out and the loads left
-// in 97, with loads that cover whole lines instead of 64 bytes of 16 rows 90), bf16 104 us (5.2 TB/s); the same with the codes widened to
-// bf16, at eight instructions a word beside an offset's second product, 121.  Small products are a launch and two trips
-// to memory: 1 x 2048 x 2048 4.1 us, 1 x 4096 x 4096 5.0 us.
+template <typename XT> constexpr int kPlanes = sizeof(XT) == 4 ? 3 : 1;
 
-// Digits in base 256 that a value is taken to.
-template <typename XT> constexpr int kDigits = sizeof(XT) == 1 ? 1 : 4;
-// Bytes of a row's 128 columns in LDS: [quarter][half][digit][16 columns], so that the lanes of a quarter, which read the digits of
-// one row side by side, read 64 consecutive bytes.  Rows lie 64 bytes off the banks' period (int8: 16).
-template <typename XT> constexpr int kFewBlock = 128 * kDigits<XT>;
-template <typename XT> constexpr int kFewPad = 16 * kDigits<XT>;
+__device__ __forceinline__ uint32_t pair16(uint32_t lo, uint32_t hi) { return (lo & 0xffffu) | hi << 16; }
 
-// Largest of the 16 lanes of a row of 16, in all of them.
-__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
-    v = max(v, row_turned<8>(v));
-    v = max(v, row_turned<4>(v));
-    v = max(v, row_turned<2>(v));
-    return max(v, row_turned<1>(v));
-}
+// Eight columns of a row as the A operand wants them: 16-bit values in the order 0 4 1 5 2 6 3 7 (fp32 in three bf16 planes, each the
+// leading eight bits of what the ones before leave: together the value, but for what lies below bf16's smallest step, 2^-133), bytes in
+// the order 0 2 4 6 1 3 5 7.
+template <typename XT> struct Frag { typedef u32x4 type; };
+template <> struct Frag<int8_t> { typedef u32x2 type; };
 
-// Bytes of four words by their place: out[d] holds byte 3 - d of a, b, c and e, lowest first.
-__device__ __forceinline__ void transpose_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t e, uint32_t (&out)[4]) {
-    const uint32_t ab_lo = __builtin_amdgcn_perm(b, a, 0x05010400u), ab_hi = __builtin_amdgcn_perm(b, a, 0x07030602u);     // a0 b0 a1 b1, a2 b2 a3 b3
-    const uint32_t ce_lo = __builtin_amdgcn_perm(e, c, 0x05010400u), ce_hi = __builtin_amdgcn_perm(e, c, 0x07030602u);
-    out[3] = __builtin_amdgcn_perm(ce_lo, ab_lo, 0x05040100u);
-    out[2] = __builtin_amdgcn_perm(ce_lo, ab_lo, 0x07060302u);
-    out[1] = __builtin_amdgcn_perm(ce_hi, ab_hi, 0x05040100u);
-    out[0] = __builtin_amdgcn_perm(ce_hi, ab_hi, 0x07060302u);
-}
-
-// Eight columns c * 8 .. of a row as digits, most significant first, bytes in the order 0 2 4 6 1 3 5 7; the 16 lanes of 128
-// columns call it together.  Returns the unit of the last digit (NaN, and zeros, if a column is not finite).
 template <typename XT>
-__device__ __forceinline__ float digits8(const XT* __restrict__ row, int64_t i, int n, u32x2 (&out)[kDigits<XT>]) {
+__device__ __forceinline__ void rows8(const XT* __restrict__ row, int64_t i, int n, typename Frag<XT>::type (&out)[kPlanes<XT>]) {
     if constexpr (sizeof(XT) == 1) {
         uint32_t lo = 0, hi = 0;
         if (i + 8 <= n) {
@@ -368,44 +340,61 @@ __device__ __forceinline__ float digits8(const XT* __restrict__ row, int64_t i, 
                 if (i + e < n) (e < 4 ? lo : hi) |= static_cast<uint32_t>(static_cast<uint8_t>(row[i + e])) << (8 * (e & 3));
         }
         out[0] = u32x2{__builtin_amdgcn_perm(hi, lo, 0x06040200u), __builtin_amdgcn_perm(hi, lo, 0x07050301u)};
-        return 1.0f;
-    } else {
-        float x[8];
+    } else if constexpr (sizeof(XT) == 2) {
+        typename Eight<XT>::type t;
         if (i < n) {
-            load8(row, static_cast<int>(i), n, x);
+            t = take8(row, static_cast<int>(i), n);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+            for (int e = 0; e < 8; ++e) t[e] = static_cast<XT>(0.0f);
         }
-        uint32_t top = 0;
+        typedef XT __attribute__((ext_vector_type(8))) eight;
+        const u32x4 b = __builtin_bit_cast(u32x4, static_cast<eight>(t));
+        // 0 4, 1 5, 2 6, 3 7
+        out[0] = u32x4{__builtin_amdgcn_perm(b[2], b[0], 0x05040100u), __builtin_amdgcn_perm(b[2], b[0], 0x07060302u),
+                       __builtin_amdgcn_perm(b[3], b[1], 0x05040100u), __builtin_amdgcn_perm(b[3], b[1], 0x07060302u)};
+    } else {
+        float v[8];
+        if (i < n) {
+            load8(row, static_cast<int>(i), n, v);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-        top = row16_max(top);
-        // all magnitudes lie below 2^e; the last digit counts in units of 2^(e - 30).  (e stays above -95, so that the unit is a normal
-        // number: what such a row loses is below 2^-126.)
-        const int e2 = max(static_cast<int>(top >> 23) - 126, -95);
-        const bool fine = top < 0x7f800000u;
-        const float up = fine ? __builtin_ldexpf(1.0f, 30 - e2) : 0.0f;      // NaN and infinity times zero convert to zero
-        uint32_t v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            // half of 256 added at each digit but the first carries into the next where the byte is to count as negative
-            v[e] = (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(x[e] * up))) + 0x00808080u) ^ 0x00808080u;
+            for (int e = 0; e < 8; ++e) v[e] = 0.0f;
         }
-        uint32_t even[4], odd[4];
-        transpose_bytes(v[0], v[2], v[4], v[6], even);
-        transpose_bytes(v[1], v[3], v[5], v[7], odd);
 #pragma unroll
-        for (int d = 0; d < 4; ++d) out[d] = u32x2{even[d], odd[d]};
-        return fine ? __builtin_ldexpf(1.0f, e2 - 30) : __builtin_nanf("");
+        for (int p = 0; p < 3; ++p) {
+            uint32_t b[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                b[e] = __float_as_uint(v[e]) >> 16;
+                v[e] -= __uint_as_float(b[e] << 16);      // exact: the bits that are left
+            }
+            out[p] = u32x4{pair16(b[0], b[4]), pair16(b[1], b[5]), pair16(b[2], b[6]), pair16(b[3], b[7])};
+        }
     }
 }
+
+// ---- up to four rows: whole numbers up to the end of a group ----
+// int8 rows are taken as they are.  Floating rows become fixed point under the largest magnitude of each 128 columns: 31 bits, as
+// four digits of -128 .. 127 in base 256, so a value is off by at most 2^-31 of that largest (a 32-bit sum that holds both loses
+// more).  The four digits of a row are four rows of the A operand, so one matrix instruction takes them all; a group's sums are
+// exact in each digit, two digits are put together exactly in 32 bits, and the rest is fp32.
+//
+// Bound by memory from a few thousand outputs up: 1 x 8192 x 128000 int8 92 us (5.9 TB/s; with the products taken out and the loads left
+// in 97, with loads that cover whole lines instead of 64 bytes of 16 rows 90), bf16 104 us (5.2 TB/s); the same with the codes widened to
+// bf16, at eight instructions a word beside an offset's second product, 121.  Small products are a launch and two trips
+// to memory: 1 x 2048 x 2048 4.1 us, 1 x 4096 x 4096 5.0 us.
+
+// Bytes of a row's 128 columns in LDS: [quarter][word of a lane][plane][eight columns], so that the lanes of a quarter, which read the planes
+// of one word side by side, read consecutive bytes.  Rows lie 16 (fp32: 64) bytes off the banks' period.
+template <typename XT> constexpr int kFewBlock = 128 * static_cast<int>(sizeof(typename Frag<XT>::type)) / 8 * kPlanes<XT>;
+template <typename XT> constexpr int kFewPad = sizeof(XT) == 4 ? 64 : 16;
 
 template <typename XT, typename ST, int GS>
 __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
     constexpr bool kInt = sizeof(XT) == 1;
     constexpr int NG = 1 << (7 - GS);
-    constexpr int kBlock = kFewBlock<XT>, D = kDigits<XT>;
+    constexpr int kBlock = kFewBlock<XT>, P = kPlanes<XT>, kWord = static_cast<int>(sizeof(typename Frag<XT>::type)) * P;
     extern __shared__ __align__(16) uint8_t few_lds[];
     __shared__ float part[2][8 * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4, v16 = lane & 15;
@@ -414,12 +403,10 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
     const int stride = gridDim.x, set0 = blockIdx.x, rows = a.rows;
     const int quads = (a.k + 511) >> 9;
     const int row_stride = a.chunk_quads * 4 * kBlock + kFewPad<XT>;
-    float* units = reinterpret_cast<float*>(few_lds + rows * row_stride);                    // [row][block of 128 columns]
-    // a lane's row of the A operand: digit v16 & 3 of row v16 >> 2 (int8: the row, four times).  Rows that do not exist repeat the
-    // last one; their sums are dropped
+    // a lane's row of the A operand: plane v16 & 3 of row v16 >> 2 (one plane: the row, four times).  Rows and planes that do not exist repeat
+    // the last one; their sums are dropped
     const int my_row = min(v16 >> 2, rows - 1);
-    const uint8_t* mine = few_lds + my_row * row_stride + (kInt ? quarter * 32 : quarter * 128 + (v16 & 3) * 16);
-    const float* unit = units + min(quarter, rows - 1) * (a.chunk_quads * 4);
+    const uint8_t* mine = few_lds + my_row * row_stride + quarter * (4 * kWord) + (P > 1 ? min(v16 & 3, P - 1) * 16 : 0);
     const uint8_t* scales = static_cast<const uint8_t*>(a.scales);
     u32x4 w[4], w2[4];
     QuadScales<ST, GS> s, s2;
@@ -457,14 +444,13 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
                 // rows of x to LDS: eight columns a lane, put where the lane that multiplies them will look
                 for (int i = threadIdx.x; i < rows * held * 64; i += blockDim.x) {
                     const int m = i / (held * 64), c = i - m * (held * 64);
-                    u32x2 v[D];
-                    const float last = digits8(x + m * a.x_stride, static_cast<int64_t>(first) * 512 + c * 8, a.k, v);
+                    typename Frag<XT>::type v[P];
+                    rows8(x + m * a.x_stride, static_cast<int64_t>(first) * 512 + c * 8, a.k, v);
                     // eighth `in` of a block: with groups of 128 a quarter's four lie side by side, else they are a quarter apart
                     const int in = c & 15, q = GS == 7 ? in >> 2 : in & 3, j = GS == 7 ? in & 3 : in >> 2;
-                    uint8_t* to = few_lds + m * row_stride + (c >> 4) * kBlock + q * 32 * D + (j >> 1) * 16 * D + (j & 1) * 8;
+                    uint8_t* to = few_lds + m * row_stride + (c >> 4) * kBlock + (q * 4 + j) * kWord;
 #pragma unroll
-                    for (int d = 0; d < D; ++d) *reinterpret_cast<u32x2*>(to + 16 * d) = v[d];
-                    if (!kInt && in == 0) units[m * (a.chunk_quads * 4) + (c >> 4)] = last;
+                    for (int p = 0; p < P; ++p) reinterpret_cast<typename Frag<XT>::type*>(to)[p] = v[p];
                 }
                 __syncthreads();
             }
@@ -478,35 +464,36 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
                 for (int u = 0; u < 4; ++u) {
                     u32x4 c = w[u];
                     if constexpr (GS < 7) transpose_quarters(c);
-                    i32x4 acc[NG];
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) acc[g] = i32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + (q * 4 + u) * kBlock + j * 16 * D);
-                        const u32x4 b{(c[2 * j] << 4) & 0xf0f0f0f0u, c[2 * j] & 0xf0f0f0f0u, (c[2 * j + 1] << 4) & 0xf0f0f0f0u, c[2 * j + 1] & 0xf0f0f0f0u};
-                        if constexpr (GS == 5) {
-                            const u32x2 a0{xa[0], xa[1]}, a1{xa[2], xa[3]}, b0{b[0], b[1]}, b1{b[2], b[3]};
-                            acc[2 * j] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a0), __builtin_bit_cast(long, b0), acc[2 * j], 0, 0, 0);
-                            acc[2 * j + 1] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a1), __builtin_bit_cast(long, b1), acc[2 * j + 1], 0, 0, 0);
-                        } else {
-                            const int g = GS == 6 ? j : 0;
-                            acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, xa), __builtin_bit_cast(i32x4, b), acc[g], 0, 0, 0);
-                        }
-                    }
                     if constexpr (kInt) {
+                        i32x4 acc[NG];
 #pragma unroll
-                        for (int g = 0; g < NG; ++g)
-                            y = fmaf(static_cast<float>(acc[g][0]), s.at(u * NG + g), y);
-                    } else {
-                        // a digit's sum stays below 2^21: two digits go together in 32 bits, exactly
-                        float t = 0.0f;
+                        for (int g = 0; g < NG; ++g) acc[g] = i32x4{0, 0, 0, 0};
 #pragma unroll
-                        for (int g = 0; g < NG; ++g) {
-                            const float hi = static_cast<float>(acc[g][0] * 256 + acc[g][1]), lo = static_cast<float>(acc[g][2] * 256 + acc[g][3]);
-                            t = fmaf(fmaf(hi, 65536.0f, lo), s.at(u * NG + g), t);
+                        for (int j = 0; j < 2; ++j) {
+                            const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + (q * 4 + u) * kBlock + j * 16);
+                            const u32x4 b{(c[2 * j] << 4) & 0xf0f0f0f0u, c[2 * j] & 0xf0f0f0f0u, (c[2 * j + 1] << 4) & 0xf0f0f0f0u, c[2 * j + 1] & 0xf0f0f0f0u};
+                            if constexpr (GS == 5) {
+                                const u32x2 a0{xa[0], xa[1]}, a1{xa[2], xa[3]}, b0{b[0], b[1]}, b1{b[2], b[3]};
+                                acc[2 * j] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a0), __builtin_bit_cast(long, b0), acc[2 * j], 0, 0, 0);
+                                acc[2 * j + 1] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a1), __builtin_bit_cast(long, b1), acc[2 * j + 1], 0, 0, 0);
+                            } else {
+                                const int g = GS == 6 ? j : 0;
+                                acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, xa), __builtin_bit_cast(i32x4, b), acc[g], 0, 0, 0);
+                            }
                         }
-                        y = fmaf(t, unit[q * 4 + u], y);
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) y = fmaf(static_cast<float>(acc[g][0]), s.at(u * NG + g), y);
+                    } else {
+                        f32x4 acc[NG];
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) acc[g] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + (q * 4 + u) * kBlock + j * kWord);
+                            acc[j * NG / 4] = product<XT>(xa, widen_word<!std::is_same<XT, _Float16>::value>(c[j]), acc[j * NG / 4]);
+                        }
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) y = fmaf(P > 1 ? (acc[g][2] + acc[g][1]) + acc[g][0] : acc[g][0], s.at(u * NG + g), y);
                     }
                 }
 #pragma unroll
@@ -522,8 +509,8 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
             if (kpart) continue;
             for (int p = 1; p < split; ++p) y += part[turn][(wave + p) * 64 + lane];
         }
-        // codes were multiplied as 16 q
-        if (quarter < rows && n < a.n) store_product(a, static_cast<int64_t>(quarter) * a.n + n, kInt ? y * (a.x_scales[quarter] * 0.0625f) : y * 0.0625f);
+        // codes in a byte's upper half were multiplied as 16 q
+        if (quarter < rows && n < a.n) store_product(a, static_cast<int64_t>(quarter) * a.n + n, y * (kInt ? a.x_scales[quarter] * 0.0625f : kWidenedUnit<XT>));
     }
 }
 
@@ -543,55 +530,6 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
 // against 18.
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-template <typename XT> constexpr int kPlanes = sizeof(XT) == 4 ? 3 : 1;
-
-__device__ __forceinline__ uint32_t pair16(uint32_t lo, uint32_t hi) { return (lo & 0xffffu) | hi << 16; }
-
-// Eight columns of a row as the A operand wants them: 16-bit values in the order 0 4 1 5 2 6 3 7 (fp32 in three planes, each the
-// leading bits of what the ones before leave), bytes in the order 0 2 4 6 1 3 5 7.
-template <typename XT> struct Frag { typedef u32x4 type; };
-template <> struct Frag<int8_t> { typedef u32x2 type; };
-
-template <typename XT>
-__device__ __forceinline__ void rows8(const XT* __restrict__ row, int64_t i, int n, typename Frag<XT>::type (&out)[kPlanes<XT>]) {
-    if constexpr (sizeof(XT) == 1) {
-        u32x2 v[1];
-        digits8<int8_t>(row, i, n, v);
-        out[0] = v[0];
-    } else if constexpr (sizeof(XT) == 2) {
-        typename Eight<XT>::type t;
-        if (i < n) {
-            t = take8(row, static_cast<int>(i), n);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) t[e] = static_cast<XT>(0.0f);
-        }
-        typedef XT __attribute__((ext_vector_type(8))) eight;
-        const u32x4 b = __builtin_bit_cast(u32x4, static_cast<eight>(t));
-        // 0 4, 1 5, 2 6, 3 7
-        out[0] = u32x4{__builtin_amdgcn_perm(b[2], b[0], 0x05040100u), __builtin_amdgcn_perm(b[2], b[0], 0x07060302u),
-                       __builtin_amdgcn_perm(b[3], b[1], 0x05040100u), __builtin_amdgcn_perm(b[3], b[1], 0x07060302u)};
-    } else {
-        float v[8];
-        if (i < n) {
-            load8(row, static_cast<int>(i), n, v);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-        }
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-            uint32_t b[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                b[e] = __float_as_uint(v[e]) >> 16;
-                v[e] -= __uint_as_float(b[e] << 16);      // exact: the bits that are left
-            }
-            out[p] = u32x4{pair16(b[0], b[4]), pair16(b[1], b[5]), pair16(b[2], b[6]), pair16(b[3], b[7])};
-        }
-    }
-}
-
 // f(0), f(1), ... with the index a constant: registers are indexed by it.
 template <int N, typename F, int... I>
 __device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }

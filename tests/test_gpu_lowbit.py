@@ -642,7 +642,7 @@ def check_whole_numbers(dev, rows, xt, sizes):
 
 
 def check_single_columns(dev, rows, xt):
-    # one column that is not 0 a row, of as many bits as its type has.  16-bit columns: the product has at most 11 + 3 bits and is exact.  fp32: its
+    # one column that is not 0 in a row, of as many bits as its type has.  16-bit columns: the product has at most 11 + 3 bits and is exact.  fp32: its
     # three parts of 8 bits give products of 11; the first two add up to 19 bits, exactly, and the third addition alone is inexact.  The
     # matrix unit is free to cut off what it does not hold, so that addition is off by less than a whole step of the sum, 2^-23 of it
     # (half a step if it rounds); the factors behind it are powers of two
@@ -675,3 +675,40 @@ def test_matvec_4bit_many_rows_range_of_columns(dev, rows, xt):
 def test_matvec_4bit_many_rows_of_whole_numbers(dev, rows, xt):
     check_whole_numbers(dev, rows, xt, ((48, 20000, 32), (48, 20000, 128), (600, 6000, 64), (4200, 2100, 128)))
     check_single_columns(dev, rows, xt)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4])
+@pytest.mark.parametrize("xt", FLOATS, ids=NAMES.get)
+def test_matvec_4bit_few_rows_with_large_columns_under_zero_codes(dev, rows, xt):
+    check_large_columns_under_zero_codes(dev, rows, xt)
+
+
+@pytest.mark.parametrize("rows", [1, 4])
+@pytest.mark.parametrize("xt", FLOATS, ids=NAMES.get)
+def test_matvec_4bit_few_rows_range_of_columns(dev, rows, xt):
+    check_the_range_of_columns(dev, rows, xt)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4])
+@pytest.mark.parametrize("xt", FLOATS, ids=NAMES.get)
+def test_matvec_4bit_few_rows_of_whole_numbers(dev, rows, xt):
+    # rows that LDS holds whole and rows that it takes in stretches, columns shared by one to eight wavefronts, one tile a workgroup and several
+    check_whole_numbers(dev, rows, xt, ((48, 20000, 32), (48, 20000, 128), (600, 6000, 64), (9000, 2100, 128), (70001, 130, 64)))
+    check_single_columns(dev, rows, xt)
+    # longer than LDS holds of one 16-bit row
+    g = gen("longest", rows, str(xt))
+    codes, s = four_bit(g, 40, 30000, 128, F32)
+    check_matvec_closely(dev, rows_like_activations(g, rows, 30000, xt), codes, s, 30000)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 5, 20])
+def test_matvec_4bit_columns_of_the_smallest_magnitudes(dev, rows):
+    # columns that are subnormal in their type, under a scale that brings the products back; fp32 columns down to bf16's smallest step
+    announce(f"matvec {rows} rows of the smallest magnitudes")
+    g = gen("smallest", rows)
+    codes, _ = four_bit(g, 20, 128, 64, F32)
+    for xt, top, scale in ((F16, -24, 1024.0), (BF16, -133, 2.0 ** 100), (F32, -133, 2.0 ** 100)):
+        x = torch.randint(-3, 4, (rows, 128), generator=g).double() * 2.0 ** top
+        s = torch.full((20, 2), scale)
+        got = lowbit.matvec_4bit(x.to(xt).to(dev), ref.pack(codes).to(dev), s.to(dev), None, F32)
+        assert torch.equal(got.cpu().double(), x @ (codes.double() * scale).T)
