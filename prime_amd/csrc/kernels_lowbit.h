@@ -287,6 +287,17 @@ __device__ __forceinline__ u32x4 widen_word(uint32_t w) {
         return u32x4{low(w), high(w), low(v), high(v)};
     }
 }
+// The codes in the lower or upper halves of a word's bytes as bytes with their sign: 16 q in an instruction or two, or q in two more.
+template <bool SIXTEEN>
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) {
+    if constexpr (SIXTEEN) return (w << 4) & 0xf0f0f0f0u;
+    else return (((w & 0x0f0f0f0fu) ^ 0x08080808u) + 0x78787878u) ^ 0x80808080u;      // q + 8, q + 128: no byte carries
+}
+template <bool SIXTEEN>
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) {
+    if constexpr (SIXTEEN) return w & 0xf0f0f0f0u;
+    else return low_codes<false>(w >> 4);
+}
 // What products with widened codes are to be multiplied by.
 template <typename XT> constexpr float kWidenedUnit = std::is_same<XT, _Float16>::value ? 1.0f : 16.0f;
 template <typename XT>
@@ -465,13 +476,15 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
                     u32x4 c = w[u];
                     if constexpr (GS < 7) transpose_quarters(c);
                     if constexpr (kInt) {
+                        // the codes count 16 times, which is taken off a group's sum, exactly, before it meets the scales: at the
+                        // end, sums could leave fp32 that the rows' scales bring back, and the rows' smallest scales would lose bits
                         i32x4 acc[NG];
 #pragma unroll
                         for (int g = 0; g < NG; ++g) acc[g] = i32x4{0, 0, 0, 0};
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             const u32x4 xa = *reinterpret_cast<const u32x4*>(mine + (q * 4 + u) * kBlock + j * 16);
-                            const u32x4 b{(c[2 * j] << 4) & 0xf0f0f0f0u, c[2 * j] & 0xf0f0f0f0u, (c[2 * j + 1] << 4) & 0xf0f0f0f0u, c[2 * j + 1] & 0xf0f0f0f0u};
+                            const u32x4 b{low_codes<true>(c[2 * j]), high_codes<true>(c[2 * j]), low_codes<true>(c[2 * j + 1]), high_codes<true>(c[2 * j + 1])};
                             if constexpr (GS == 5) {
                                 const u32x2 a0{xa[0], xa[1]}, a1{xa[2], xa[3]}, b0{b[0], b[1]}, b1{b[2], b[3]};
                                 acc[2 * j] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, a0), __builtin_bit_cast(long, b0), acc[2 * j], 0, 0, 0);
@@ -482,7 +495,7 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
                             }
                         }
 #pragma unroll
-                        for (int g = 0; g < NG; ++g) y = fmaf(static_cast<float>(acc[g][0]), s.at(u * NG + g), y);
+                        for (int g = 0; g < NG; ++g) y = fmaf(static_cast<float>(acc[g][0]) * 0.0625f, s.at(u * NG + g), y);
                     } else {
                         f32x4 acc[NG];
 #pragma unroll
@@ -509,8 +522,7 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
             if (kpart) continue;
             for (int p = 1; p < split; ++p) y += part[turn][(wave + p) * 64 + lane];
         }
-        // codes in a byte's upper half were multiplied as 16 q
-        if (quarter < rows && n < a.n) store_product(a, static_cast<int64_t>(quarter) * a.n + n, y * (kInt ? a.x_scales[quarter] * 0.0625f : kWidenedUnit<XT>));
+        if (quarter < rows && n < a.n) store_product(a, static_cast<int64_t>(quarter) * a.n + n, y * (kInt ? a.x_scales[quarter] : kWidenedUnit<XT>));
     }
 }
 
@@ -626,18 +638,21 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
                         constexpr int g = decltype(gc)::value, kSteps = 4 / NG;      // words of a lane in a group
                         const float f = static_cast<float>(s[t][u / RUN][u % RUN * NG + g]);
                         if constexpr (kInt) {
+                            // 16 q costs a product more for each of 4 MT sums, q four instructions more for each word: 64 rows in groups of 32 take 78 us
+                            // with q (8192 x 22528, fp32 scales) and 84 with 16 q
+                            constexpr bool kSixteen = MT <= kSteps;
                             i32x4 acc[MT];
 #pragma unroll
                             for (int m = 0; m < MT; ++m) acc[m] = i32x4{0, 0, 0, 0};
                             if constexpr (GS == 5) {
-                                const u32x2 cb{(v[g] << 4) & 0xf0f0f0f0u, v[g] & 0xf0f0f0f0u};
+                                const u32x2 cb{low_codes<kSixteen>(v[g]), high_codes<kSixteen>(v[g])};
 #pragma unroll
                                 for (int m = 0; m < MT; ++m)
                                     acc[m] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, xa[u][0][m][g]), __builtin_bit_cast(long, cb), acc[m], 0, 0, 0);
                             } else {
                                 each<kSteps / 2>([&](auto jc) {
                                     constexpr int j = g * kSteps + 2 * decltype(jc)::value;
-                                    const u32x4 cb{(v[j] << 4) & 0xf0f0f0f0u, v[j] & 0xf0f0f0f0u, (v[j + 1] << 4) & 0xf0f0f0f0u, v[j + 1] & 0xf0f0f0f0u};
+                                    const u32x4 cb{low_codes<kSixteen>(v[j]), high_codes<kSixteen>(v[j]), low_codes<kSixteen>(v[j + 1]), high_codes<kSixteen>(v[j + 1])};
 #pragma unroll
                                     for (int m = 0; m < MT; ++m) {
                                         const frag lo = xa[u][0][m][j], hi = xa[u][0][m][j + 1];
@@ -649,7 +664,7 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
 #pragma unroll
                             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) y[t][m][i] = fmaf(static_cast<float>(acc[m][i]), f, y[t][m][i]);
+                                for (int i = 0; i < 4; ++i) y[t][m][i] = fmaf(static_cast<float>(acc[m][i]) * (kSixteen ? 0.0625f : 1.0f), f, y[t][m][i]);
                         } else {
                             f32x4 acc[MT];
 #pragma unroll
@@ -695,7 +710,7 @@ __global__ __launch_bounds__(512) void matvec4_many_kernel(MatvecArgs a) {
                 const int64_t at = static_cast<int64_t>(row0 + row) * a.n + n;
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
-                    if (row + r < rows) store_product(a, at + static_cast<int64_t>(r) * a.n, v[r] * (kInt ? a.x_scales[row0 + row + r] * 0.0625f : kWidenedUnit<XT>));
+                    if (row + r < rows) store_product(a, at + static_cast<int64_t>(r) * a.n, v[r] * (kInt ? a.x_scales[row0 + row + r] : kWidenedUnit<XT>));
             }
             if constexpr (kBuffers == 1) __syncthreads();
 #pragma unroll

@@ -712,3 +712,18 @@ def test_matvec_4bit_columns_of_the_smallest_magnitudes(dev, rows):
         s = torch.full((20, 2), scale)
         got = lowbit.matvec_4bit(x.to(xt).to(dev), ref.pack(codes).to(dev), s.to(dev), None, F32)
         assert torch.equal(got.cpu().double(), x @ (codes.double() * scale).T)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 5, 20, 40])
+def test_matvec_4bit_int8_rows_between_large_and_small_scales(dev, rows):
+    # sums of code x scale up to fp32's last power of two and row scales down to its smallest normal number, and the other way round
+    for group in (32, 64, 128):
+        for scale, x_scale in ((2.0 ** 110, 2.0 ** -126), (2.0 ** -126, 2.0 ** 110), (2.0 ** 110, 1.5 * 2.0 ** -130)):
+            announce(f"matvec {rows} x 128 x 20 group {group} int8, scales {scale:g} and {x_scale:g}")
+            codes = torch.full((20, 128), 7, dtype=torch.int8)
+            codes[1::2] = -8
+            x = torch.full((rows, 128), 127, dtype=I8)
+            s, xs = torch.full((20, 128 // group), scale), torch.full((rows,), x_scale)
+            got = lowbit.matvec_4bit(x.to(dev), ref.pack(codes).to(dev), s.to(dev), xs.to(dev))
+            want = (x.double() @ (codes.double() * scale).T) * xs.double().unsqueeze(-1)      # 17 bits at most: exact
+            assert torch.equal(got.cpu().double(), want)
