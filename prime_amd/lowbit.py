@@ -15,13 +15,14 @@ The norm stands in for src/zeroband/models/norms.py:128,176; the others have no 
 
 Registered as ``torch.library`` ops in the namespace ``prime_lowbit`` (``prime::`` is the closed set
 of the compression path), for ROCm tensors only: a CPU tensor reaches no kernel and the dispatcher
-raises.  The functions below take plain CUDA tensors straight to the C ABI and everything else (fake,
-traced, CPU tensors) to the dispatcher.  Every call runs on the current stream of its tensors'
+raises.  The functions below take plain CUDA tensors of an eager call straight to the C ABI and everything
+else (fake and CPU tensors, tensor subclasses, calls under ``torch.compile``, a tracer, a dispatch mode or a
+``torch.func`` transform, forward-mode duals) to the dispatcher.  Every call runs on the current stream of its tensors'
 device, allocates its outputs (and the backward pass its scratch) from torch's caching allocator,
 and can be captured into a HIP graph.
 
-Codes carry no gradient, so a call whose inputs require one is refused while gradients are being
-recorded; inside a ``torch.autograd.Function`` (or ``torch.no_grad()``) pair
+Codes carry no gradient, so a call whose inputs require one, or carry a tangent, is refused while gradients
+are being recorded; inside a ``torch.autograd.Function`` (or ``torch.no_grad()``) pair
 ``add_rms_norm_quantize`` with ``rms_norm_quantize_backward``.
 """
 from __future__ import annotations
@@ -29,6 +30,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _on, _stream
@@ -56,6 +58,10 @@ def _fail(name: str, what: str):
     raise RuntimeError(f"{name}: {what}")
 
 
+def _no_gradient(name: str):
+    _fail(name, "records no gradient; call it inside a torch.autograd.Function or under torch.no_grad()")
+
+
 def _check_inputs(name: str, dev: torch.device, *tensors: Optional[torch.Tensor]) -> None:
     """One device, and no gradient asked of an op that records none."""
     grads = torch.is_grad_enabled()
@@ -65,7 +71,7 @@ def _check_inputs(name: str, dev: torch.device, *tensors: Optional[torch.Tensor]
         if t.device != dev:
             _fail(name, f"all tensors must live on one device, got {t.device} beside {dev}")
         if grads and t.requires_grad:
-            _fail(name, "records no gradient; call it inside a torch.autograd.Function or under torch.no_grad()")
+            _no_gradient(name)
 
 
 def _wants_gradient(*tensors: Optional[torch.Tensor]) -> bool:
@@ -322,6 +328,27 @@ _LIB.impl("dequantize_4bit", _dequantize_4bit, "CUDA")
 _LIB.impl("matvec_4bit", _matvec_4bit, "CUDA")
 
 
+# What the dispatcher asks first where gradients could be recorded: it refuses, in reverse and in forward mode, what the ops could only drop.
+def _refusal_of_gradients(name: str):
+    op = getattr(torch.ops.prime_lowbit, name).default
+
+    def kernel(*args, **kwargs):
+        reverse = torch.is_grad_enabled()
+        forward = forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()
+        if reverse or forward:
+            for t in (*args, *kwargs.values()):
+                if isinstance(t, torch.Tensor) and ((reverse and t.requires_grad) or (forward and forward_ad.unpack_dual(t).tangent is not None)):
+                    _no_gradient(name)
+        with torch._C._AutoDispatchBelowAutograd():
+            return op(*args, **kwargs)
+
+    return kernel
+
+
+for _name in ("rms_norm_quantize", "add_rms_norm_quantize", "rms_norm_quantize_backward", "quantize_4bit", "dequantize_4bit", "matvec_4bit"):
+    _LIB.impl(_name, _refusal_of_gradients(_name), "Autograd")
+
+
 # shape-only implementations so the ops can be traced: the same checks, no kernel
 @torch.library.register_fake("prime_lowbit::rms_norm_quantize")
 def _(x, weight, eps=1e-6, dtype=torch.int8):
@@ -364,8 +391,23 @@ def _(x, packed, scales, x_scales=None, dtype=None):
     return x.new_empty(x.shape[:-1] + (n,), dtype=dtype)
 
 
-def _plain(t: torch.Tensor) -> bool:
-    return type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda
+def _eager() -> bool:
+    """No compiler, tracer, dispatch mode, ``torch.func`` transform or forward-mode level that would have to see the op."""
+    return not (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._functorch.peek_interpreter_stack() is not None
+                or forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None)
+
+
+def _plain(first: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:
+    """An eager call on tensors whose memory holds their values."""
+    if not (_eager() and first.is_cuda and type(first) in _PLAIN and not first.is_neg()):
+        return False
+    for t in others:
+        if t is not None and (type(t) not in _PLAIN or t.is_neg()):
+            return False
+    return True
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, dtype: torch.dtype = torch.int8):
@@ -375,7 +417,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, 
 
     The scale is the largest of a row over 127 (448), and a code the nearest number of its type, ties to
     even, exactly.  A row that holds a value that is not finite gets scale NaN and codes 0."""
-    if _plain(x):
+    if _plain(x, weight):
         return _rms_norm_quantize(x, weight, eps, dtype)
     return torch.ops.prime_lowbit.rms_norm_quantize(x, weight, eps, dtype)
 
@@ -383,7 +425,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, 
 def add_rms_norm_quantize(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, dtype: torch.dtype = torch.int8):
     """``rms_norm_quantize`` of ``hidden = x + residual`` (one type and shape; the sum is rounded to that type before it is
     normalised): (codes, scales, hidden, inv_rms)."""
-    if _plain(x):
+    if _plain(x, residual, weight):
         return _add_rms_norm_quantize(x, residual, weight, eps, dtype)
     return torch.ops.prime_lowbit.add_rms_norm_quantize(x, residual, weight, eps, dtype)
 
@@ -393,7 +435,7 @@ def rms_norm_quantize_backward(grad: torch.Tensor, hidden: torch.Tensor, weight:
     """Gradients of the norm, straight through the rounding to codes: (grad_x, grad_weight) from ``grad``, that of
     ``codes * scales``, and ``grad_hidden``, that of the stored sum (optional).  ``hidden`` is what the forward pass returned
     (its ``x`` without a residual); grad_x is the gradient of ``x`` and of the residual alike."""
-    if _plain(hidden):
+    if _plain(hidden, grad, weight, inv_rms, grad_hidden):
         return _rms_norm_quantize_backward(grad, hidden, weight, inv_rms, grad_hidden)
     return torch.ops.prime_lowbit.rms_norm_quantize_backward(grad, hidden, weight, inv_rms, grad_hidden)
 
@@ -412,7 +454,7 @@ def quantize_4bit(weight: torch.Tensor, group_size: int = 128, scale_dtype: torc
 def dequantize_4bit(packed: torch.Tensor, scales: torch.Tensor, columns: Optional[int] = None, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The matrix [n, columns] that 4-bit codes stand for: ``code * scale`` in 32 bits, rounded to ``dtype``.  ``columns``: the
     row length before it was filled up to whole groups (default: all that the codes hold)."""
-    if _plain(packed):
+    if _plain(packed, scales):
         return _dequantize_4bit(packed, scales, columns, dtype)
     return torch.ops.prime_lowbit.dequantize_4bit(packed, scales, columns, dtype)
 
@@ -429,6 +471,6 @@ def matvec_4bit(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, x_s
     group's scale is applied.  At most 2^26 outputs; rows of ``packed`` and ``scales`` may be slices of a larger matrix,
     less than 4 GiB apart.  Meant for the rows of a decoding step; for hundreds of rows take ``dequantize_4bit`` and a library
     product."""
-    if _plain(x):
+    if _plain(x, packed, scales, x_scales):
         return _matvec_4bit(x, packed, scales, x_scales, dtype)
     return torch.ops.prime_lowbit.matvec_4bit(x, packed, scales, x_scales, dtype)

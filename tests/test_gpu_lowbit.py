@@ -727,3 +727,64 @@ def test_matvec_4bit_int8_rows_between_large_and_small_scales(dev, rows):
             got = lowbit.matvec_4bit(x.to(dev), ref.pack(codes).to(dev), s.to(dev), xs.to(dev))
             want = (x.double() @ (codes.double() * scale).T) * xs.double().unsqueeze(-1)      # 17 bits at most: exact
             assert torch.equal(got.cpu().double(), want)
+
+
+def test_compiled_traced_and_transformed_calls_reach_the_ops(dev):
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    g = gen("traced")
+    x, r = rows_like_activations(g, 6, 200, F32).to(dev), rows_like_activations(g, 6, 200, F32).to(dev)
+    w = (1 + 0.1 * torch.randn(200, generator=g)).to(dev)
+
+    def step(x, r, w):
+        codes, scales, hidden, inv = lowbit.add_rms_norm_quantize(x, r, w)
+        packed, s = lowbit.quantize_4bit(hidden, 32)
+        y = lowbit.matvec_4bit(codes, packed, s, scales)
+        return (y, lowbit.dequantize_4bit(packed, s, 200)) + lowbit.rms_norm_quantize_backward(hidden, x, w, inv)
+
+    want = step(x, r, w)
+    torch._dynamo.reset()
+    got = torch.compile(step, backend="eager", fullgraph=True)(x, r, w)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = make_fx(step)(x, r, w)
+    assert sum("prime_lowbit" in str(n.target) for n in graph.graph.nodes) == 5
+    assert all(torch.equal(a, b) for a, b in zip(graph(r, x, w), step(r, x, w)))          # not what it was traced with
+    # a call for each row, and the calls that would drop a gradient
+    for a, b in zip(torch.vmap(lambda t: lowbit.rms_norm_quantize(t, w))(x), lowbit.rms_norm_quantize(x, w)):
+        assert torch.equal(a, b)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no gradient"):
+        lowbit.rms_norm_quantize(forward_ad.make_dual(x, r), w)
+    for transform in (lambda: torch.func.grad(lambda t: lowbit.rms_norm_quantize(t, w)[1].sum())(x),
+                      lambda: torch.func.jvp(lambda t: lowbit.rms_norm_quantize(t, w)[1], (x,), (r,))):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            transform()
+    # a view whose memory holds the negated values
+    z = torch.complex(x, r).contiguous()
+    neg = torch._neg_view(x)
+    assert torch.equal(lowbit.rms_norm_quantize(neg, w)[0], lowbit.rms_norm_quantize(-x, w)[0])
+    assert torch.equal(lowbit.add_rms_norm_quantize(x, z.conj().imag, w)[2], x - r)
+
+
+def test_the_pair_in_an_autograd_function_compiles(dev):
+    class Norm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, weight):
+            codes, scales, inv = lowbit.rms_norm_quantize(x, weight)
+            ctx.save_for_backward(x, weight, inv)
+            return codes.float() * scales.unsqueeze(-1)
+
+        @staticmethod
+        def backward(ctx, grad):
+            return lowbit.rms_norm_quantize_backward(grad, *ctx.saved_tensors)
+
+    g = gen("compiled pair")
+    base, w, dy = rows_like_activations(g, 9, 130, F32).to(dev), torch.ones(130, device=dev), torch.randn(9, 130, generator=g).to(dev)
+    torch._dynamo.reset()
+    results = []
+    for fn in (Norm.apply, torch.compile(lambda x, w: Norm.apply(x, w), backend="aot_eager", fullgraph=True)):
+        x, weight = base.clone().requires_grad_(), w.clone().requires_grad_()
+        y = fn(x, weight)
+        y.backward(dy)
+        results.append((y.detach(), x.grad, weight.grad))
+    assert all(torch.equal(a, b) for a, b in zip(*results))

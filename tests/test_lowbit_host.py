@@ -176,3 +176,92 @@ def test_outer_weights_come_under_their_own_names(monkeypatch):
         got = state.outer_weights_4bit(wrapped)
         assert got.keys() == {prefix + n for n in want}
         assert all(torch.equal(got[prefix + n][0], w) for n, w in want.items())
+
+
+def test_only_eager_calls_pass_the_dispatcher_by():
+    """Whatever has to see an op (a compiler, a tracer, a mode, a transform) is noticed, though its tensors are plain by their type."""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    seen = {}
+
+    def look(name):
+        def f(t):
+            seen[name] = lowbit._eager()
+            return t * 2
+        return f
+
+    x = torch.randn(2, 3)
+    look("plain")(x)
+    with torch.no_grad():
+        look("no_grad")(x)
+    make_fx(look("make_fx"))(x)
+    torch.vmap(look("vmap"))(x)
+    torch.func.grad(lambda t: look("grad")(t).sum())(x)
+    torch.func.jvp(look("jvp"), (x,), (x,))
+    torch.jit.trace(look("trace"), x, check_trace=False)
+    with forward_ad.dual_level():
+        look("dual")(forward_ad.make_dual(x, x))
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    with Mode():
+        look("mode")(x)
+    look("plain again")(x)
+    assert seen == {"plain": True, "no_grad": True, "make_fx": False, "vmap": False, "grad": False, "jvp": False, "trace": False, "dual": False,
+                    "mode": False, "plain again": True}
+    compiled = torch.compile(lambda t: t + 1 if lowbit._eager() else t - 1, backend="eager", fullgraph=True)
+    assert torch.equal(compiled(x), x - 1)
+
+
+def _ops_of(fn, *args):
+    """The ops in the one graph that ``fn`` is compiled to (which is not run)."""
+    names = []
+
+    def backend(gm, inputs):
+        names.extend(str(n.target) for n in gm.graph.nodes if n.op == "call_function" and "prime_lowbit" in str(n.target))
+        outputs = [n for n in gm.graph.nodes if n.op == "output"][0].args[0]
+        return lambda *a: tuple(torch.zeros(n.meta["example_value"].shape, dtype=n.meta["example_value"].dtype) for n in outputs)
+
+    torch._dynamo.reset()
+    torch.compile(fn, backend=backend, fullgraph=True)(*args)
+    return names
+
+
+def test_every_function_compiles_to_its_op_in_one_graph():
+    x, w, inv = torch.randn(3, 64), torch.ones(64), torch.ones(3)
+    packed, s = torch.zeros(4, 32, dtype=torch.uint8), torch.ones(4, 1)
+    for name, fn, args in (("rms_norm_quantize", lambda a, b: lowbit.rms_norm_quantize(a, b), (x, w)),
+                           ("add_rms_norm_quantize", lambda a, b: lowbit.add_rms_norm_quantize(a, a, b, 1e-5, torch.float8_e4m3fn), (x, w)),
+                           ("rms_norm_quantize_backward", lambda a, b, c: lowbit.rms_norm_quantize_backward(a, a, b, c), (x, w, inv)),
+                           ("quantize_4bit", lambda a: lowbit.quantize_4bit(a, 32), (x,)),
+                           ("dequantize_4bit", lambda a, b: lowbit.dequantize_4bit(a, b, 60), (packed, s)),
+                           ("matvec_4bit", lambda a, b, c: lowbit.matvec_4bit(a, b, c), (x, packed, s))):
+        ops = _ops_of(fn, *args)
+        assert len(ops) == 1 and name in ops[0], (name, ops)
+
+
+def test_gradients_are_refused_by_the_dispatcher_in_both_modes():
+    from torch.autograd import forward_ad
+
+    x, w = torch.randn(3, 64, device="meta"), torch.ones(64, device="meta")
+    packed, s = torch.zeros(4, 32, dtype=torch.uint8, device="meta"), torch.ones(4, 1, device="meta")
+    calls = (lambda t: lowbit.rms_norm_quantize(t, w), lambda t: lowbit.add_rms_norm_quantize(x, t, w),
+             lambda t: lowbit.rms_norm_quantize_backward(t, x, w, torch.ones(3, device="meta")), lambda t: lowbit.quantize_4bit(t, 64),
+             lambda t: lowbit.matvec_4bit(t, packed, s), lambda t: lowbit.dequantize_4bit(packed, t[:, :1].repeat(2, 1)[:4].contiguous()))
+    for call in calls:
+        call(x)
+        with torch.no_grad():
+            call(x.clone().requires_grad_())
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(x.clone().requires_grad_())
+        with forward_ad.dual_level():
+            call(x)
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call(forward_ad.make_dual(x, x))
+        for transform in (lambda: torch.func.grad(lambda t: torch.utils._pytree.tree_leaves(call(t))[-1].float().sum())(x), lambda: torch.func.jvp(call, (x,), (x,))):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                transform()
