@@ -112,6 +112,23 @@ def _check_norm(name: str, x: torch.Tensor, weight: torch.Tensor, like: Tuple[Tu
     return dim
 
 
+def _check_norm_call(name: str, x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float, dtype: torch.dtype) -> None:
+    _check_norm(name, x, weight, (("residual", residual),))
+    if dtype not in CODE_DTYPES:
+        _fail(name, f"codes are torch.int8 or torch.float8_e4m3fn, got {dtype}")
+    if not eps >= 0.0:
+        _fail(name, f"eps must not be negative, got {eps}")
+    _check_inputs(name, x.device, x, residual, weight)
+
+
+def _check_backward_call(name: str, grad: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor, inv_rms: torch.Tensor,
+                         grad_hidden: Optional[torch.Tensor]) -> None:
+    _check_norm(name, hidden, weight, (("grad", grad), ("grad_hidden", grad_hidden)))
+    if inv_rms.dtype != torch.float32 or inv_rms.shape != hidden.shape[:-1]:
+        _fail(name, f"inv_rms must be Float of shape {tuple(hidden.shape[:-1])}, got {inv_rms.dtype} of {tuple(inv_rms.shape)}")
+    _check_inputs(name, hidden.device, grad, hidden, weight, inv_rms, grad_hidden)
+
+
 def _norm(name: str, x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float, dtype: torch.dtype):
     xt, wt, shape, dev = x.dtype, weight.dtype, x.shape, x.device
     # one expression for the calls that are right; the checks that say what is wrong run only for the others
@@ -119,12 +136,7 @@ def _norm(name: str, x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
             and dtype in CODE_DTYPES and eps >= 0.0 and weight.device == dev
             and (residual is None or (residual.shape == shape and residual.dtype is xt and residual.device == dev))
             and not _wants_gradient(x, weight, residual)):
-        _check_norm(name, x, weight, (("residual", residual),))
-        if dtype not in CODE_DTYPES:
-            _fail(name, f"codes are torch.int8 or torch.float8_e4m3fn, got {dtype}")
-        if not eps >= 0.0:
-            _fail(name, f"eps must not be negative, got {eps}")
-        _check_inputs(name, dev, x, residual, weight)
+        _check_norm_call(name, x, residual, weight, eps, dtype)
     dim = shape[-1]
     lib = _lib.load()
     with _on(dev):
@@ -166,10 +178,7 @@ def _rms_norm_quantize_backward(grad, hidden, weight, inv_rms, grad_hidden=None)
             and grad.device == dev and weight.device == dev and inv_rms.device == dev
             and (grad_hidden is None or (grad_hidden.shape == shape and grad_hidden.dtype is ht and grad_hidden.device == dev))
             and not _wants_gradient(grad, hidden, weight, inv_rms, grad_hidden)):
-        _check_norm(name, hidden, weight, (("grad", grad), ("grad_hidden", grad_hidden)))
-        if inv_rms.dtype != torch.float32 or inv_rms.shape != shape[:-1]:
-            _fail(name, f"inv_rms must be Float of shape {tuple(shape[:-1])}, got {inv_rms.dtype} of {tuple(inv_rms.shape)}")
-        _check_inputs(name, dev, grad, hidden, weight, inv_rms, grad_hidden)
+        _check_backward_call(name, grad, hidden, weight, inv_rms, grad_hidden)
     dim = shape[-1]
     lib = _lib.load()
     with _on(dev):
@@ -202,23 +211,23 @@ def _groups(name: str, k: int, group_size: int) -> int:
     return -(-k // group_size)
 
 
-def _check_matrix(name: str, weight: torch.Tensor) -> None:
+def _check_quantize(name: str, weight: torch.Tensor, group_size: int, scale_dtype: torch.dtype) -> Tuple[int, int, int]:
+    """(rows, columns, groups of a row) of a matrix to be packed."""
+    if weight.dtype not in _FLOATS:
+        _fail(name, f"expected a Float, BFloat16 or Half weight but found {weight.dtype}")
     if weight.dim() != 2 or weight.shape[1] < 1 or weight.shape[1] > MAX_DIM:
         _fail(name, f"a matrix with rows of 1 to 2^30 weights is needed, got shape {tuple(weight.shape)}")
+    if scale_dtype not in _SCALES:
+        _fail(name, f"scales are torch.bfloat16 or torch.float32, got {scale_dtype}")
+    if _wants_gradient(weight):
+        _no_gradient(name)
+    n, k = weight.shape
+    return n, k, _groups(name, k, group_size)
 
 
 def _quantize_4bit(weight, group_size=128, scale_dtype=torch.bfloat16):
-    name = "quantize_4bit"
-    if weight.dtype not in _FLOATS:
-        _fail(name, f"expected a Float, BFloat16 or Half weight but found {weight.dtype}")
-    _check_matrix(name, weight)
-    if scale_dtype not in _SCALES:
-        _fail(name, f"scales are torch.bfloat16 or torch.float32, got {scale_dtype}")
-    n, k = weight.shape
-    groups = _groups(name, k, group_size)
+    n, k, groups = _check_quantize("quantize_4bit", weight, group_size, scale_dtype)
     dev = weight.device
-    if _wants_gradient(weight):
-        _check_inputs(name, dev, weight)
     lib = _lib.load()
     with _on(dev):
         w, stride = _rows(weight, k)
@@ -260,14 +269,18 @@ def _dense_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() or t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _dequantize_4bit(packed, scales, columns=None, dtype=torch.float32):
-    name = "dequantize_4bit"
-    n, k, group = _check_packed(name, packed, scales, columns)
+def _check_dequantize(name: str, packed: torch.Tensor, scales: torch.Tensor, columns: Optional[int], dtype: torch.dtype) -> Tuple[int, int, int]:
+    sizes = _check_packed(name, packed, scales, columns)
     if dtype not in _FLOATS:
         _fail(name, f"weights are Float, BFloat16 or Half, got {dtype}")
+    if scales.device != packed.device or _wants_gradient(scales):
+        _check_inputs(name, packed.device, packed, scales)
+    return sizes
+
+
+def _dequantize_4bit(packed, scales, columns=None, dtype=torch.float32):
+    n, k, group = _check_dequantize("dequantize_4bit", packed, scales, columns, dtype)
     dev = packed.device
-    if scales.device != dev or _wants_gradient(scales):
-        _check_inputs(name, dev, packed, scales)
     lib = _lib.load()
     with _on(dev):
         packed, scales = _dense_rows(packed), _dense_rows(scales)
@@ -294,15 +307,15 @@ def _check_matvec(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torc
         dtype = torch.float32 if x.dtype == torch.int8 else x.dtype
     if dtype not in _FLOATS:
         _fail(name, f"products are Float, BFloat16 or Half, got {dtype}")
+    dev = x.device
+    if packed.device != dev or scales.device != dev or (x_scales is not None and x_scales.device != dev) or _wants_gradient(x, scales, x_scales):
+        _check_inputs(name, dev, x, packed, scales, x_scales)
     return n, k, group, dtype
 
 
 def _matvec_4bit(x, packed, scales, x_scales=None, dtype=None):
-    name = "matvec_4bit"
-    n, k, group, dtype = _check_matvec(name, x, packed, scales, x_scales, dtype)
+    n, k, group, dtype = _check_matvec("matvec_4bit", x, packed, scales, x_scales, dtype)
     dev = x.device
-    if packed.device != dev or scales.device != dev or (x_scales is not None and x_scales.device != dev) or _wants_gradient(x, scales, x_scales):
-        _check_inputs(name, dev, x, packed, scales, x_scales)
     lib = _lib.load()
     with _on(dev):
         x2, stride = _rows(x, k)
@@ -352,14 +365,14 @@ for _name in ("rms_norm_quantize", "add_rms_norm_quantize", "rms_norm_quantize_b
 # shape-only implementations so the ops can be traced: the same checks, no kernel
 @torch.library.register_fake("prime_lowbit::rms_norm_quantize")
 def _(x, weight, eps=1e-6, dtype=torch.int8):
-    _check_norm("rms_norm_quantize", x, weight)
+    _check_norm_call("rms_norm_quantize", x, None, weight, eps, dtype)
     lead = x.shape[:-1]
     return x.new_empty(x.shape, dtype=dtype), x.new_empty(lead, dtype=torch.float32), x.new_empty(lead, dtype=torch.float32)
 
 
 @torch.library.register_fake("prime_lowbit::add_rms_norm_quantize")
 def _(x, residual, weight, eps=1e-6, dtype=torch.int8):
-    _check_norm("add_rms_norm_quantize", x, weight, (("residual", residual),))
+    _check_norm_call("add_rms_norm_quantize", x, residual, weight, eps, dtype)
     lead = x.shape[:-1]
     return (x.new_empty(x.shape, dtype=dtype), x.new_empty(lead, dtype=torch.float32), x.new_empty(x.shape),
             x.new_empty(lead, dtype=torch.float32))
@@ -367,21 +380,19 @@ def _(x, residual, weight, eps=1e-6, dtype=torch.int8):
 
 @torch.library.register_fake("prime_lowbit::rms_norm_quantize_backward")
 def _(grad, hidden, weight, inv_rms, grad_hidden=None):
-    _check_norm("rms_norm_quantize_backward", hidden, weight, (("grad", grad), ("grad_hidden", grad_hidden)))
+    _check_backward_call("rms_norm_quantize_backward", grad, hidden, weight, inv_rms, grad_hidden)
     return hidden.new_empty(hidden.shape), weight.new_empty(weight.shape)
 
 
 @torch.library.register_fake("prime_lowbit::quantize_4bit")
 def _(weight, group_size=128, scale_dtype=torch.bfloat16):
-    _check_matrix("quantize_4bit", weight)
-    n, k = weight.shape
-    groups = _groups("quantize_4bit", k, group_size)
+    n, _, groups = _check_quantize("quantize_4bit", weight, group_size, scale_dtype)
     return weight.new_empty((n, groups * group_size // 2), dtype=torch.uint8), weight.new_empty((n, groups), dtype=scale_dtype)
 
 
 @torch.library.register_fake("prime_lowbit::dequantize_4bit")
 def _(packed, scales, columns=None, dtype=torch.float32):
-    n, k, _ = _check_packed("dequantize_4bit", packed, scales, columns)
+    n, k, _ = _check_dequantize("dequantize_4bit", packed, scales, columns, dtype)
     return packed.new_empty((n, k), dtype=dtype)
 
 

@@ -265,3 +265,26 @@ def test_gradients_are_refused_by_the_dispatcher_in_both_modes():
         for transform in (lambda: torch.func.grad(lambda t: torch.utils._pytree.tree_leaves(call(t))[-1].float().sum())(x), lambda: torch.func.jvp(call, (x,), (x,))):
             with pytest.raises(RuntimeError, match="no gradient"):
                 transform()
+
+
+@pytest.mark.parametrize("case", range(len(_refusals())))
+def test_what_a_call_refuses_its_trace_refuses(case):
+    """The shape-only implementations make the checks of the ones that launch: a graph is not made of calls that cannot run."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    what, call, args = _refusals()[case]
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        args = tuple(mode.from_tensor(a) if isinstance(a, torch.Tensor) else a for a in args)
+        with pytest.raises(RuntimeError, match=what):
+            getattr(torch.ops.prime_lowbit, call.__name__[1:])(*args)
+
+
+def test_tensors_on_two_devices_are_refused_in_a_trace():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x, w = torch.empty(3, 64, device="meta"), torch.empty(64)
+        packed, s = torch.empty(4, 32, dtype=torch.uint8, device="meta"), torch.empty(4, 1)
+        for call in (lambda: lowbit.rms_norm_quantize(x, w), lambda: lowbit.dequantize_4bit(packed, s), lambda: lowbit.matvec_4bit(x, packed, s)):
+            with pytest.raises(RuntimeError, match="device"):
+                call()
