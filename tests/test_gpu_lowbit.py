@@ -788,3 +788,14 @@ def test_the_pair_in_an_autograd_function_compiles(dev):
         y.backward(dy)
         results.append((y.detach(), x.grad, weight.grad))
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 24, 64])
+@pytest.mark.parametrize("xt", FLOATS, ids=NAMES.get)
+def test_matvec_4bit_of_floating_rows_closely(dev, rows, xt):
+    # within the roundings of the terms' own sums: rows in stretches and in several visits, ragged ends, every size of group
+    for n, k, group, st in ((48, 20000, 128, BF16), (15, 5604, 32, F32), (600, 6000, 64, BF16), (2090, 4300, 128, F32), (33, 1999, 32, BF16), (4099, 130, 64, F32)):
+        g = gen("closely", rows, str(xt), n, k, group)
+        announce(f"matvec {rows} x {k} x {n} group {group} {xt}, closely")
+        codes, s = four_bit(g, n, k, group, st)
+        check_matvec_closely(dev, rows_like_activations(g, rows, k, F32).to(xt), codes, s, k)

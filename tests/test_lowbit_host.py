@@ -288,3 +288,23 @@ def test_tensors_on_two_devices_are_refused_in_a_trace():
         for call in (lambda: lowbit.rms_norm_quantize(x, w), lambda: lowbit.dequantize_4bit(packed, s), lambda: lowbit.matvec_4bit(x, packed, s)):
             with pytest.raises(RuntimeError, match="device"):
                 call()
+
+
+@pytest.mark.parametrize("n, k, group", [(48, 20000, 128), (15, 5604, 32), (60, 6000, 64), (20, 4300, 128)])
+@pytest.mark.parametrize("xt", [torch.bfloat16, torch.float16, torch.float32])
+def test_the_bound_of_products_notices_lost_columns(n, k, group, xt):
+    # 128 columns left out, or one column met with its neighbour's code, of a reference that is otherwise exact
+    g = torch.Generator().manual_seed(n * k)
+    codes = torch.randint(-8, 8, (n, -(-k // group) * group), generator=g, dtype=torch.int8)
+    s = 0.01 * torch.exp(0.5 * torch.randn(n, codes.shape[1] // group, generator=g))
+    x = (torch.randn(3, k, generator=g) * torch.exp(0.3 * torch.randn(k, generator=g))).to(xt)
+    want, bound = ref.matvec(x, None, codes, s, k)[0], ref.matvec_bound(x, codes, s, k)
+    assert ref.outside(want.float(), want, bound) <= 0
+    for first in range(0, k, 128):
+        less = x.clone()
+        less[:, first:first + 128] = 0
+        assert ref.outside(ref.matvec(less, None, codes, s, k)[0].float(), want, bound) > 0
+    column = int((x[0, :-1].abs().float()).argmax())
+    wrong = codes.clone()
+    wrong[:, column] = codes[:, column + 1]
+    assert ref.outside(ref.matvec(x, None, wrong, s, k)[0].float(), want, bound) > 0
