@@ -335,7 +335,7 @@ int prime_matvec_4bit(const void* x, int64_t x_stride, int x_type, const float* 
     if (!x || !packed || !scales || !out || (x_type == PRIME_I8) != (x_scales != nullptr))
         return fail(PRIME_EINVAL, "prime_matvec_4bit: null operand, or scales without int8 rows");
     const int64_t groups = (k + group - 1) / group;
-    const int64_t scale_bytes = scale_stride * type_bytes(scale_type);
+    const int64_t scale_bytes = scale_stride > 0xffffffffLL ? scale_stride : scale_stride * type_bytes(scale_type);
     if (packed_stride > 0xffffffffLL || scale_bytes > 0xffffffffLL) return fail(PRIME_EINVAL, "prime_matvec_4bit: rows of codes or scales 4 GiB apart");
     MatvecArgs a{x, x_scales, packed, scales, out, x_stride, static_cast<uint32_t>(packed_stride), static_cast<uint32_t>(scale_bytes), static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k),
                  static_cast<int>(groups * group / 2), static_cast<int>(groups), out_type, 0, 0, 0, 0};

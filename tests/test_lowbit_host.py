@@ -308,3 +308,11 @@ def test_the_bound_of_products_notices_lost_columns(n, k, group, xt):
     wrong = codes.clone()
     wrong[:, column] = codes[:, column + 1]
     assert ref.outside(ref.matvec(x, None, wrong, s, k)[0].float(), want, bound) > 0
+
+
+def test_c_abi_refuses_scales_so_far_apart_that_their_bytes_leave_64_bits():
+    from prime_amd import _lib
+
+    lib, p = _lib.load(), ctypes.c_void_p(4096)
+    for stride in (1 << 30, 1 << 32, 1 << 61, 1 << 62, (1 << 63) - 1):
+        assert lib.prime_matvec_4bit(p, 64, 0, None, p, 32, p, stride, 2, 3, 64, 64, 0, p, 0, None) == -1, stride
