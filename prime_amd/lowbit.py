@@ -33,7 +33,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
-from .ops import _on, _stream
+from .ops import _raw_stream, _stream
 
 GROUP_SIZES = (32, 64, 128)
 CODE_DTYPES = (torch.int8, torch.float8_e4m3fn)
@@ -52,6 +52,15 @@ _LIB.define("rms_norm_quantize_backward(Tensor grad, Tensor hidden, Tensor weigh
 _LIB.define("quantize_4bit(Tensor weight, int group_size=128, ScalarType scale_dtype=bfloat16) -> (Tensor, Tensor)")
 _LIB.define("dequantize_4bit(Tensor packed, Tensor scales, int? columns=None, ScalarType dtype=float) -> Tensor")
 _LIB.define("matvec_4bit(Tensor x, Tensor packed, Tensor scales, Tensor? x_scales=None, ScalarType? dtype=None) -> Tensor")
+
+
+# looked up once: a call's time on the host is what bounds the small ones
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_compiling = torch.compiler.is_compiling
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_transform = torch._C._functorch.peek_interpreter_stack
+_tracing_state = torch._C._get_tracing_state
+_stream_of = _raw_stream if _raw_stream is not None else lambda index: _stream(torch.device("cuda", index))
 
 
 def _fail(name: str, what: str):
@@ -138,26 +147,28 @@ def _norm(name: str, x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
             and not _wants_gradient(x, weight, residual)):
         _check_norm_call(name, x, residual, weight, eps, dtype)
     dim = shape[-1]
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _norm(name, x, residual, weight, eps, dtype)
     lib = _lib.load()
-    with _on(dev):
-        lead = shape[:-1]
-        x2, xs = _rows(x, dim)
-        if not weight.is_contiguous():
-            weight = weight.contiguous()
-        codes = _like(x, dtype)
-        scales = x.new_empty(lead, dtype=torch.float32)
-        inv_rms = x.new_empty(lead, dtype=torch.float32)
-        hidden = None
-        rp = hp = None
-        rs = 0
-        if residual is not None:
-            r2, rs = _rows(residual, dim)
-            hidden = _like(x, xt)
-            rp, hp = r2.data_ptr(), hidden.data_ptr()
-        rc = lib.prime_rms_norm_quantize(x2.data_ptr(), xs, rp, rs, weight.data_ptr(), x.numel() // dim, dim, _TYPE[xt], _TYPE[wt], _TYPE[dtype], eps,
-                                         codes.data_ptr(), scales.data_ptr(), hp, inv_rms.data_ptr(), _stream(dev))
-        if rc:
-            _lib.check(rc, "prime_rms_norm_quantize")
+    lead = shape[:-1]
+    x2, xs = _rows(x, dim)
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    codes = _like(x, dtype)
+    scales = x.new_empty(lead, dtype=torch.float32)
+    inv_rms = x.new_empty(lead, dtype=torch.float32)
+    hidden = None
+    rp = hp = None
+    rs = 0
+    if residual is not None:
+        r2, rs = _rows(residual, dim)
+        hidden = _like(x, xt)
+        rp, hp = r2.data_ptr(), hidden.data_ptr()
+    rc = lib.prime_rms_norm_quantize(x2.data_ptr(), xs, rp, rs, weight.data_ptr(), x.numel() // dim, dim, _TYPE[xt], _TYPE[wt], _TYPE[dtype], eps,
+                                     codes.data_ptr(), scales.data_ptr(), hp, inv_rms.data_ptr(), _stream_of(dev.index))
+    if rc:
+        _lib.check(rc, "prime_rms_norm_quantize")
     return codes, scales, hidden, inv_rms
 
 
@@ -180,28 +191,30 @@ def _rms_norm_quantize_backward(grad, hidden, weight, inv_rms, grad_hidden=None)
             and not _wants_gradient(grad, hidden, weight, inv_rms, grad_hidden)):
         _check_backward_call(name, grad, hidden, weight, inv_rms, grad_hidden)
     dim = shape[-1]
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _rms_norm_quantize_backward(grad, hidden, weight, inv_rms, grad_hidden)
     lib = _lib.load()
-    with _on(dev):
-        g2, gs = _rows(grad, dim)
-        h2, hs = _rows(hidden, dim)
-        dp, ds = None, 0
-        if grad_hidden is not None:
-            d2, ds = _rows(grad_hidden, dim)
-            dp = d2.data_ptr()
-        if not weight.is_contiguous():
-            weight = weight.contiguous()
-        if not inv_rms.is_contiguous():
-            inv_rms = inv_rms.contiguous()
-        rows = hidden.numel() // dim
-        grad_x = _like(hidden, ht)
-        grad_weight = torch.empty_like(weight)
-        # the call's own scratch and no workspace of the stream: a captured call keeps it in its graph's memory
-        nbytes = lib.prime_rms_norm_backward_scratch_bytes(rows, dim)
-        scratch = hidden.new_empty((nbytes,), dtype=torch.uint8)
-        rc = lib.prime_rms_norm_quantize_backward(g2.data_ptr(), gs, h2.data_ptr(), hs, weight.data_ptr(), inv_rms.data_ptr(), dp, ds, rows, dim,
-                                                  _TYPE[ht], _TYPE[wt], grad_x.data_ptr(), grad_weight.data_ptr(), scratch.data_ptr(), nbytes, _stream(dev))
-        if rc:
-            _lib.check(rc, "prime_rms_norm_quantize_backward")
+    g2, gs = _rows(grad, dim)
+    h2, hs = _rows(hidden, dim)
+    dp, ds = None, 0
+    if grad_hidden is not None:
+        d2, ds = _rows(grad_hidden, dim)
+        dp = d2.data_ptr()
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    if not inv_rms.is_contiguous():
+        inv_rms = inv_rms.contiguous()
+    rows = hidden.numel() // dim
+    grad_x = _like(hidden, ht)
+    grad_weight = torch.empty_like(weight)
+    # the call's own scratch and no workspace of the stream: a captured call keeps it in its graph's memory
+    nbytes = lib.prime_rms_norm_backward_scratch_bytes(rows, dim)
+    scratch = hidden.new_empty((nbytes,), dtype=torch.uint8)
+    rc = lib.prime_rms_norm_quantize_backward(g2.data_ptr(), gs, h2.data_ptr(), hs, weight.data_ptr(), inv_rms.data_ptr(), dp, ds, rows, dim,
+                                              _TYPE[ht], _TYPE[wt], grad_x.data_ptr(), grad_weight.data_ptr(), scratch.data_ptr(), nbytes, _stream_of(dev.index))
+    if rc:
+        _lib.check(rc, "prime_rms_norm_quantize_backward")
     return grad_x, grad_weight
 
 
@@ -228,15 +241,17 @@ def _check_quantize(name: str, weight: torch.Tensor, group_size: int, scale_dtyp
 def _quantize_4bit(weight, group_size=128, scale_dtype=torch.bfloat16):
     n, k, groups = _check_quantize("quantize_4bit", weight, group_size, scale_dtype)
     dev = weight.device
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _quantize_4bit(weight, group_size, scale_dtype)
     lib = _lib.load()
-    with _on(dev):
-        w, stride = _rows(weight, k)
-        packed = weight.new_empty((n, groups * group_size // 2), dtype=torch.uint8)
-        scales = weight.new_empty((n, groups), dtype=scale_dtype)
-        rc = lib.prime_quantize_4bit(w.data_ptr(), stride, n, k, _TYPE[w.dtype], group_size, _TYPE[scale_dtype], packed.data_ptr(),
-                                     scales.data_ptr(), _stream(dev))
-        if rc:
-            _lib.check(rc, "prime_quantize_4bit")
+    w, stride = _rows(weight, k)
+    packed = weight.new_empty((n, groups * group_size // 2), dtype=torch.uint8)
+    scales = weight.new_empty((n, groups), dtype=scale_dtype)
+    rc = lib.prime_quantize_4bit(w.data_ptr(), stride, n, k, _TYPE[w.dtype], group_size, _TYPE[scale_dtype], packed.data_ptr(),
+                                 scales.data_ptr(), _stream_of(dev.index))
+    if rc:
+        _lib.check(rc, "prime_quantize_4bit")
     return packed, scales
 
 
@@ -281,14 +296,16 @@ def _check_dequantize(name: str, packed: torch.Tensor, scales: torch.Tensor, col
 def _dequantize_4bit(packed, scales, columns=None, dtype=torch.float32):
     n, k, group = _check_dequantize("dequantize_4bit", packed, scales, columns, dtype)
     dev = packed.device
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _dequantize_4bit(packed, scales, columns, dtype)
     lib = _lib.load()
-    with _on(dev):
-        packed, scales = _dense_rows(packed), _dense_rows(scales)
-        out = packed.new_empty((n, k), dtype=dtype)
-        rc = lib.prime_dequantize_4bit(packed.data_ptr(), packed.stride(0), scales.data_ptr(), scales.stride(0), n, k, group, _TYPE[scales.dtype],
-                                       out.data_ptr(), _TYPE[dtype], _stream(dev))
-        if rc:
-            _lib.check(rc, "prime_dequantize_4bit")
+    packed, scales = _dense_rows(packed), _dense_rows(scales)
+    out = packed.new_empty((n, k), dtype=dtype)
+    rc = lib.prime_dequantize_4bit(packed.data_ptr(), packed.stride(0), scales.data_ptr(), scales.stride(0), n, k, group, _TYPE[scales.dtype],
+                                   out.data_ptr(), _TYPE[dtype], _stream_of(dev.index))
+    if rc:
+        _lib.check(rc, "prime_dequantize_4bit")
     return out
 
 
@@ -316,20 +333,22 @@ def _check_matvec(name: str, x: torch.Tensor, packed: torch.Tensor, scales: torc
 def _matvec_4bit(x, packed, scales, x_scales=None, dtype=None):
     n, k, group, dtype = _check_matvec("matvec_4bit", x, packed, scales, x_scales, dtype)
     dev = x.device
+    if _current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _matvec_4bit(x, packed, scales, x_scales, dtype)
     lib = _lib.load()
-    with _on(dev):
-        x2, stride = _rows(x, k)
-        packed, scales = _dense_rows(packed), _dense_rows(scales)
-        xp = None
-        if x_scales is not None:
-            x_scales = x_scales.contiguous()
-            xp = x_scales.data_ptr()
-        shape = x.shape
-        out = x.new_empty((shape[0], n) if len(shape) == 2 else shape[:-1] + (n,), dtype=dtype)
-        rc = lib.prime_matvec_4bit(x2.data_ptr(), stride, _TYPE[x.dtype], xp, packed.data_ptr(), packed.stride(0), scales.data_ptr(), scales.stride(0),
-                                   x.numel() // k, n, k, group, _TYPE[scales.dtype], out.data_ptr(), _TYPE[dtype], _stream(dev))
-        if rc:
-            _lib.check(rc, "prime_matvec_4bit")
+    x2, stride = _rows(x, k)
+    packed, scales = _dense_rows(packed), _dense_rows(scales)
+    xp = None
+    if x_scales is not None:
+        x_scales = x_scales.contiguous()
+        xp = x_scales.data_ptr()
+    shape = x.shape
+    out = x.new_empty((shape[0], n) if len(shape) == 2 else shape[:-1] + (n,), dtype=dtype)
+    rc = lib.prime_matvec_4bit(x2.data_ptr(), stride, _TYPE[x.dtype], xp, packed.data_ptr(), packed.stride(0), scales.data_ptr(), scales.stride(0),
+                               x.numel() // k, n, k, group, _TYPE[scales.dtype], out.data_ptr(), _TYPE[dtype], _stream_of(dev.index))
+    if rc:
+        _lib.check(rc, "prime_matvec_4bit")
     return out
 
 
@@ -404,8 +423,7 @@ def _(x, packed, scales, x_scales=None, dtype=None):
 
 def _eager() -> bool:
     """No compiler, tracer, dispatch mode, ``torch.func`` transform or forward-mode level that would have to see the op."""
-    return not (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._functorch.peek_interpreter_stack() is not None
-                or forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None)
+    return not (_compiling() or _dispatch_modes() or _transform() is not None or forward_ad._current_level >= 0 or _tracing_state() is not None)
 
 
 def _plain(first: torch.Tensor, *others: Optional[torch.Tensor]) -> bool:

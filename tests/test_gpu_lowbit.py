@@ -799,3 +799,35 @@ def test_matvec_4bit_of_floating_rows_closely(dev, rows, xt):
         announce(f"matvec {rows} x {k} x {n} group {group} {xt}, closely")
         codes, s = four_bit(g, n, k, group, st)
         check_matvec_closely(dev, rows_like_activations(g, rows, k, F32).to(xt), codes, s, k)
+
+
+def test_calls_make_their_tensors_device_the_current_one(dev, monkeypatch):
+    # one device stands in for two: it counts as another one until its guard is entered
+    g = gen("another device")
+    x, w = rows_like_activations(g, 3, 96, F32).to(dev), torch.ones(96, device=dev)
+    inv = torch.ones(3, device=dev)
+    packed, s = lowbit.quantize_4bit(x, 32)
+    calls = [lambda: lowbit.rms_norm_quantize(x, w), lambda: lowbit.add_rms_norm_quantize(x, x, w), lambda: lowbit.rms_norm_quantize_backward(x, x, w, inv, x),
+             lambda: lowbit.quantize_4bit(x, 64), lambda: lowbit.dequantize_4bit(packed, s), lambda: lowbit.matvec_4bit(x, packed, s)]
+    want = [torch.utils._pytree.tree_leaves(call()) for call in calls]
+    state = {"current": 1, "entered": []}
+
+    class Guard:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            state["entered"].append(self.device)
+            state["current"] = self.device.index
+
+        def __exit__(self, *exc):
+            state["current"] = 1
+            return False
+
+    with monkeypatch.context() as m:
+        m.setattr(lowbit, "_current_device", lambda: state["current"])
+        m.setattr(torch.cuda, "device", Guard)
+        got = [torch.utils._pytree.tree_leaves(call()) for call in calls]
+    assert state["entered"] == [x.device] * len(calls)
+    for a, b in zip(got, want):
+        assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(a, b))
