@@ -399,9 +399,9 @@ int prime_dequantize_4bit(const uint8_t* packed, int64_t packed_stride, const vo
 /* Products of rows with such a matrix: out[m][i] = x_scales[m] * sum over groups of scale[i][g] * sum over the
  * group's j of code[i][j] * x[m][j], rounded once to out_type (dense rows of n).  x: PRIME_F32, PRIME_BF16 or PRIME_F16
  * rows (x_scales NULL), or PRIME_I8 codes with a scale per row, as prime_rms_norm_quantize gives them: the
- * sums within a group are then exact.  Floating rows are summed in 32 bits: up to four rows as fixed point of 31 bits
- * under the largest magnitude of each 128 columns, more rows as they are (the last bits can depend on the number of
- * rows).  A row that holds a value that is not finite has no finite products; other rows are not touched.  Magnitudes
+ * sums within a group are then exact.  Floating rows: every product with a code is exact, and sums are 32-bit, in an
+ * order that depends on the number of rows (so do the last bits); of fp32 columns what lies below 2^-133 is dropped.
+ * A row that holds a value that is not finite has no finite products; other rows are not touched.  Magnitudes
  * beyond 2^120 may overflow before their group's scale is applied.  n <= 2^26; rows of codes and of scales less than
  * 4 GiB apart.  Meant for the few rows of a decoding step; many rows (hundreds) are better served by
  * prime_dequantize_4bit and a library product. */

@@ -45,6 +45,9 @@ void with_once(bool once, F&& f) {
     else f(std::false_type{});
 }
 
+// Lanes of a row: about as few as hold it in two vectors of eight each, so that a row's reductions and barrier are few beside its loads.  67 million
+// elements of bf16 with residual, and in brackets with 256 lanes for 64 and twice as many for 256 and 512: rows of 256 elements 169 us (411), 512
+// 83 (195), 1024 74 (118), 4096 73 (80), 8192 74 (81); rows of 16384 in registers 96, in the loop 129.
 template <typename XT, typename WT, bool ONCE>
 void launch_rms_norm(const NormArgs& a, double bytes, hipStream_t st) {
     const int64_t r = a.rows;
@@ -58,7 +61,9 @@ void launch_rms_norm(const NormArgs& a, double bytes, hipStream_t st) {
     else launch(kIdRmsNorm, bytes, rms_norm_loop_kernel<XT, WT>, all, 1024, st, a);
 }
 
-// Workgroups (= partial rows of the weight's gradient) of the backward pass, and its scratch.
+// Workgroups (= partial rows of the weight's gradient) of the backward pass, and its scratch.  Lanes as above: 67 million elements of bf16, and in brackets
+// with twice as many: rows of 256 elements 246 us (444), 512 102 (169), 1024 79 (105), 2048 75 (104), 4096 71 (90), 8192 76 (72); rows of
+// 16384 in registers 72, by two kernels 123.
 constexpr int kGradRegisterDim = 16384;      // rows up to this long stay in registers
 int grad_lanes(int64_t dim) { return dim <= 1024 ? 64 : dim <= 2048 ? 128 : dim <= 4096 ? 256 : dim <= 8192 ? 512 : 1024; }
 int grad_stretches(int64_t dim) { return static_cast<int>((dim + 2047) / 2048); }
@@ -108,10 +113,13 @@ int group_shift(int group) { return group == 32 ? 5 : group == 64 ? 6 : 7; }
 // Up to four rows.
 template <typename XT, typename ST, int GS>
 void launch_matvec_few(MatvecArgs a, double bytes, hipStream_t st) {
+    // two workgroups of eight wavefronts beside each other: 4 x 8192 x 22528 fp32 34 us, with 28 KiB 39, with 112 KiB 45; of what 56 KiB do not
+    // hold whole and 112 do, bf16 29, 31 and 25
     constexpr int kMostLds = 56 << 10;
     const int held = a.rows, quads = (a.k + 511) / 512, quad_bytes = 4 * kFewBlock<XT>;
     a.tiles = (a.n + 15) / 16;
-    // wavefronts that share a tile's columns: enough for 16 wavefronts a compute unit, but not more than it has stretches
+    // wavefronts that share a tile's columns: enough for 16 wavefronts a compute unit, but not more than it has stretches (1 x 8192 x 22528 int8
+    // 21.8 us, for 8 wavefronts 27.9, for 32 24.2)
     const int wanted = cu_count() * 16;
     a.split_shift = 0;
     while (a.split_shift < 3 && (static_cast<int64_t>(a.tiles) << a.split_shift) < wanted && (2 << a.split_shift) <= quads) ++a.split_shift;
@@ -165,12 +173,13 @@ void launch_matvec_many_as(MatvecArgs a, double bytes, hipStream_t st) {
 
 // Tiles of rows, blocks of columns and tiles of outputs of a wavefront: what 256 registers hold, next to the scales of a round (which
 // groups of 32 have four times as many of).  Up to 16 rows take six blocks and half the outputs where that saves a visit: 7 x 5604 x 11263
-// fp16 groups of 32 19 us against 23; where it does not, four blocks: 16 x 8192 x 22528 bf16 33 us (eight blocks do not fit: 40).
+// fp16 groups of 32 19 us against 23 (16 since codes are widened with their sign); where it does not, four blocks: 16 x 8192 x 22528 bf16 35 us
+// (eight blocks do not fit: 40).
 template <typename XT, typename ST, int GS>
 void launch_matvec_many(const MatvecArgs& a, double bytes, hipStream_t st) {
     constexpr bool k32 = sizeof(XT) == 4, k8 = sizeof(XT) == 1, kWide = GS == 5 && sizeof(ST) == 4 && !k8;
     // more rows in tiles of 16 all the same where each tile finds a compute unit of its own: a wavefront's work is then a
-    // quarter as long, and the codes that every tile reads come from the caches: 59 x 6720 x 76 bf16 34 us with 64 rows a workgroup
+    // quarter as long, and the codes that every tile reads come from the caches: 59 x 6720 x 76 bf16 15 us, and 34 with 64 rows a workgroup
     const bool small = (static_cast<int64_t>(a.rows) + 15) / 16 * ((static_cast<int64_t>(a.n) + 31) / 32) <= cu_count();
     if (a.rows <= 16 || small) {
         if constexpr (k32) launch_matvec_many_as<XT, ST, GS, 1, 2, 2>(a, bytes, st);
@@ -188,6 +197,8 @@ void launch_matvec(const MatvecArgs& a, int group, int scale_type, double bytes,
     auto go = [&](auto gs) {
         constexpr int GS = decltype(gs)::value;
         with_scale_type(scale_type, [&](auto s) {
+            // four rows are what 16 rows of the A operand hold with three planes each: 4 x 4096 x 4096 bf16 6.3 us, by the kernel for more 9.0;
+            // 4 x 8192 x 22528 bf16 29.0 and 30.5, fp32 34.3 and 37.2
             if (a.rows <= 4) launch_matvec_few<XT, decltype(s), GS>(a, bytes, st);
             else launch_matvec_many<XT, decltype(s), GS>(a, bytes, st);
         });

@@ -216,9 +216,10 @@ __global__ __launch_bounds__(256) void group4_unpack_kernel(UnpackArgs a) {
 // quarters (four instructions for four words), so that an instruction's columns lie in one group and its sums can be scaled on
 // their own.  The rows are brought into the order in which codes come out of their words.
 //
-// Two kernels.  Up to four rows are bound by the codes' way from memory: everything is whole numbers up to the end of a group, so
-// that a word of eight codes costs three instructions (a code in the upper half of a byte is 16 q).  More rows are
-// multiplied as they are, at eight instructions a word.
+// Two kernels, one for up to four rows, which is bound by the codes' way from memory, and one for more.  In both a product with a code is exact:
+// int8 rows meet codes as bytes, and a group's sums are whole numbers; floating rows meet codes as 16-bit floating-point
+// numbers (widen_word()), and their sums are fp32, of the terms themselves: what a column adds to the error goes with its own term, and
+// a code of 0 makes it nothing.
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -258,7 +259,8 @@ __device__ __forceinline__ void transpose_quarters(u32x4& w) {
 
 // Eight codes of a word as 16-bit numbers with their sign, in the order 0 4 1 5 2 6 3 7: bf16 holds q / 16, fp16 q, both exactly.  (Beside an
 // offset, as 24 + q, a word takes eight instructions instead of thirteen and nine.  But then a column passes through the sums at up to 24 times
-// its size whatever its code is, and what a large one leaves there as rounding hides the others, and beyond 2^116 as infinity all of them.)
+// its size whatever its code is, and what a large one leaves there as rounding hides the others, and beyond 2^116 as infinity all of them.  64 x
+// 8192 x 22528 took 74 us so, with the offset's own sums read from LDS, and takes 70.)
 template <bool BF16>
 __device__ __forceinline__ u32x4 widen_word(uint32_t w) {
     if constexpr (BF16) {
@@ -385,16 +387,16 @@ __device__ __forceinline__ void rows8(const XT* __restrict__ row, int64_t i, int
     }
 }
 
-// ---- up to four rows: whole numbers up to the end of a group ----
-// int8 rows are taken as they are.  Floating rows become fixed point under the largest magnitude of each 128 columns: 31 bits, as
-// four digits of -128 .. 127 in base 256, so a value is off by at most 2^-31 of that largest (a 32-bit sum that holds both loses
-// more).  The four digits of a row are four rows of the A operand, so one matrix instruction takes them all; a group's sums are
-// exact in each digit, two digits are put together exactly in 32 bits, and the rest is fp32.
+// ---- up to four rows ----
+// The rows stay in LDS and the codes pass by.  Rows are taken as they are; the three planes of an fp32 row are three rows of the A operand, so
+// that one matrix instruction takes them all, and are added at a group's end, the smallest first.  (Floating rows were fixed point under
+// the largest of 128 columns before, four int8 digits each: 1 x 8192 x 128000 bf16 took 93 us instead of 100 in a row of calls, 4 x 8192 x 22528
+// 35 instead of 30.  But columns far below that largest were lost, also where its code is 0.)
 //
 // Bound by memory from a few thousand outputs up: 1 x 8192 x 128000 int8 92 us (5.9 TB/s; with the products taken out and the loads left
-// in 97, with loads that cover whole lines instead of 64 bytes of 16 rows 90), bf16 104 us (5.2 TB/s); the same with the codes widened to
-// bf16, at eight instructions a word beside an offset's second product, 121.  Small products are a launch and two trips
-// to memory: 1 x 2048 x 2048 4.1 us, 1 x 4096 x 4096 5.0 us.
+// in 97, with loads that cover whole lines instead of 64 bytes of 16 rows 90), bf16 107 to 114 (92 without the products; 61 % of each SIMD's
+// cycles are vector and 15 % matrix instructions).  Words of a group in sums of their own, so that no product waits for the one before, cost
+// 2 % there.  Small products are a launch and two trips to memory: 1 x 2048 x 2048 4.0 us, 1 x 4096 x 4096 4.8 us.
 
 // Bytes of a row's 128 columns in LDS: [quarter][word of a lane][plane][eight columns], so that the lanes of a quarter, which read the planes
 // of one word side by side, read consecutive bytes.  Rows lie 16 (fp32: 64) bytes off the banks' period.
@@ -527,19 +529,17 @@ __global__ __launch_bounds__(512) void matvec4_few_kernel(MatvecArgs a) {
 }
 
 // ---- more rows: 16, 32 or 64 at a time ----
-// Here the matrix cores' work grows with the rows and the rows are taken as they are: bf16 and fp16 codes are widened beside an
-// offset (widen_word()), and the sums of a group start from what the offset adds, taken off; fp32 rows are three bf16 rows,
-// which together are exact; int8 as above.  The rows stay where they are and the codes pass by: the eight wavefronts of a
-// workgroup split the columns, each holds its share of the rows in registers for all of the workgroup's outputs, and
+// Here the matrix cores' work grows with the rows: fp32 rows are three bf16 rows.  The rows stay where they are and the codes pass by: the
+// eight wavefronts of a workgroup split the columns, each holds its share of the rows in registers for all of the workgroup's outputs, and
 // only codes and scales are loaded in the loop, a round of outputs ahead.  The wavefronts' sums of a round meet in LDS.  Rows too
 // long for the registers take several visits, whose sums LDS keeps.
-// 16 x 8192 x 22528 bf16 33 us, 64 rows 74 us.  Up to 16 rows are bound by the loads' way through few, large rounds (without the
-// products 32 us, without the loads 22), 64 rows by both (58 and 68 us; without the sums' way through LDS 61 us; of each SIMD's cycles
-// 38 % are vector and 16 % matrix instructions).  What changes nothing or costs: three rounds in flight in registers of their own
-// (74 to 78 us, products of 2048 columns twice the time), the offsets' sums by fp32 matrix instructions instead of from LDS (70 to 75),
-// workgroups that begin at different columns (73 to 75).  One barrier a round is worth 3 us of the 64 rows.  The first form kept the rows
-// in LDS, with a barrier for every 256 columns: each stretch waited for its loads, 64 x 8192 x 22528 91 us, 7 x 5604 x 11263 fp16 37 us
-// against 18.
+// 16 x 8192 x 22528 bf16 35 us, 64 rows 70 us (fp32 46 and 117, int8 64 rows 63).  Up to 16 rows are bound by the loads' way through few, large
+// rounds and by the products (without the products 27 us, without the loads 24), 64 rows by the products and the sums' way through LDS
+// (without the products 41 us, without the loads 67, without the sums' way 61; of each SIMD's cycles 41 % are vector and 16 % matrix
+// instructions).  Measured before the codes were widened with their sign, when 64 rows took 74 us, and neither kept: three rounds in flight in
+// registers of their own (74 to 78 us, products of 2048 columns twice the time), workgroups that begin at different columns (73 to 75).  One
+// barrier a round was worth 3 us.  The first form kept the rows in LDS, with a barrier for every 256 columns: each stretch waited for
+// its loads, 64 x 8192 x 22528 91 us, 7 x 5604 x 11263 fp16 37 us against 18 (now 16).
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 // f(0), f(1), ... with the index a constant: registers are indexed by it.

@@ -494,10 +494,10 @@ def matvec_4bit(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, x_s
     Half, or int8 codes with ``x_scales`` (Float, one a row), as ``rms_norm_quantize`` gives them (sums within a group exact).
     ``dtype``: of the products, rounded once; default the rows' type, Float for int8 rows.
 
-    Floating rows are summed in 32 bits: up to four rows as fixed point of 31 bits under the largest magnitude of each 128
-    columns, more rows as they are, so the last bits of a row's products can depend on how many rows come with it.  A row that holds a
-    value that is not finite has no finite products (other rows are not touched), and magnitudes beyond 2^120 may overflow before their
-    group's scale is applied.  At most 2^26 outputs; rows of ``packed`` and ``scales`` may be slices of a larger matrix,
+    Floating rows are summed in 32 bits, of exact products with the codes, in an order that depends on the number of rows (so the last
+    bits of a row's products can too); of Float columns what lies below 2^-133 is dropped.  A row that holds a value that is not
+    finite has no finite products (other rows are not touched), and magnitudes beyond 2^120 may overflow before their group's scale is
+    applied.  At most 2^26 outputs; rows of ``packed`` and ``scales`` may be slices of a larger matrix,
     less than 4 GiB apart.  Meant for the rows of a decoding step; for hundreds of rows take ``dequantize_4bit`` and a library
     product."""
     if _plain(x, packed, scales, x_scales):
