@@ -49,9 +49,17 @@ def _find_first_number(s: str) -> int:
     return int(match.group()) if match else -1
 
 
-def _plain_name(name: str) -> str:
-    """A parameter's name without what ``torch.compile`` puts in front of a wrapped module's own."""
-    return ".".join(part for part in name.split(".") if part != "_orig_mod")
+def _trainable(model: nn.Module) -> List[Tuple[str, str, nn.Parameter]]:
+    """(name, name without what ``torch.compile`` and a data-parallel wrapper put in front of a module's own, parameter) of every
+    parameter that is trained."""
+    inner = getattr(model, "_orig_mod", model)
+    wrapper = "module." if isinstance(inner, (nn.parallel.DistributedDataParallel, nn.DataParallel)) else ""
+    out = []
+    for name, p in model.named_parameters():
+        if p.requires_grad:
+            own = ".".join(part for part in name.split(".") if part != "_orig_mod")
+            out.append((name, own[len(wrapper):], p))
+    return out
 
 
 class Diloco:
@@ -85,7 +93,7 @@ class Diloco:
         for name, p in items:
             if p.dtype != torch.float32 or p.device != dev or not p.data.is_contiguous():
                 raise RuntimeError(f"parameter {name}: contiguous fp32 parameters on one device are required")
-        self._names = [(_plain_name(name), p.shape) for name, p in items]
+        self._names = [(own, p.shape) for _, own, p in _trainable(model)]
         numel = sum(p.numel() for _, p in items)
         self.outer_data_flat = torch.empty(numel, device=dev, dtype=torch.float32)
         self.grad_flat = torch.zeros(numel, device=dev, dtype=torch.float32)
@@ -188,12 +196,12 @@ class Diloco:
         step agreed on, in the form ``lowbit.matvec_4bit`` takes, for evaluation or decoding between outer steps (the
         inner weights drift from them).  Parameters of other than two dimensions (norm weights, biases) are left out.
         ``model`` must have the trainable parameters that this state was built from."""
-        items = [(name, p) for name, p in model.named_parameters() if p.requires_grad]
+        items = _trainable(model)
         # by name and shape, not by number alone: with one layer frozen and another no longer, each name would get its neighbour's weights
-        if [(_plain_name(name), p.shape) for name, p in items] != self._names:
+        if [(own, p.shape) for _, own, p in items] != self._names:
             raise RuntimeError("model does not match the one this state was built from")
         out = {}
-        for (name, p), view in zip(items, self._views):
+        for (name, _, p), view in zip(items, self._views):
             if p.dim() == 2:
                 out[name] = lowbit.quantize_4bit(view[0].view(p.shape), group_size, scale_dtype)
         return out

@@ -316,3 +316,14 @@ def test_c_abi_refuses_scales_so_far_apart_that_their_bytes_leave_64_bits():
     lib, p = _lib.load(), ctypes.c_void_p(4096)
     for stride in (1 << 30, 1 << 32, 1 << 61, 1 << 62, (1 << 63) - 1):
         assert lib.prime_matvec_4bit(p, 64, 0, None, p, 32, p, stride, 2, 3, 64, 64, 0, p, 0, None) == -1, stride
+
+
+def test_outer_weights_of_a_data_parallel_model(monkeypatch):
+    from prime_amd.diloco import Diloco
+
+    monkeypatch.setattr(lowbit, "quantize_4bit", lambda w, group, dtype: (w.clone(), None))
+    model = torch.nn.Sequential(torch.nn.Linear(64, 32), torch.nn.Linear(32, 64))
+    wrapped = torch.nn.DataParallel(model)
+    for built, given, prefix in ((model, wrapped, "module."), (wrapped, model, ""), (wrapped, torch.compile(wrapped, backend="eager"), "_orig_mod.module.")):
+        got = Diloco(0.7, built).outer_weights_4bit(given)
+        assert {n: torch.equal(w, model.get_parameter(n[len(prefix):])) for n, (w, _) in got.items()} == {prefix + "0.weight": True, prefix + "1.weight": True}
